@@ -258,6 +258,102 @@ navi_status navi_linear_noalloc(const float *d_x, int32_t ldx, int32_t M, const 
                                 const float *bias, const float *residual, int32_t act, float *d_y, int32_t ldy,
                                 char *err, size_t errlen);
 
+/* ---- several requests on one pool of cache pages: drafted tokens and their attention -------
+ * No counterpart in the reference, which decodes one token of one request at a time over its own
+ * cache. For servers whose requests share one pool of cache rows and check several drafted tokens a
+ * step. A pool holds, per layer, K and V rows [n_pages * page_size][kv_dim] of two-byte elements: the
+ * layout of navi_kv_view, whose max_pos rows become pages of page_size rows (a single request's
+ * cache is a pool of one page). Request i keeps position t in row
+ * block_table[i][t / page_size] * page_size + t % page_size, its slot. One step:
+ *   navi_kv_plan         pages, slots, positions and ancestors of the step's rows
+ *   navi_kv_append       a layer's q|k|v rows: K and V into the pages, q for the attention
+ *   navi_tree_attention  a layer's attention of those rows over the pages
+ *   navi_kv_commit       the accepted rows moved to their positions, in every layer
+ * These four enqueue on `stream` (a hipStream_t of the library's device, used as it is: NULL is HIP's
+ * default stream, navi_device_stream() the library's) and return without waiting. They allocate
+ * nothing and may be captured into a graph. The calling thread's current device is left as it was. Every pointer in a struct or named d_* is
+ * device memory of the library's device; a stream of another device is refused. */
+
+typedef struct {                       /* a step's requests and rows on a pool of pages */
+    int32_t n_requests;
+    int32_t page_size;                 /* cache rows a page holds */
+    int32_t n_pages;                   /* pages of the pool; n_pages * page_size < 2^31 */
+    int32_t max_blocks;                /* columns of block_table: the most pages a request can hold */
+    int32_t n_rows;                    /* rows the row_* arrays have room for */
+    int32_t max_new;                   /* the most rows one request takes in the step */
+    int32_t *block_table;              /* [n_requests][max_blocks]: page of each block, -1 none */
+    const int32_t *n_past;             /* [n_requests]: cached rows before the step */
+    int32_t *cu_rows;                  /* [n_requests + 1]: request i's rows are cu_rows[i] .. cu_rows[i + 1] - 1 */
+    int32_t *row_slot;                 /* [n_rows]: the row's slot in the pool, -1 none */
+    int32_t *row_pos;                  /* [n_rows]: the row's position: n_past + its depth in the tree */
+    uint64_t *row_mask;                /* [n_rows]: bit a: the row sees row a of its request's step */
+} navi_kv_pages;
+
+typedef struct {
+    int32_t n_head, n_kv_head, head_dim;   /* n_head a multiple of n_kv_head; head_dim 64 or 128 */
+    int32_t kv_dtype;                      /* of the pool: NAVI_DT_F16 or NAVI_DT_BF16 */
+} navi_kv_heads;
+
+/* The step's block tables and slot maps from its lengths. Per request: d_n_new[i] rows are added to
+ * n_past[i]; d_n_new[i] < 0 says that the request has ended (no rows; its pages go back). d_parent: [n_rows],
+ * for each row the index within its request's rows of the row it follows, smaller than its own, or -1 for the
+ * last cached row: a tree of up to 64 rows a request (max_new <= 64); several rows may follow the
+ * last cached one. NULL: each row follows the one before it, any number of rows.
+ * State: d_table_in [n_requests][max_blocks], d_held_in [n_requests] (pages each request holds), a stack of free
+ * pages d_free_pages [n_pages] whose first *d_free_in entries are free. Ended requests' pages are pushed first, in
+ * order; then each request in order takes the pages that n_past + d_n_new rows need above those it holds,
+ * each from the top. Results: the arrays of `pages` but n_past; d_held [n_requests], d_free [1], and
+ * d_status [n_requests]:
+ *   0  done
+ *   1  the pages left did not suffice (a request after it that needs pages is refused too)
+ *   2  lengths out of range: negative, more than max_new rows, past max_blocks pages, held pages
+ *      outside 0 .. max_blocks, or rows past n_rows
+ *   3  a parent that does not come before its row
+ * A request with a status other than 0 keeps its pages and takes none; its rows get slot -1 (and
+ * position and mask 0 unless the status is 1). row_mask bit a is set for the row's ancestors and itself; without
+ * d_parent, for rows 0 .. min(own index, 63). Table entries past the held pages are -1; entries of row_*
+ * past the last request's rows are left as they were. d_held, d_free and pages->block_table may be
+ * d_held_in, d_free_in and d_table_in. d_scratch: 4 * n_requests words. */
+navi_status navi_kv_plan(const navi_kv_pages *pages, const int32_t *d_n_new, const int32_t *d_parent, const int32_t *d_table_in,
+                         const int32_t *d_held_in, const int32_t *d_free_in, int32_t *d_free_pages, int32_t *d_held,
+                         int32_t *d_free, int32_t *d_status, int32_t *d_scratch, void *stream, char *err, size_t errlen);
+/* A layer's projected rows into the pages: row r of d_x (f32, or the pool's type; stride ldx) holds n_head q heads, then
+ * n_kv_head k heads, then n_kv_head v heads. q and k heads are RMS-normed (d_q_norm, d_k_norm f32 [head_dim];
+ * NULL: not normed) and turned by d_rot (f32 [n_rot][head_dim]: cos | sin of position p's angles in row p,
+ * element i with element i + head_dim / 2; NULL: not turned). k and v are rounded to the pool's type and stored in
+ * row row_slot[r] of d_k and d_v (stride ld_kv); q goes to row r of d_q (f32, or the pool's type; stride ldq). Rows
+ * past cu_rows[n_requests] are left alone; a slot outside the pool stores no k and v; a position
+ * outside 0 .. n_rot - 1 stores no k and v and a q of zeros. Strides in elements; strides and
+ * pointers keep every row 16-byte aligned. d_q may be d_x with the same type and stride. */
+navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *heads, const void *d_x, int32_t x_dtype, int32_t ldx,
+                           const float *d_q_norm, const float *d_k_norm, float eps, const float *d_rot, int32_t n_rot, void *d_k,
+                           void *d_v, int32_t ld_kv, void *d_q, int32_t q_dtype, int32_t ldq, void *stream, char *err,
+                           size_t errlen);
+/* A layer's attention of the step's rows: row r of request i attends to positions 0 .. n_past[i] - 1 and
+ * to the step's rows a of its request with bit a of row_mask[r], at positions n_past[i] + a (the step's K and V are in
+ * the pages): out = softmax(scale q . K) V per head, heads grouped n_head / n_kv_head to a kv head. max_new <= 64; one
+ * row a request is ordinary single-token decode. d_q and d_out have one type: the pool's, or f32 over an f16
+ * pool (q and the probabilities then travel as f16 hi + lo pairs). What a row does not see has no influence,
+ * infinities and NaN included; a position whose page is outside the pool is not seen; a row that sees
+ * nothing gets zeros. Rows past cu_rows[n_requests] and past max_new of a request are left as they were.
+ * max_keys: the most positions a request may reach (n_past + rows), by which the work is split; longer
+ * requests are still right, but slow. d_ws: navi_tree_workspace(...) bytes, 16-byte aligned, for this call
+ * alone until it is done: calls that may overlap need a workspace each. Alignment as navi_kv_append. */
+navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads *heads, const void *d_q, int32_t q_dtype, int32_t ldq,
+                                const void *d_k, const void *d_v, int32_t ld_kv, float scale, int32_t max_keys, void *d_out,
+                                int32_t ldo, void *d_ws, size_t ws_bytes, void *stream, char *err, size_t errlen);
+/* Workspace bytes of navi_tree_attention (host only; 0 when the work is not split, or the arguments are not valid). */
+size_t navi_tree_workspace(const navi_kv_pages *pages, const navi_kv_heads *heads, int32_t max_keys);
+/* The accepted rows of each request moved into place in every layer of `kv` (n_layer, max_pos >= the pool's rows, kv_dim the
+ * row stride, a multiple of 8): with path = d_path[i][0 .. d_accept[i] - 1] (stride max_path <= 64), the indexes of accepted rows within
+ * the request's step in ascending order, position n_past[i] + j takes the K and V of position n_past[i] + path[j].
+ * d_n_past_out[i] = n_past[i] + d_accept[i] (not the array n_past itself). d_status[i]: 0, or 2 where d_accept[i] is outside
+ * 0 .. max_path, the path does not ascend or leaves the request's rows, or a page is outside the pool: nothing is moved and
+ * d_n_past_out[i] = n_past[i]. Pages past the new length stay with the request. */
+navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, const int32_t *d_path, int32_t max_path,
+                           const int32_t *d_accept, int32_t *d_n_past_out, int32_t *d_status, void *stream, char *err,
+                           size_t errlen);
+
 /* ---- vocoder: codes -> 24 kHz PCM (vocoder.h:27-55) -------------------------- */
 
 typedef struct navi_vocoder navi_vocoder;

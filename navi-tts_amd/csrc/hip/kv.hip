@@ -1,0 +1,558 @@
+// A pool of cache pages shared by several requests on gfx950 (the C ABI's navi_kv_*): a step's block
+// tables and slots from the requests' lengths, its K and V rows into the pages, and the accepted
+// drafts' rows moved into place. The attention that reads the pages is in tree.hip.
+#include "dev_common.h"
+#include "kv.h"
+
+#include <algorithm>
+
+namespace navi_amd {
+namespace kv {
+
+navi_status check_pages(const char *who, const navi_kv_pages *p, char *err, size_t errlen) {
+    if (!p || !p->block_table || !p->n_past || !p->cu_rows || (p->n_rows > 0 && (!p->row_slot || !p->row_pos || !p->row_mask))) {
+        set_err(err, errlen, "%s: null argument", who);
+        return NAVI_ERR_INVALID;
+    }
+    if (p->n_requests < 1 || p->n_requests > 65535 || p->page_size < 1 || p->n_pages < 1 || p->max_blocks < 1 || p->n_rows < 0 || p->max_new < 1 ||
+        static_cast<int64_t>(p->n_pages) * p->page_size > INT32_MAX) {
+        set_err(err, errlen, "%s: pages out of range (requests %d, page size %d, pages %d, blocks %d, rows %d, new rows %d)", who,
+                p->n_requests, p->page_size, p->n_pages, p->max_blocks, p->n_rows, p->max_new);
+        return NAVI_ERR_INVALID;
+    }
+    return NAVI_OK;
+}
+
+navi_status check_heads(const char *who, const navi_kv_heads *h, int ld_kv, char *err, size_t errlen) {
+    if (!h) {
+        set_err(err, errlen, "%s: null argument", who);
+        return NAVI_ERR_INVALID;
+    }
+    if (h->n_head < 1 || h->n_kv_head < 1 || h->n_head > 1024 || h->n_head % h->n_kv_head != 0) {
+        set_err(err, errlen, "%s: %d heads over %d kv heads", who, h->n_head, h->n_kv_head);
+        return NAVI_ERR_INVALID;
+    }
+    if ((h->head_dim != 64 && h->head_dim != 128) || (h->kv_dtype != NAVI_DT_F16 && h->kv_dtype != NAVI_DT_BF16)) {
+        set_err(err, errlen, "%s: unsupported head_dim %d or cache type %d (64 or 128; f16 or bf16)", who, h->head_dim, h->kv_dtype);
+        return NAVI_ERR_UNSUPPORTED;
+    }
+    if (ld_kv < h->n_kv_head * h->head_dim || ld_kv % 8 != 0) {
+        set_err(err, errlen, "%s: cache row stride %d for %d kv heads of %d", who, ld_kv, h->n_kv_head, h->head_dim);
+        return NAVI_ERR_INVALID;
+    }
+    return NAVI_OK;
+}
+
+// ---- plan ------------------------------------------------------------------------------------
+
+struct PlanArgs {
+    const int32_t *n_past, *n_new, *parent, *table_in, *held_in, *free_in;
+    int32_t *free_pages, *table, *held, *n_free, *status, *cu, *slot, *pos;
+    uint64_t *mask;
+    int4 *rec;                         // per request: what the fill reads (below)
+    int n, n_pages, blocks, n_rows, max_new;
+    Div page;
+};
+// rec = { held pages before, pages taken, stack index of the first page taken, flags }
+constexpr int REC_ENDED = 1, REC_REFUSED = 2, REC_BAD = 4;
+
+constexpr int PT = 1024, PW = PT / WAVE;   // the planning block: 16 waves
+
+// Exclusive prefix sum over the block's threads; *total the whole sum. red: PW values of LDS.
+__device__ __forceinline__ int64_t block_before(int64_t v, int64_t *red, int64_t &total) {
+    const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int64_t x = v;
+#pragma unroll
+    for (int o = 1; o < WAVE; o <<= 1) {
+        const int64_t y = __shfl_up(static_cast<long long>(x), o);
+        if (l >= o) x += y;
+    }
+    __syncthreads();                                  // red's readers of the call before are done
+    if (l == 63) red[w] = x;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+        if (i < w) before += red[i];
+        total += red[i];
+    }
+    return before + x - v;
+}
+
+// The page of block b of a request: kept from its table, or taken from the stack (whose top part was
+// filled before); -1: none.
+__device__ __forceinline__ int page_at(const PlanArgs &a, int i, const int4 &r, int b) {
+    if (b < r.x) return gld(a.table_in + static_cast<size_t>(i) * a.blocks + b);
+    return b - r.x < r.y ? gld(a.free_pages + (r.z - (b - r.x))) : -1;
+}
+
+// Ancestors (itself included) of node `lane` as bits, by pointer jumping: after round k a node has
+// the bits of its 2^k nearest, so six rounds cover 64 nodes. par < 0: nothing above. All lanes call it.
+__device__ __forceinline__ uint64_t ancestors(int par) {
+    const int l = threadIdx.x & 63;
+    uint64_t m = uint64_t(1) << l;
+#pragma unroll
+    for (int k = 0; k < 6; ++k) {
+        const int src = par < 0 ? l : par;
+        const uint64_t um = __shfl(static_cast<unsigned long long>(m), src);
+        const int up = __shfl(par, src);
+        if (par >= 0) {
+            m |= um;
+            par = up;
+        }
+    }
+    return m;
+}
+
+// Rows and table entries of request i from its record, part `part` of `parts` (a part: `width` threads
+// from thread `t`, a multiple of a wave).
+__device__ __forceinline__ void fill_request(const PlanArgs &a, int i, int part, int parts, int t, int width) {
+    const int4 r = a.rec[i];
+    const int c0 = gld(a.cu + i), count = gld(a.cu + i + 1) - c0;
+    const int past = gld(a.n_past + i);
+    const bool ended = r.w & REC_ENDED, bad = r.w & REC_BAD, none = r.w & (REC_BAD | REC_REFUSED);
+    const int held = ended ? 0 : r.x + r.y;
+    for (int b = part * width + t; b < a.blocks; b += parts * width) {
+        // a request with lengths out of range keeps its table as it is
+        const int p = bad ? gld(a.table_in + static_cast<size_t>(i) * a.blocks + b) : b < held ? page_at(a, i, r, b) : -1;
+        gst(a.table + static_cast<size_t>(i) * a.blocks + b, p);
+    }
+    auto slot_of = [&](int j) {
+        if (none) return -1;
+        const int at = past + j, b = div_by(a.page, at), p = page_at(a, i, r, b);
+        const bool in = static_cast<unsigned>(p) < static_cast<unsigned>(a.n_pages);
+        return in ? p * static_cast<int>(a.page.d) + (at - b * static_cast<int>(a.page.d)) : -1;
+    };
+    if (a.parent && !bad) {                           // at most 64 rows: one wave's
+        if (part == 0 && t < WAVE) {
+            const int j = t;
+            const uint64_t m = ancestors(j < count ? gld(a.parent + c0 + j) : -1);
+            if (j < count) {
+                gst(a.slot + c0 + j, slot_of(j));
+                gst(a.pos + c0 + j, past + static_cast<int>(__popcll(m)) - 1);
+                gst(a.mask + c0 + j, m);
+            }
+        }
+        return;
+    }
+    for (int j = part * width + t; j < count; j += parts * width) {
+        gst(a.slot + c0 + j, slot_of(j));
+        gst(a.pos + c0 + j, bad ? 0 : past + j);
+        gst(a.mask + c0 + j, bad ? uint64_t(0) : j >= 63 ? ~uint64_t(0) : (uint64_t(2) << j) - 1);
+    }
+}
+
+// One block plans all requests: row offsets, the checks, the stack; FILL: the tables and rows too, a
+// wave a request at a time. Thread t takes requests t, t + PT, ...: a request's values meet their
+// neighbours' in the prefix sums only, so they are read again in each pass rather than held.
+template <bool FILL>
+__global__ void __launch_bounds__(PT) k_plan(PlanArgs a) {
+    __shared__ int64_t red[PW];
+    __shared__ int s_top;
+    const int tid = threadIdx.x, wv = tid >> 6, l = tid & 63;
+    const int64_t room = min(static_cast<int64_t>(a.blocks) * a.page.d, static_cast<int64_t>(INT32_MAX));
+    // rows: offsets, and which lengths are in range
+    int64_t rows = 0, total;
+    for (int i0 = 0; i0 < a.n; i0 += PT) {
+        const int i = i0 + tid;
+        int past = 0, add = 0, held = 0;
+        if (i < a.n) {
+            past = gld(a.n_past + i);
+            add = gld(a.n_new + i);
+            held = gld(a.held_in + i);
+        }
+        const int count = max(add, 0);
+        const int64_t at = rows + block_before(count, red, total);
+        rows += total;
+        if (i < a.n) {
+            const bool bad = past < 0 || held < 0 || held > a.blocks || add > a.max_new || at + count > a.n_rows ||
+                             (add >= 0 && static_cast<int64_t>(past) + count > room);
+            gst(a.cu + i, static_cast<int>(min(at, static_cast<int64_t>(a.n_rows))));
+            gst(a.status + i, bad ? 2 : 0);
+            a.rec[i] = int4{held, 0, 0, (add < 0 ? REC_ENDED : 0) | (bad ? REC_BAD : 0)};
+        }
+    }
+    if (tid == 0) gst(a.cu + a.n, static_cast<int>(min(rows, static_cast<int64_t>(a.n_rows))));
+    __threadfence_block();
+    __syncthreads();
+    // parents come before their rows: a wave a request, a lane a row
+    if (a.parent) {
+        for (int i = wv; i < a.n; i += PW) {
+            if (a.rec[i].w & (REC_BAD | REC_ENDED)) continue;
+            const int c0 = gld(a.cu + i), count = gld(a.cu + i + 1) - c0;
+            const int p = l < count ? gld(a.parent + c0 + l) : -1;
+            if (__ballot(p < -1 || p >= l) != 0 && l == 0) {
+                gst(a.status + i, 3);
+                a.rec[i].w |= REC_BAD;
+            }
+        }
+        __threadfence_block();
+        __syncthreads();
+    }
+    // the ended requests' pages go onto the stack, a wave a request
+    int top = min(max(gld(a.free_in), 0), a.n_pages);
+    for (int i0 = 0; i0 < a.n; i0 += PT) {
+        const int i = i0 + tid;
+        int back = 0;
+        if (i < a.n) {
+            const int4 r = a.rec[i];
+            if ((r.w & (REC_ENDED | REC_BAD)) == REC_ENDED) back = r.x;
+        }
+        const int64_t before = block_before(back, red, total);
+        if (i < a.n && back > 0) a.rec[i].z = static_cast<int>(min(top + before, static_cast<int64_t>(a.n_pages)));
+        if (total > 0) {
+            __threadfence_block();
+            __syncthreads();
+            for (int k = i0 + wv; k < min(a.n, i0 + PT); k += PW) {
+                const int4 r = a.rec[k];
+                if ((r.w & (REC_ENDED | REC_BAD)) != REC_ENDED) continue;
+                for (int b = l; b < r.x && r.z + b < a.n_pages; b += WAVE)
+                    gst(a.free_pages + r.z + b, gld(a.table_in + static_cast<size_t>(k) * a.blocks + b));
+            }
+        }
+        top = static_cast<int>(min(top + total, static_cast<int64_t>(a.n_pages)));
+    }
+    // pages taken, in order, as long as they last
+    int64_t asked = 0;
+    int taken_all = 0;
+    if (tid == 0) s_top = 0;
+    for (int i0 = 0; i0 < a.n; i0 += PT) {
+        const int i = i0 + tid;
+        int4 r{0, 0, 0, REC_BAD};
+        int64_t want = 0;
+        if (i < a.n) {
+            r = a.rec[i];
+            if (!(r.w & (REC_BAD | REC_ENDED))) {
+                const int len = gld(a.n_past + i) + max(gld(a.n_new + i), 0);       // <= room
+                want = max((len > 0 ? div_by(a.page, len - 1) + 1 : 0) - r.x, 0);
+            }
+        }
+        const int64_t off = asked + block_before(want, red, total);
+        asked += total;
+        const bool refused = want > 0 && off + want > top;
+        if (i < a.n) {
+            const int taken = refused ? 0 : static_cast<int>(want);
+            if (refused) gst(a.status + i, 1);
+            if (!(r.w & (REC_BAD | REC_ENDED)))
+                a.rec[i] = int4{r.x, taken, static_cast<int>(max<int64_t>(top - 1 - off, 0)), r.w | (refused ? REC_REFUSED : 0)};
+            gst(a.held + i, (r.w & (REC_ENDED | REC_BAD)) == REC_ENDED ? 0 : r.x + taken);
+            // the granted requests' pages lie without gaps below the top
+            if (taken > 0) atomicMax(&s_top, static_cast<int>(off) + taken);
+        }
+    }
+    __threadfence_block();
+    __syncthreads();
+    taken_all = s_top;
+    if (tid == 0) gst(a.n_free, top - taken_all);
+    if constexpr (FILL)
+        for (int i = wv; i < a.n; i += PW) fill_request(a, i, 0, 1, l, WAVE);
+}
+
+constexpr int FT = 256;
+__global__ void __launch_bounds__(FT) k_plan_fill(PlanArgs a) {
+    fill_request(a, blockIdx.x, blockIdx.y, gridDim.y, threadIdx.x, FT);
+}
+
+// ---- append ----------------------------------------------------------------------------------
+
+struct AppendArgs {
+    const void *x;
+    const float *qn, *kn, *rot;
+    void *k, *v, *q;
+    const int32_t *cu, *slot, *pos;
+    float eps;
+    int n, n_rows, n_rot, slots, hq, hk, ldx, ldkv, ldq;
+    Div heads;                         // by hq + 2 hk
+};
+
+// Four consecutive elements as f32, and back with one rounding to nearest (ties to even).
+template <class T>
+__device__ __forceinline__ f32x4_t load4(const T *p) {
+    if constexpr (sizeof(T) == 4) return ld4(reinterpret_cast<const float *>(p));
+    else {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        const T4 t = *(const NAVI_GLOBAL T4 *) p;
+        return f32x4_t{static_cast<float>(t[0]), static_cast<float>(t[1]), static_cast<float>(t[2]), static_cast<float>(t[3])};
+    }
+}
+template <class T>
+__device__ __forceinline__ void store4(T *p, f32x4_t v) {
+    if constexpr (sizeof(T) == 4) st4(reinterpret_cast<float *>(p), v);
+    else {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        *(NAVI_GLOBAL T4 *) p = T4{static_cast<T>(v[0]), static_cast<T>(v[1]), static_cast<T>(v[2]), static_cast<T>(v[3])};
+    }
+}
+
+// One head of one row takes D / 8 lanes: lane c holds elements 4c .. 4c + 3 of each half, the pairs that
+// the rotation mixes, so a head is read, normed, turned and written from registers.
+template <class X, class Q, class E, int D>
+__global__ void __launch_bounds__(256) k_append(AppendArgs a) {
+    constexpr int LN = D / 8, HB = 256 / LN;
+    const int c = threadIdx.x % LN, nh = a.hq + 2 * a.hk;
+    const int task = blockIdx.x * HB + threadIdx.x / LN;
+    const int r = div_by(a.heads, task), h = task - r * nh;
+    if (r >= min(gld(a.cu + a.n), a.n_rows)) return;
+    const X *x = static_cast<const X *>(a.x) + static_cast<size_t>(r) * a.ldx + h * D + 4 * c;
+    f32x4_t x0 = load4(x), x1 = load4(x + D / 2);
+    const int slot = gld(a.slot + r), pos = gld(a.pos + r);
+    const bool in = !a.rot || static_cast<unsigned>(pos) < static_cast<unsigned>(a.n_rot);
+    const bool isq = h < a.hq;
+    if (h < a.hq + a.hk) {
+        const float *w = isq ? a.qn : a.kn;
+        if (w) {
+            float ss = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ss = fmaf(x0[j], x0[j], fmaf(x1[j], x1[j], ss));
+            ss += dpp_red<0xB1>(ss);
+            ss += dpp_red<0x4E>(ss);
+            ss += dpp_red<0x141>(ss);
+            if (LN == 16) ss += dpp_red<0x140>(ss);
+            const float scl = rsqrtf(ss / static_cast<float>(D) + a.eps);
+            const f32x4_t w0 = ld4(w + 4 * c), w1 = ld4(w + D / 2 + 4 * c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x0[j] = x0[j] * scl * w0[j];
+                x1[j] = x1[j] * scl * w1[j];
+            }
+        }
+        if (a.rot && in) {
+            const float *t = a.rot + static_cast<size_t>(pos) * D + 4 * c;
+            const f32x4_t cs = ld4(t), sn = ld4(t + D / 2);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float y0 = x0[j] * cs[j] - x1[j] * sn[j], y1 = x1[j] * cs[j] + x0[j] * sn[j];
+                x0[j] = y0;
+                x1[j] = y1;
+            }
+        }
+    }
+    if (isq) {
+        if (!in) x0 = x1 = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        Q *q = static_cast<Q *>(a.q) + static_cast<size_t>(r) * a.ldq + h * D + 4 * c;
+        store4(q, x0);
+        store4(q + D / 2, x1);
+    } else if (in && static_cast<unsigned>(slot) < static_cast<unsigned>(a.slots)) {
+        const bool isk = h < a.hq + a.hk;
+        E *d = static_cast<E *>(isk ? a.k : a.v) + static_cast<size_t>(slot) * a.ldkv + (h - a.hq - (isk ? 0 : a.hk)) * D + 4 * c;
+        store4(d, x0);
+        store4(d + D / 2, x1);
+    }
+}
+
+template <class X, class Q, class E>
+void launch_append(const AppendArgs &a, int D, hipStream_t s) {
+    const int64_t tasks = static_cast<int64_t>(a.n_rows) * (a.hq + 2 * a.hk), per = 256 / (D / 8);
+    const dim3 grid(static_cast<unsigned>((tasks + per - 1) / per));
+    if (D == 128) hipLaunchKernelGGL((k_append<X, Q, E, 128>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_append<X, Q, E, 64>), grid, dim3(256), 0, s, a);
+}
+
+template <class E>
+void launch_append_types(const AppendArgs &a, bool xf, bool qf, int D, hipStream_t s) {
+    if (xf && qf) launch_append<float, float, E>(a, D, s);
+    else if (xf) launch_append<float, E, E>(a, D, s);
+    else if (qf) launch_append<E, float, E>(a, D, s);
+    else launch_append<E, E, E>(a, D, s);
+}
+
+// ---- commit ----------------------------------------------------------------------------------
+
+constexpr int CL = 32;                 // layers a launch
+struct CommitArgs {
+    void *k[CL], *v[CL];
+    const int32_t *table, *n_past, *cu, *path, *accept;
+    int32_t *past_out, *status;
+    int max_path, blocks, n_pages, ld, write;   // write: this launch stores the results
+    Div page;
+};
+
+// Block (columns, request, layer and K or V): each thread moves 16 bytes of a row for the whole path, in order. A
+// path ascends, so its j-th source lies at or above position j: a row is read before, or when, it
+// is written, and batches of eight that read before they write keep that.
+constexpr int CT = 128;
+__global__ void __launch_bounds__(CT) k_commit(CommitArgs a) {
+    __shared__ int src[WAVE], dst[WAVE];
+    __shared__ int s_n;
+    const int i = blockIdx.y, l = threadIdx.x;
+    const int past = gld(a.n_past + i), count = gld(a.cu + i + 1) - gld(a.cu + i), n = gld(a.accept + i);
+    if (l < WAVE) {
+        bool bad = n < 0 || n > a.max_path || past < 0;
+        int p = -1;
+        if (!bad && l < n) p = gld(a.path + static_cast<size_t>(i) * a.max_path + l);
+        const int prev = __shfl_up(p, 1);
+        auto slot_of = [&](int node) {
+            const int64_t at = static_cast<int64_t>(past) + node;
+            if (at >= static_cast<int64_t>(a.blocks) * a.page.d || at > INT32_MAX) return -1;
+            const int b = div_by(a.page, static_cast<int>(at)), g = gld(a.table + static_cast<size_t>(i) * a.blocks + b);
+            return static_cast<unsigned>(g) < static_cast<unsigned>(a.n_pages)
+                       ? g * static_cast<int>(a.page.d) + static_cast<int>(at) - b * static_cast<int>(a.page.d) : -1;
+        };
+        if (!bad && l < n) {
+            bad = p < 0 || p >= count || (l > 0 && p <= prev);
+            if (!bad) {
+                src[l] = slot_of(p);
+                dst[l] = slot_of(l);
+                bad = src[l] < 0 || dst[l] < 0;
+            }
+        }
+        const bool any = __ballot(bad) != 0;
+        if (l == 0) {
+            s_n = any ? 0 : n;
+            if (a.write && blockIdx.x == 0 && blockIdx.z == 0) {
+                gst(a.past_out + i, any ? past : past + n);
+                gst(a.status + i, any ? 2 : 0);
+            }
+        }
+    }
+    __syncthreads();
+    const int m = s_n, col = (blockIdx.x * CT + l) * 8;
+    if (col >= a.ld) return;
+    uint16_t *base = static_cast<uint16_t *>(blockIdx.z & 1 ? a.v[blockIdx.z >> 1] : a.k[blockIdx.z >> 1]) + col;
+    for (int j0 = 0; j0 < m; j0 += 8) {
+        u32x4_t t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j0 + j < m && src[j0 + j] != dst[j0 + j])
+                t[j] = *(const NAVI_GLOBAL u32x4_t *) (base + static_cast<size_t>(src[j0 + j]) * a.ld);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j0 + j < m && src[j0 + j] != dst[j0 + j])
+                *(NAVI_GLOBAL u32x4_t *) (base + static_cast<size_t>(dst[j0 + j]) * a.ld) = t[j];
+    }
+}
+
+} // namespace kv
+} // namespace navi_amd
+
+using namespace navi_amd;
+using namespace navi_amd::kv;
+
+extern "C" {
+
+navi_status navi_kv_plan(const navi_kv_pages *pages, const int32_t *d_n_new, const int32_t *d_parent, const int32_t *d_table_in,
+                         const int32_t *d_held_in, const int32_t *d_free_in, int32_t *d_free_pages, int32_t *d_held,
+                         int32_t *d_free, int32_t *d_status, int32_t *d_scratch, void *stream, char *err, size_t errlen) {
+    navi_status st = check_pages("kv_plan", pages, err, errlen);
+    if (st != NAVI_OK) return st;
+    if (!d_n_new || !d_table_in || !d_held_in || !d_free_in || !d_free_pages || !d_held || !d_free || !d_status || !d_scratch) {
+        set_err(err, errlen, "kv_plan: null argument");
+        return NAVI_ERR_INVALID;
+    }
+    if (d_parent && pages->max_new > 64) {
+        set_err(err, errlen, "kv_plan: trees of up to %d rows a request; at most 64", pages->max_new);
+        return NAVI_ERR_INVALID;
+    }
+    if (!aligned16(d_scratch)) {
+        set_err(err, errlen, "kv_plan: d_scratch is not 16-byte aligned");
+        return NAVI_ERR_INVALID;
+    }
+    OnDevice dev;
+    if ((st = dev.enter(stream, "kv_plan", err, errlen)) != NAVI_OK) return st;
+    const PlanArgs a{pages->n_past, d_n_new, d_parent, d_table_in, d_held_in, d_free_in, d_free_pages, pages->block_table, d_held, d_free,
+                     d_status, pages->cu_rows, pages->row_slot, pages->row_pos, pages->row_mask, reinterpret_cast<int4 *>(d_scratch),
+                     pages->n_requests, pages->n_pages, pages->max_blocks, pages->n_rows, pages->max_new,
+                     make_div(static_cast<uint32_t>(pages->page_size))};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int64_t words = static_cast<int64_t>(pages->n_requests) * pages->max_blocks + pages->n_rows;
+    if (words <= 4096) {
+        hipLaunchKernelGGL(k_plan<true>, dim3(1), dim3(PT), 0, s, a);
+    } else {
+        hipLaunchKernelGGL(k_plan<false>, dim3(1), dim3(PT), 0, s, a);
+        const int longest = std::max(pages->max_blocks, d_parent ? 1 : std::min(pages->max_new, pages->n_rows));
+        hipLaunchKernelGGL(k_plan_fill, dim3(pages->n_requests, std::min((longest + 4 * FT - 1) / (4 * FT), 256)), dim3(FT), 0, s, a);
+    }
+    NAVI_TRY_HIP(hipGetLastError(), err, errlen);
+    return NAVI_OK;
+}
+
+navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *heads, const void *d_x, int32_t x_dtype, int32_t ldx,
+                           const float *d_q_norm, const float *d_k_norm, float eps, const float *d_rot, int32_t n_rot, void *d_k,
+                           void *d_v, int32_t ld_kv, void *d_q, int32_t q_dtype, int32_t ldq, void *stream, char *err,
+                           size_t errlen) {
+    navi_status st = check_pages("kv_append", pages, err, errlen);
+    if (st == NAVI_OK) st = check_heads("kv_append", heads, ld_kv, err, errlen);
+    if (st != NAVI_OK) return st;
+    const int D = heads->head_dim, nh = heads->n_head + 2 * heads->n_kv_head;
+    if ((x_dtype != NAVI_DT_F32 && x_dtype != heads->kv_dtype) || (q_dtype != NAVI_DT_F32 && q_dtype != heads->kv_dtype)) {
+        set_err(err, errlen, "kv_append: unsupported types (x %d, q %d, cache %d)", x_dtype, q_dtype, heads->kv_dtype);
+        return NAVI_ERR_UNSUPPORTED;
+    }
+    if (!rows_ok(d_x, x_dtype, ldx, static_cast<long>(nh) * D) || !rows_ok(d_q, q_dtype, ldq, static_cast<long>(heads->n_head) * D) || !d_k ||
+        !d_v || !aligned16(d_k) || !aligned16(d_v) || !aligned16(d_q_norm) || !aligned16(d_k_norm) || !aligned16(d_rot) ||
+        (d_rot && n_rot < 1)) {
+        set_err(err, errlen, "kv_append: a null or misaligned pointer, or a stride too small (ldx %d, ldq %d, n_rot %d)", ldx, ldq, n_rot);
+        return NAVI_ERR_INVALID;
+    }
+    if (static_cast<int64_t>(pages->n_rows) * nh + 256 > INT32_MAX) {
+        set_err(err, errlen, "kv_append: %d rows of %d heads are too many for one call", pages->n_rows, nh);
+        return NAVI_ERR_INVALID;
+    }
+    OnDevice dev;
+    if ((st = dev.enter(stream, "kv_append", err, errlen)) != NAVI_OK) return st;
+    if (pages->n_rows == 0) return NAVI_OK;
+    const AppendArgs a{d_x, d_q_norm, d_k_norm, d_rot, d_k, d_v, d_q, pages->cu_rows, pages->row_slot, pages->row_pos, eps, pages->n_requests,
+                       pages->n_rows, n_rot, pages->n_pages * pages->page_size, heads->n_head, heads->n_kv_head, ldx, ld_kv, ldq,
+                       make_div(static_cast<uint32_t>(nh))};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (heads->kv_dtype == NAVI_DT_F16) launch_append_types<_Float16>(a, x_dtype == NAVI_DT_F32, q_dtype == NAVI_DT_F32, D, s);
+    else launch_append_types<__bf16>(a, x_dtype == NAVI_DT_F32, q_dtype == NAVI_DT_F32, D, s);
+    NAVI_TRY_HIP(hipGetLastError(), err, errlen);
+    return NAVI_OK;
+}
+
+navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, const int32_t *d_path, int32_t max_path,
+                           const int32_t *d_accept, int32_t *d_n_past_out, int32_t *d_status, void *stream, char *err,
+                           size_t errlen) {
+    navi_status st = check_pages("kv_commit", pages, err, errlen);
+    if (st != NAVI_OK) return st;
+    if (!kv || !kv->k || !kv->v || !d_path || !d_accept || !d_n_past_out || !d_status) {
+        set_err(err, errlen, "kv_commit: null argument");
+        return NAVI_ERR_INVALID;
+    }
+    if (d_n_past_out == pages->n_past) {
+        set_err(err, errlen, "kv_commit: d_n_past_out is n_past itself, which other blocks still read");
+        return NAVI_ERR_INVALID;
+    }
+    if (max_path < 1 || max_path > 64 || kv->n_layer < 1 || kv->kv_dim < 8 || kv->kv_dim % 8 != 0 ||
+        static_cast<int64_t>(kv->max_pos) < static_cast<int64_t>(pages->n_pages) * pages->page_size) {
+        set_err(err, errlen, "kv_commit: out of range (max_path %d, layers %d, row %d, %d cache rows for %d pages of %d)", max_path, kv->n_layer,
+                kv->kv_dim, kv->max_pos, pages->n_pages, pages->page_size);
+        return NAVI_ERR_INVALID;
+    }
+    for (int l = 0; l < kv->n_layer; ++l)
+        if (!kv->k[l] || !kv->v[l] || !aligned16(kv->k[l]) || !aligned16(kv->v[l])) {
+            set_err(err, errlen, "kv_commit: layer %d's cache is null or not 16-byte aligned", l);
+            return NAVI_ERR_INVALID;
+        }
+    OnDevice dev;
+    if ((st = dev.enter(stream, "kv_commit", err, errlen)) != NAVI_OK) return st;
+    for (int l0 = 0; l0 < kv->n_layer; l0 += CL) {
+        const int n = std::min(CL, kv->n_layer - l0);
+        CommitArgs a{};
+        for (int l = 0; l < n; ++l) {
+            a.k[l] = kv->k[l0 + l];
+            a.v[l] = kv->v[l0 + l];
+        }
+        a.table = pages->block_table;
+        a.n_past = pages->n_past;
+        a.cu = pages->cu_rows;
+        a.path = d_path;
+        a.accept = d_accept;
+        a.past_out = d_n_past_out;
+        a.status = d_status;
+        a.max_path = max_path;
+        a.blocks = pages->max_blocks;
+        a.n_pages = pages->n_pages;
+        a.ld = kv->kv_dim;
+        a.write = l0 == 0;
+        a.page = make_div(static_cast<uint32_t>(pages->page_size));
+        hipLaunchKernelGGL(k_commit, dim3((kv->kv_dim / 8 + CT - 1) / CT, pages->n_requests, 2 * n), dim3(CT), 0,
+                           static_cast<hipStream_t>(stream), a);
+    }
+    NAVI_TRY_HIP(hipGetLastError(), err, errlen);
+    return NAVI_OK;
+}
+
+} // extern "C"

@@ -1,0 +1,23 @@
+// The attention of drafted rows over a paged cache (tree.hip) as a host launcher: navi_tree_attention and
+// the talker's verification (prefill.hip) run it.
+#pragma once
+
+#include "kv.h"
+
+namespace navi_amd {
+namespace tree {
+
+struct Call {
+    const navi_kv_pages *pages;
+    const navi_kv_heads *heads;
+    const void *q, *k, *v;
+    void *out, *ws;
+    size_t ws_bytes;
+    int q_dtype, ldq, ldkv, ldo, max_keys;
+    float scale;
+};
+size_t workspace(const navi_kv_pages &pages, const navi_kv_heads &heads, int max_keys);
+void launch(const Call &c, hipStream_t s);   // arguments already checked
+
+} // namespace tree
+} // namespace navi_amd

@@ -41,6 +41,7 @@ EXPORTS = [
     "navi_speaker_last_ms", "navi_speaker_tap_mel", "navi_speaker_dim",
     "navi_streams_tap_hidden",
     "navi_streams_tap_logits", "navi_streams_tap_cp_logits",
+    "navi_kv_plan", "navi_kv_append", "navi_kv_commit", "navi_tree_attention", "navi_tree_workspace",
 ]
 
 
@@ -81,6 +82,20 @@ class TensorRef(C.Structure):
 class KvView(C.Structure):
     _fields_ = [("n_layer", C.c_int32), ("max_pos", C.c_int32), ("kv_dim", C.c_int32),
                 ("k", C.POINTER(C.c_void_p)), ("v", C.POINTER(C.c_void_p))]
+
+
+DT_F32, DT_F16, DT_BF16 = 0, 1, 2            # navi_dtype
+
+
+class KvPages(C.Structure):
+    """navi_kv_pages: a step's requests and rows on a pool of cache pages (device addresses)."""
+    _fields_ = [("n_requests", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32), ("max_blocks", C.c_int32),
+                ("n_rows", C.c_int32), ("max_new", C.c_int32), ("block_table", C.c_void_p), ("n_past", C.c_void_p),
+                ("cu_rows", C.c_void_p), ("row_slot", C.c_void_p), ("row_pos", C.c_void_p), ("row_mask", C.c_void_p)]
+
+
+class KvHeads(C.Structure):
+    _fields_ = [("n_head", C.c_int32), ("n_kv_head", C.c_int32), ("head_dim", C.c_int32), ("kv_dtype", C.c_int32)]
 
 
 class Sampling(C.Structure):
@@ -247,6 +262,17 @@ def lib() -> C.CDLL:
     L.navi_streams_max_streams.argtypes = [C.c_void_p]
     L.navi_streams_last_ms.argtypes = [C.c_void_p]
     L.navi_streams_last_ms.restype = C.c_double
+    L.navi_kv_plan.argtypes = [C.POINTER(KvPages)] + [C.c_void_p] * 11 + [E, C.c_size_t]
+    L.navi_kv_append.argtypes = [C.POINTER(KvPages), C.POINTER(KvHeads), C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p,
+                                 C.c_float, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32,
+                                 C.c_int32, C.c_void_p, E, C.c_size_t]
+    L.navi_kv_commit.argtypes = [C.POINTER(KvPages), C.POINTER(KvView), C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                 C.c_void_p, E, C.c_size_t]
+    L.navi_tree_attention.argtypes = [C.POINTER(KvPages), C.POINTER(KvHeads), C.c_void_p, C.c_int32, C.c_int32, C.c_void_p,
+                                      C.c_void_p, C.c_int32, C.c_float, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_size_t,
+                                      C.c_void_p, E, C.c_size_t]
+    L.navi_tree_workspace.argtypes = [C.POINTER(KvPages), C.POINTER(KvHeads), C.c_int32]
+    L.navi_tree_workspace.restype = C.c_size_t
     _lib = L
     return L
 
@@ -724,6 +750,50 @@ def linear(d_x: int, ldx: int, M: int, w: int, K: int, N: int, d_y: int, ldy: in
     err = C.create_string_buffer(256)
     fn = lib().navi_linear_noalloc if noalloc else lib().navi_linear
     _check(fn(d_x, ldx, M, w, K, N, bias, residual, act, d_y, ldy, err, 256), err)
+
+
+# ---- several requests on one pool of cache pages ---------------------------------------
+# Every argument that is not a size is a device address; `stream`: a hipStream_t (None: HIP's default
+# stream, navi_device_stream() the library's). The calls enqueue and return.
+
+def kv_plan(pages: KvPages, *, n_new: int, table_in: int, held_in: int, free_in: int, free_pages: int, held: int, free: int,
+            status: int, scratch: int, parent: int | None = None, stream: int | None = None):
+    """navi_kv_plan: block tables, slots, positions and ancestors of a step's rows, from the requests' lengths."""
+    err = C.create_string_buffer(256)
+    _check(lib().navi_kv_plan(pages, n_new, parent, table_in, held_in, free_in, free_pages, held, free, status, scratch, stream,
+                              err, 256), err)
+
+
+def kv_append(pages: KvPages, heads: KvHeads, x: int, x_dtype: int, ldx: int, k: int, v: int, ld_kv: int, q: int, q_dtype: int,
+              ldq: int, *, q_norm: int | None = None, k_norm: int | None = None, eps: float = 1e-6, rot: int | None = None,
+              n_rot: int = 0, stream: int | None = None):
+    """navi_kv_append: a layer's q|k|v rows normed and turned, K and V into the pages, q to `q`."""
+    err = C.create_string_buffer(256)
+    _check(lib().navi_kv_append(pages, heads, x, x_dtype, ldx, q_norm, k_norm, eps, rot, n_rot, k, v, ld_kv, q, q_dtype, ldq,
+                                stream, err, 256), err)
+
+
+def tree_workspace(pages: KvPages, heads: KvHeads, max_keys: int) -> int:
+    """navi_tree_workspace: the bytes of workspace that tree_attention needs."""
+    return lib().navi_tree_workspace(pages, heads, max_keys)
+
+
+def tree_attention(pages: KvPages, heads: KvHeads, q: int, q_dtype: int, ldq: int, k: int, v: int, ld_kv: int, scale: float,
+                   max_keys: int, out: int, ldo: int, ws: int | None, ws_bytes: int, *, stream: int | None = None):
+    """navi_tree_attention: a layer's attention of the step's rows over the pages."""
+    err = C.create_string_buffer(256)
+    _check(lib().navi_tree_attention(pages, heads, q, q_dtype, ldq, k, v, ld_kv, scale, max_keys, out, ldo, ws, ws_bytes, stream,
+                                     err, 256), err)
+
+
+def kv_commit(pages: KvPages, k, v, ld_kv: int, path: int, max_path: int, accept: int, n_past: int, status: int, *,
+              stream: int | None = None):
+    """navi_kv_commit: the accepted rows of each request moved into place in every layer; k, v: one address a layer."""
+    n = len(k)
+    kp, vp = (C.c_void_p * n)(*k), (C.c_void_p * n)(*v)
+    view = KvView(n, pages.n_pages * pages.page_size, ld_kv, C.cast(kp, C.POINTER(C.c_void_p)), C.cast(vp, C.POINTER(C.c_void_p)))
+    err = C.create_string_buffer(256)
+    _check(lib().navi_kv_commit(pages, view, path, max_path, accept, n_past, status, stream, err, 256), err)
 
 
 # ---- vocoder ---------------------------------------------------------------------------
