@@ -269,7 +269,7 @@ navi_status navi_linear_noalloc(const float *d_x, int32_t ldx, int32_t M, const 
  *   navi_kv_append       a layer's q|k|v rows: K and V into the pages, q for the attention
  *   navi_tree_attention  a layer's attention of those rows over the pages
  *   navi_kv_commit       the accepted rows moved to their positions, in every layer
- * These four enqueue on `stream` (a hipStream_t of the library's device, used as it is: NULL is HIP's
+ * (navi_talker_verify runs the middle two in every layer of the talker.) The four enqueue on `stream` (a hipStream_t of the library's device, used as it is: NULL is HIP's
  * default stream, navi_device_stream() the library's) and return without waiting. They allocate
  * nothing and may be captured into a graph. The calling thread's current device is left as it was. Every pointer in a struct or named d_* is
  * device memory of the library's device; a stream of another device is refused. */
@@ -353,6 +353,17 @@ size_t navi_tree_workspace(const navi_kv_pages *pages, const navi_kv_heads *head
 navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, const int32_t *d_path, int32_t max_path,
                            const int32_t *d_accept, int32_t *d_n_past_out, int32_t *d_status, void *stream, char *err,
                            size_t errlen);
+/* The talker over a planned step: the layers of navi_talker_prefill on the step's rows d_rows f32 [n_rows][hidden]
+ * (drafted step inputs; one row a request is a decode step, a chain of 64 a piece of a prompt), each row seeing its
+ * request's cached positions and its ancestors in the step. Stores the rows' K and V in the pages of every layer, and
+ * every row's post-norm hidden in d_hidden f32 [n_rows][hidden] and its logits in d_logits f32 [n_rows][vocab]
+ * (NULL: not computed). kv: the pool (n_layer, kv_dim and at least n_pages * page_size rows as navi_talker_kv's), or NULL: the
+ * talker's own cache, whose max_positions rows are then the pages. n_rows <= max_prompt_tokens, max_new <= 64.
+ * max_keys as in navi_tree_attention, at most max_positions; positions past it get no K and V. Rows that belong to no
+ * request hold nothing of use. Errors as navi_talker_prefill.
+ * Runs on the library stream (plan on it too) and is synchronous; navi_talker_last_ms is its device time. */
+navi_status navi_talker_verify(navi_talker *t, const navi_kv_view *kv, const navi_kv_pages *pages, int32_t max_keys, const float *d_rows,
+                               float *d_hidden, float *d_logits, char *err, size_t errlen);
 
 /* ---- vocoder: codes -> 24 kHz PCM (vocoder.h:27-55) -------------------------- */
 

@@ -27,6 +27,7 @@
 #include "host_util.h"
 #include "linear.h"
 #include "rows.h"
+#include "tree.h"
 
 #include <algorithm>
 #include <cmath>
@@ -484,6 +485,23 @@ __global__ void __launch_bounds__(BT) k_tiled_row_norm(const float *x, int m, co
     if (xn2) st4(xn2 + i, o);
 }
 
+// Every row of the tiled residual stream x, RMS-normed as k_tiled_row_norm's one: y [rows][H], row = block.
+__global__ void __launch_bounds__(BT) k_tiled_rows_norm(const float *x, const float *w, float eps, float *y, int H) {
+    __shared__ float red[4];
+    const int i = threadIdx.x * 4;                            // H == 4 * BT
+    const f32x4_t v = ld4(x + rows::pk_a(blockIdx.x, i, H));
+    const f32x4_t wv = ld4(w + i);
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ss = fmaf(v[j], v[j], ss);
+    ss = block_sum256(ss, red);
+    const float scale = rsqrtf(ss / static_cast<float>(H) + eps);
+    f32x4_t o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = v[j] * scale * wv[j];
+    st4(y + static_cast<size_t>(blockIdx.x) * H + i, o);
+}
+
 } // namespace pf
 } // namespace navi_amd
 
@@ -512,6 +530,11 @@ struct navi_talker {
     // prompt's keys and values as MFMA fragments; att and h hold f16 pairs (gemm.h pk_s) there, q too above SHORT_KEYS
     uint16_t *kf = nullptr, *vf = nullptr;
     float *rot = nullptr;
+    // navi_talker_verify's, allocated by its first call and grown when needed: the rotation of all max_pos positions and
+    // the attention's workspace
+    float *rot_all = nullptr;
+    void *tree_ws = nullptr;
+    size_t tree_bytes = 0;
     size_t part_floats = 0;
     uint32_t *flag = nullptr;
     bool flag_set = false;             // whether a call may have left the flag set
@@ -545,6 +568,7 @@ struct navi_talker {
         if (ev1) (void) hipEventDestroy(ev1);
         if (h_flag) (void) hipHostFree(h_flag);
         if (h_stage) (void) hipHostFree(h_stage);
+        if (tree_ws) (void) hipFree(tree_ws);
         for (void *p : owned) (void) hipFree(p);
     }
 };
@@ -1005,6 +1029,94 @@ navi_status navi_talker_prefill(navi_talker *t, const float *d_rows, int32_t n_r
     const navi_status st = flag_result(*t, "prefill", err, errlen);
     if (st != NAVI_OK) return st;
     t->n_used = T;
+    return NAVI_OK;
+}
+
+navi_status navi_talker_verify(navi_talker *t, const navi_kv_view *kv, const navi_kv_pages *pages, int32_t max_keys, const float *d_rows,
+                               float *d_hidden, float *d_logits, char *err, size_t errlen) {
+    if (!t || !pages || !d_rows || !d_hidden) {
+        set_err(err, errlen, "talker: verify: null argument");
+        return NAVI_ERR_INVALID;
+    }
+    navi_status st = kv::check_pages("talker: verify", pages, err, errlen);
+    if (st != NAVI_OK) return st;
+    navi_kv_view own;
+    if (!kv) {
+        (void) navi_talker_kv(t, &own, nullptr);
+        kv = &own;
+    }
+    const int T = pages->n_rows, H = t->H, QKVW = t->QD + 2 * t->KVD;
+    if (T < 1 || T > t->max_prompt || pages->max_new > 64) {
+        set_err(err, errlen, "talker: verify of %d rows, up to %d a request (at most %d, and 64)", T, pages->max_new, t->max_prompt);
+        return NAVI_ERR_INVALID;
+    }
+    if (kv->n_layer != t->L || kv->kv_dim != t->KVD || !kv->k || !kv->v ||
+        static_cast<int64_t>(kv->max_pos) < static_cast<int64_t>(pages->n_pages) * pages->page_size) {
+        set_err(err, errlen, "talker: verify: a cache of %d layers, rows of %d, %d rows for %d pages of %d", kv->n_layer, kv->kv_dim, kv->max_pos,
+                pages->n_pages, pages->page_size);
+        return NAVI_ERR_INVALID;
+    }
+    for (int l = 0; l < t->L; ++l)
+        if (!kv->k[l] || !kv->v[l] || !kv::aligned16(kv->k[l]) || !kv::aligned16(kv->v[l])) {
+            set_err(err, errlen, "talker: verify: layer %d's cache is null or not 16-byte aligned", l);
+            return NAVI_ERR_INVALID;
+        }
+    if (max_keys < 1 || max_keys > t->max_pos) {
+        set_err(err, errlen, "talker: verify: max_keys %d outside 1 .. max_positions (%d)", max_keys, t->max_pos);
+        return NAVI_ERR_INVALID;
+    }
+    if (!kv::aligned16(d_rows) || !kv::aligned16(d_hidden) || !kv::aligned16(d_logits)) {
+        set_err(err, errlen, "talker: verify: a pointer is not 16-byte aligned");
+        return NAVI_ERR_INVALID;
+    }
+    if ((st = ensure_device(err, errlen)) != NAVI_OK) return st;
+    hipStream_t s = device_state().stream;
+    if (!t->rot_all) {
+        float *rot = nullptr;
+        if ((st = t->alloc(rot, static_cast<size_t>(t->max_pos) * HD, err, errlen)) != NAVI_OK) return st;
+        hipLaunchKernelGGL(k_rotation, dim3(static_cast<unsigned>(t->max_pos)), dim3(HD / 2), 0, s, t->invf, rot);
+        t->rot_all = rot;
+    }
+    const navi_kv_heads heads{t->NQ, t->NKV, HD, NAVI_DT_F16};
+    const size_t need = tree::workspace(*pages, heads, max_keys);
+    if (need > t->tree_bytes) {
+        NAVI_TRY_HIP(hipStreamSynchronize(s), err, errlen);
+        if (t->tree_ws) (void) hipFree(t->tree_ws);
+        t->tree_ws = nullptr;
+        t->tree_bytes = 0;
+        NAVI_TRY_HIP(hipMalloc(&t->tree_ws, need), err, errlen);
+        t->tree_bytes = need;
+    }
+    NAVI_TRY_HIP(hipEventRecord(t->ev0, s), err, errlen);
+    rows::tile_rows(d_rows, T, H, t->x, s, t->flag);
+    t->flag_set = true;
+    // rows that belong to no request are not written by the attention: zeros, not what a prefill left there
+    NAVI_TRY_HIP(hipMemsetAsync(t->att, 0, static_cast<size_t>((T + 15) / 16 * 16) * t->QD * sizeof(float), s), err, errlen);
+    for (int l = 0; l < t->L; ++l) {
+        const LayerW &w = t->layers[l];
+        bool ok = rows::launch_rows_pk(rows::EPI_PLAIN, true, t->x, T, H, w.ln1, t->eps, w.qkv_t, QKVW, t->part, QKVW, t->flag, s);
+        st = navi_kv_append(pages, &heads, t->part, NAVI_DT_F32, QKVW, w.qn, w.kn, t->eps, t->rot_all, t->max_pos, kv->k[l], kv->v[l], t->KVD,
+                            t->q, NAVI_DT_F32, t->QD, s, err, errlen);
+        if (st != NAVI_OK) return st;
+        tree::launch({pages, &heads, t->q, kv->k[l], kv->v[l], t->att, t->tree_ws, t->tree_bytes, NAVI_DT_F32, t->QD, t->KVD, t->QD, max_keys,
+                      1.f / std::sqrt(static_cast<float>(HD)), true}, s);
+        ok = ok && rows::launch_rows_pk(rows::EPI_RESID, false, t->att, T, t->QD, nullptr, 0.f, w.o_t, H, t->x, 0, t->flag, s) &&
+             rows::launch_rows_pk(rows::EPI_SWIGLU, true, t->x, T, H, w.ln2, t->eps, w.gu_t, t->F, t->h, 0, t->flag, s) &&
+             rows::launch_rows_pk(rows::EPI_RESID, false, t->h, T, t->F, nullptr, 0.f, w.d_t, H, t->x, 0, t->flag, s);
+        if (!ok) {
+            set_err(err, errlen, "talker: a projection shape the prefill's tiled kernels do not take");
+            return NAVI_ERR_UNSUPPORTED;
+        }
+    }
+    hipLaunchKernelGGL(k_tiled_rows_norm, dim3(T), dim3(BT), 0, s, t->x, t->final_norm, t->eps, d_hidden, H);
+    if (d_logits)
+        rows::launch_rows(rows::EPI_PLAIN, false, d_hidden, H, T, H, nullptr, 0.f, t->head, t->V, nullptr, 0, nullptr, 0, d_logits, t->V, t->flag, s);
+    NAVI_TRY_HIP(hipGetLastError(), err, errlen);
+    NAVI_TRY_HIP(hipEventRecord(t->ev1, s), err, errlen);
+    if ((st = check_flag(*t, "verify", err, errlen)) != NAVI_OK) return st;
+    float ms = 0.f;
+    NAVI_TRY_HIP(hipEventElapsedTime(&ms, t->ev0, t->ev1), err, errlen);
+    t->last_ms = ms;
     return NAVI_OK;
 }
 

@@ -15,6 +15,7 @@ struct Call {
     size_t ws_bytes;
     int q_dtype, ldq, ldkv, ldo, max_keys;
     float scale;
+    bool tiled;                        // f32 out in the tile layout of rows.h (ldo unused)
 };
 size_t workspace(const navi_kv_pages &pages, const navi_kv_heads &heads, int max_keys);
 void launch(const Call &c, hipStream_t s);   // arguments already checked

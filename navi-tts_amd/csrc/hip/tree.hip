@@ -21,6 +21,7 @@
 //  * Few requests: a request's keys are split over several blocks, whose partial results (unnormalised sums,
 //    reference, sum) a second kernel joins in split order.
 #include "dev_common.h"
+#include "tile_layout.h"
 #include "tree.h"
 
 #include <algorithm>
@@ -45,6 +46,7 @@ struct Args {
     const int32_t *table, *n_past, *cu;
     const uint64_t *mask;
     int n, hkv, g, blocks, n_pages, n_rows, max_new, ldq, ldkv, ldo, splits, tiles, groups;   // tiles: of a split
+    int tiled;                         // f32 out: in the tile layout of rows.h, heads * D wide
     Div page, heads_per;               // heads_per: by g
     float scale;                       // scale * log2 e
 };
@@ -76,6 +78,18 @@ __device__ __forceinline__ bool any_special(u32x4_t x) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) b |= (x[i] & LO) == LO || (x[i] & HI) == HI;
     return b;
+}
+
+// Four consecutive columns of an output row.
+template <class E, bool PAIR>
+__device__ __forceinline__ void store_out(const Args &a, int row, int col, int width, f32x4_t o) {
+    if constexpr (PAIR) {
+        st4(static_cast<float *>(a.out) + (a.tiled ? rows::pk_a(row, col, width) : static_cast<size_t>(row) * a.ldo + col), o);
+    } else {
+        typedef typename Types<E>::v4 v4;
+        *(NAVI_GLOBAL v4 *) (static_cast<E *>(a.out) + static_cast<size_t>(row) * a.ldo + col) =
+            v4{static_cast<E>(o[0]), static_cast<E>(o[1]), static_cast<E>(o[2]), static_cast<E>(o[3])};
+    }
 }
 
 template <class T, class U>
@@ -404,10 +418,7 @@ __global__ void __launch_bounds__(BT) k_tree(Args a) {
                 }
             } else {
                 const float inv = mx == NONE ? 0.f : 1.f / total;
-                o *= inv;
-                const size_t at = static_cast<size_t>(c0 + j) * a.ldo + static_cast<size_t>(head) * D + col;
-                if constexpr (PAIR) st4(static_cast<float *>(a.out) + at, o);
-                else *(NAVI_GLOBAL v4 *) (static_cast<E *>(a.out) + at) = v4{static_cast<E>(o[0]), static_cast<E>(o[1]), static_cast<E>(o[2]), static_cast<E>(o[3])};
+                store_out<E, PAIR>(a, c0 + j, head * D + col, a.hkv * a.g * D, o * inv);
             }
         }
     }
@@ -416,7 +427,6 @@ __global__ void __launch_bounds__(BT) k_tree(Args a) {
 // Joins the splits of every row in split order: block (head and column tile, row of the request, request).
 template <class E, bool PAIR, int D>
 __global__ void __launch_bounds__(BT) k_tree_join(Args a) {
-    typedef typename Types<E>::v4 v4;
     const int req = blockIdx.z, j = blockIdx.y, heads = a.hkv * a.g;
     const int c0 = gld(a.cu + req), c1 = min(gld(a.cu + req + 1), a.n_rows);
     if (j >= c1 - c0) return;
@@ -438,10 +448,7 @@ __global__ void __launch_bounds__(BT) k_tree_join(Args a) {
         total += f * z;
         o += x * f;
     }
-    o *= m == NONE ? 0.f : 1.f / total;
-    const size_t to = static_cast<size_t>(c0 + j) * a.ldo + static_cast<size_t>(head) * D + col;
-    if constexpr (PAIR) st4(static_cast<float *>(a.out) + to, o);
-    else *(NAVI_GLOBAL v4 *) (static_cast<E *>(a.out) + to) = v4{static_cast<E>(o[0]), static_cast<E>(o[1]), static_cast<E>(o[2]), static_cast<E>(o[3])};
+    store_out<E, PAIR>(a, c0 + j, head * D + col, heads * D, o * (m == NONE ? 0.f : 1.f / total));
 }
 
 // How a call is cut: query tiles of a block, groups of them, splits of the keys and 32-key tiles of a split.
@@ -505,6 +512,7 @@ void launch(const Call &x, hipStream_t s) {
     a.splits = c.splits;
     a.tiles = c.tiles;
     a.groups = c.groups;
+    a.tiled = x.tiled;
     a.page = kv::make_div(static_cast<uint32_t>(p.page_size));
     a.heads_per = kv::make_div(static_cast<uint32_t>(a.g));
     a.scale = x.scale * 1.44269504088896340736f;
@@ -570,7 +578,7 @@ navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads 
     kv::OnDevice dev;
     if ((st = dev.enter(stream, "tree_attention", err, errlen)) != NAVI_OK) return st;
     if (pages->n_rows == 0) return NAVI_OK;
-    tree::launch({pages, heads, d_q, d_k, d_v, d_out, d_ws, ws_bytes, q_dtype, ldq, ld_kv, ldo, max_keys, scale}, static_cast<hipStream_t>(stream));
+    tree::launch({pages, heads, d_q, d_k, d_v, d_out, d_ws, ws_bytes, q_dtype, ldq, ld_kv, ldo, max_keys, scale, false}, static_cast<hipStream_t>(stream));
     NAVI_TRY_HIP(hipGetLastError(), err, errlen);
     return NAVI_OK;
 }

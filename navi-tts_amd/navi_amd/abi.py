@@ -42,6 +42,7 @@ EXPORTS = [
     "navi_streams_tap_hidden",
     "navi_streams_tap_logits", "navi_streams_tap_cp_logits",
     "navi_kv_plan", "navi_kv_append", "navi_kv_commit", "navi_tree_attention", "navi_tree_workspace",
+    "navi_talker_verify",
 ]
 
 
@@ -262,6 +263,8 @@ def lib() -> C.CDLL:
     L.navi_streams_max_streams.argtypes = [C.c_void_p]
     L.navi_streams_last_ms.argtypes = [C.c_void_p]
     L.navi_streams_last_ms.restype = C.c_double
+    L.navi_talker_verify.argtypes = [C.c_void_p, C.POINTER(KvView), C.POINTER(KvPages), C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                     E, C.c_size_t]
     L.navi_kv_plan.argtypes = [C.POINTER(KvPages)] + [C.c_void_p] * 11 + [E, C.c_size_t]
     L.navi_kv_append.argtypes = [C.POINTER(KvPages), C.POINTER(KvHeads), C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p,
                                  C.c_float, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32,
@@ -727,6 +730,12 @@ class Talker:
         err = C.create_string_buffer(256)
         _check(lib().navi_talker_prefill(self.h, d_rows, n_rows, err, 256), err)
         self.kv.n_used = n_rows
+
+    def verify(self, pages: KvPages, max_keys: int, d_rows: int, d_hidden: int, d_logits: int | None = None, kv=None):
+        """navi_talker_verify: the talker over a planned step's rows; kv: a KvCache as the pool, None: the talker's own."""
+        err = C.create_string_buffer(256)
+        _check(lib().navi_talker_verify(self.h, C.byref(kv.view) if kv is not None else None, pages, max_keys, d_rows, d_hidden,
+                                        d_logits, err, 256), err)
 
     @property
     def d_hidden(self) -> int:

@@ -1,0 +1,190 @@
+"""navi_talker_verify over planned steps against the CPU oracle: a prompt prefilled into the talker's own cache and one
+taken in as a chain of rows, trees of drafted rows on both, the accepted rows committed, and the next step on what
+was committed. Bars as the prefill's: 2e-2 max abs and cosine > 0.9995 against the oracle's rows."""
+import numpy as np
+import pytest
+import torch
+
+from gpu_util import compare, log
+from kv_util import random_tree
+
+pytestmark = pytest.mark.gpu
+TOL_ABS, TOL_COS, PAGE = 2e-2, 0.9995, 16
+
+
+def i32(v):
+    return torch.tensor(np.asarray(v, dtype=np.int64).astype(np.int32), dtype=torch.int32, device="cuda")
+
+
+@pytest.fixture(scope="module")
+def side(small_blob):
+    from navi_amd import abi
+    from oracle.model import Oracle
+    abi.device_open()
+    W = abi.DeviceWeights(small_blob, select=lambda t: t.name.startswith("talker."))
+    return abi, Oracle(small_blob), abi.Talker(W, max_prompt_tokens=128, max_positions=512), W
+
+
+class Pool:
+    """The requests' state on the device, over the talker's own cache as pages of 16 rows."""
+
+    def __init__(self, abi, talker, n, taken):
+        self.abi, self.t, self.n, self.n_pages, self.blocks = abi, talker, n, 512 // PAGE, 12
+        rest = list(range(self.n_pages - 1, -1, -1))
+        table = [[-1] * self.blocks for _ in range(n)]
+        for i, pages in taken.items():
+            table[i][:len(pages)] = pages
+            rest = [p for p in rest if p not in pages]
+        self.table, self.held, self.free, self.stack = i32(table), i32([len(taken.get(i, [])) for i in range(n)]), i32([len(rest)]), i32(rest + [0] * (self.n_pages - len(rest)))
+        self.past = i32([0] * n)
+
+    def step(self, trees, rows, kv=None, logits=True, spare=0):
+        abi, new = self.abi, [len(t) for t in trees]
+        R = sum(new) + spare
+        self.cu, self.slot, self.pos, self.status = i32([0] * (self.n + 1)), i32([-1] * R), i32([0] * R), i32([0] * self.n)
+        self.mask, scratch = torch.zeros(R, dtype=torch.int64, device="cuda"), i32([0] * 4 * self.n)
+        d_new, d_par = i32(new), i32([p for t in trees for p in t] + [0] * spare)
+        d_rows = torch.cat([torch.from_numpy(np.concatenate(rows).astype(np.float32)), torch.zeros(spare, 1024)]).cuda()
+        hid, lg = torch.zeros(R, 1024, device="cuda"), torch.zeros(R, self.t.params.talker.vocab, device="cuda")
+        self.pages = abi.KvPages(self.n, PAGE, self.n_pages, self.blocks, R, 64, *(x.data_ptr() for x in (self.table, self.past, self.cu, self.slot, self.pos, self.mask)))
+        torch.cuda.synchronize()
+        abi.kv_plan(self.pages, n_new=d_new.data_ptr(), parent=d_par.data_ptr(), table_in=self.table.data_ptr(), held_in=self.held.data_ptr(),
+                    free_in=self.free.data_ptr(), free_pages=self.stack.data_ptr(), held=self.held.data_ptr(), free=self.free.data_ptr(),
+                    status=self.status.data_ptr(), scratch=scratch.data_ptr(), stream=abi.lib().navi_device_stream())
+        self.t.verify(self.pages, self.blocks * PAGE, d_rows.data_ptr(), hid.data_ptr(), lg.data_ptr() if logits else None, kv=kv)
+        assert self.status.tolist() == [0] * self.n
+        return hid.cpu().numpy(), lg.cpu().numpy()
+
+    def commit(self, paths, kv):
+        st = self.abi.lib().navi_device_stream()
+        path, acc, past, status = i32([p + [0] * (64 - len(p)) for p in paths]), i32([len(p) for p in paths]), i32([0] * self.n), i32([0] * self.n)
+        torch.cuda.synchronize()
+        self.abi.kv_commit(self.pages, list(kv.k), list(kv.v), kv.kv_dim, path.data_ptr(), 64, acc.data_ptr(), past.data_ptr(), status.data_ptr(), stream=st)
+        torch.cuda.synchronize()
+        assert status.tolist() == [0] * self.n
+        self.past.copy_(past)
+
+
+def oracle_rows(ora, history, x):
+    """Post-norm hidden and logits of rows x after the rows of `history`."""
+    kv = ora.new_kv(256)
+    rows = np.concatenate([history, x]).astype(np.float32)
+    h, lg = ora.talker_forward(torch.from_numpy(rows), kv, 0)
+    return h.numpy()[len(history):], lg.numpy()[len(history):]
+
+
+def chain_of(tree, j):
+    out = []
+    while j >= 0:
+        out.insert(0, j)
+        j = tree[j]
+    return out
+
+
+def check(ora, history, tree, x, hid, lg, what):
+    for j in range(len(tree)):
+        c = chain_of(tree, j)
+        if j % 3 and j != len(tree) - 1 and len(tree) > 8:
+            continue                                          # every third node of a larger tree
+        h, l = oracle_rows(ora, history, x[c])
+        for got, want, name in ((hid[j], h[-1], "hidden"), (lg[j], l[-1], "logits")):
+            d, cos = compare(got, want)
+            assert d < TOL_ABS and cos > TOL_COS, (what, j, name, d, cos)
+
+
+@pytest.mark.parametrize("nodes", [1, 7, 40])
+def test_verify_against_the_oracle(side, nodes):
+    abi, ora, talker, _ = side
+    rng = np.random.default_rng(nodes)
+    prompt = [rng.standard_normal((n, 1024)).astype(np.float32) for n in (37, 21)]
+    d = abi.DeviceBuffer(prompt[0].nbytes)
+    d.upload(prompt[0])
+    talker.prefill(d.ptr, 37)                                 # rows 0..36: pages 0, 1 and 2
+    pool = Pool(abi, talker, 2, {0: [0, 1, 2]})
+    pool.past.copy_(i32([37, 0]))
+    # the second prompt goes in as a chain of 21 rows, beside one row of the first request
+    first = rng.standard_normal((1, 1024)).astype(np.float32)
+    trees, x = [[-1], [j - 1 for j in range(21)]], [first, prompt[1]]
+    hid, lg = pool.step(trees, x)
+    check(ora, prompt[0], trees[0], first, hid[:1], lg[:1], "one row")
+    h, l = oracle_rows(ora, np.zeros((0, 1024), np.float32), prompt[1])
+    for got, want in ((hid[1:], h), (lg[1:], l)):
+        dmax, cos = compare(got, want)
+        assert dmax < TOL_ABS and cos > TOL_COS, ("chain", dmax, cos)
+    pool.commit([[0], list(range(21))], talker.kv)
+    history = [np.concatenate([prompt[0], first]), prompt[1]]
+    # trees on both, then one row each on what was accepted
+    for step in range(2):
+        trees = [random_tree(rng, nodes), random_tree(rng, max(1, nodes - 3))] if step == 0 else [[-1], [-1]]
+        x = [rng.standard_normal((len(t), 1024)).astype(np.float32) for t in trees]
+        hid, lg = pool.step(trees, x, spare=2)
+        at = 0
+        for i, t in enumerate(trees):
+            check(ora, history[i], t, x[i], hid[at:at + len(t)], lg[at:at + len(t)], ("request", i, "step", step))
+            at += len(t)
+        paths = [chain_of(t, len(t) - 1) for t in trees]
+        pool.commit(paths, talker.kv)
+        history = [np.concatenate([h, xi[p]]) for h, xi, p in zip(history, x, paths)]
+    log(f"verify {nodes} nodes: {talker.last_ms():.2f} ms for one row each")
+
+
+def test_a_row_does_not_depend_on_the_other_requests(side):
+    abi, _, talker, _ = side
+    rng = np.random.default_rng(5)
+    x = [rng.standard_normal((n, 1024)).astype(np.float32) for n in (5, 3, 8)]
+    trees = [[-1, 0, 1, 1, 2], [-1, 0, 0], [-1, 0, 1, 2, 3, 4, 5, 6]]
+    kv = abi.KvCache(talker.kv.n_layer, 512, 1024)            # a pool of the caller's
+    all_h, all_l = Pool(abi, talker, 3, {}).step(trees, x, kv=kv)
+    at = 0
+    for t, xi in zip(trees, x):
+        h, l = Pool(abi, talker, 1, {}).step([t], [xi], kv=kv)
+        # (the attention may add a long request's keys in another order: f32 sums)
+        assert np.abs(h - all_h[at:at + len(t)]).max() < 1e-3 and np.abs(l - all_l[at:at + len(t)]).max() < 1e-3
+        h2, _ = Pool(abi, talker, 1, {}).step([t], [xi], kv=kv, logits=False)
+        assert np.array_equal(h, h2)
+        at += len(t)
+
+
+def test_verify_after_a_long_prefill_and_refusals(side):
+    """A prefill above 64 rows leaves f16 pairs in the handle's buffers: rows of no request must not read them."""
+    abi, _, talker, _ = side
+    rng = np.random.default_rng(6)
+    p = rng.standard_normal((100, 1024)).astype(np.float32)
+    d = abi.DeviceBuffer(p.nbytes)
+    d.upload(p)
+    talker.prefill(d.ptr, 100)
+    pool = Pool(abi, talker, 1, {0: list(range(7))})
+    pool.past.copy_(i32([100]))
+    hid, lg = pool.step([[-1, 0]], [p[:2]], spare=11)
+    assert np.isfinite(hid[:2]).all() and np.isfinite(lg[:2]).all()
+    g, b = pool.pages, torch.zeros(64, 1024, device="cuda").data_ptr()
+
+    def refused(status, **kw):
+        a = dict(pages=g, max_keys=192, d_rows=b, d_hidden=b, kv=None)
+        a.update(kw)
+        with pytest.raises(abi.NaviError) as e:
+            talker.verify(**a)
+        assert e.value.status == status, e.value
+
+    def with_(**kw):
+        q = type(g).from_buffer_copy(g)
+        for k, v in kw.items():
+            setattr(q, k, v)
+        return q
+
+    refused(4, d_rows=None)
+    refused(4, d_hidden=None)
+    refused(4, d_hidden=b + 4)
+    refused(4, max_keys=0)
+    refused(4, max_keys=513)
+    refused(4, pages=with_(n_rows=129))
+    refused(4, pages=with_(n_rows=0))
+    refused(4, pages=with_(max_new=65))
+    refused(4, pages=with_(n_pages=33))
+    refused(4, kv=abi.KvCache(1, 512, 1024))
+    refused(4, kv=abi.KvCache(talker.kv.n_layer, 511, 1024))
+    x = np.full((1, 1024), 1e6, np.float32)                   # leaves the f16 range inside the layers
+    x[0, ::2] = np.nan
+    with pytest.raises(abi.NaviError) as e:
+        pool.step([[-1]], [x])
+    assert e.value.status == 4 and "f16 range" in str(e.value)
