@@ -25,6 +25,7 @@
 #include "tree.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace navi_amd {
 namespace tree {
@@ -42,13 +43,14 @@ constexpr float NONE = -INFINITY;
 struct Args {
     const void *q, *k, *v;
     void *out;
-    float *po, *pm;                    // split: partial sums [split][row * heads + head][D], then (reference, sum) pairs
+    float *po, *pm;                    // the parts of requests that are cut (part_of)
     const int32_t *table, *n_past, *cu;
     const uint64_t *mask;
-    int n, hkv, g, blocks, n_pages, n_rows, max_new, ldq, ldkv, ldo, splits, tiles, groups;   // tiles: of a split
+    int n, hkv, g, blocks, n_pages, n_rows, max_new, ldq, ldkv, ldo, workers, groups;
     int tiled;                         // f32 out: in the tile layout of rows.h, heads * D wide
+    int flip;                          // scale < 0: the scores' sign goes into q
     Div page, heads_per;               // heads_per: by g
-    float scale;                       // scale * log2 e
+    float scale;                       // |scale| * log2 e
 };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -110,9 +112,74 @@ __device__ __forceinline__ float row_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
-// PAIR: q and out are f32, q and p travel as hi + lo pairs. NT: 16-row query tiles of a block.
-template <class E, bool PAIR, int D, int NT>
-__global__ void __launch_bounds__(BT) k_tree(Args a) {
+// Where request `req` stands: its rows of the step, cached positions and positions in all.
+struct Where {
+    int c0, rows, past, len;
+};
+__device__ __forceinline__ Where where_is(const Args &a, int req) {
+    const int64_t room = min(static_cast<int64_t>(a.blocks) * a.page.d, static_cast<int64_t>(INT32_MAX - 4 * KT * NW));
+    Where w;
+    w.c0 = gld(a.cu + req);
+    const int count = max(min(gld(a.cu + req + 1), a.n_rows) - w.c0, 0);
+    w.rows = min(count, a.max_new);
+    w.past = static_cast<int>(min<int64_t>(max(gld(a.n_past + req), 0), room));
+    w.len = static_cast<int>(min<int64_t>(static_cast<int64_t>(w.past) + count, room));
+    return w;
+}
+
+// Requests of uneven length over evenly long chunks: with `workers` wanted blocks a kv head and query group, a chunk is
+// at most total / workers steps (of KT * NW keys), and a request is cut into as few even chunks of that as it takes:
+// at most workers + requests of them, in the requests' order.
+constexpr int MAXB = BT;               // most requests of a call that is cut
+struct Chunks {
+    int before[MAXB + 1];              // chunks before request i
+    int steps[MAXB];
+    Where at[MAXB];
+    int red[NW];
+    float sum[NW];
+};
+__device__ __forceinline__ int block_upto(int v, int *red) {
+    const int wv = threadIdx.x >> 6, upto = wave_incl_scan(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) red[wv] = upto;
+    __syncthreads();
+    int off = 0;
+#pragma unroll
+    for (int i = 0; i < NW - 1; ++i) off += i < wv ? red[i] : 0;
+    return off + upto;
+}
+__device__ __forceinline__ void lay_out(const Args &a, int qrow0, Chunks &q) {
+    const int t = threadIdx.x;
+    Where w{0, 0, 0, 0};
+    if (t < a.n) w = where_is(a, t);
+    const int steps = w.rows * a.g > qrow0 ? (w.len + KT * NW - 1) / (KT * NW) : 0;
+    // the steps in all, exact below 2^24; above (lengths out of all proportion) rounded up, so that the chunks stay as few
+    const float part = wave_sum(static_cast<float>(steps));
+    if ((t & 63) == 0) q.sum[t >> 6] = part;
+    __syncthreads();
+    float total = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) total += q.sum[i];
+    const int most = max(total < 16777216.f ? (static_cast<int>(total) + a.workers - 1) / a.workers
+                                            : static_cast<int>(total * 1.001f / static_cast<float>(a.workers)) + 1, 1);
+    const int chunks = block_upto((steps + most - 1) / most, q.red);
+    if (t == 0) q.before[0] = 0;
+    if (t < a.n) {
+        q.before[t + 1] = chunks;
+        q.steps[t] = steps;
+        q.at[t] = w;
+    }
+    __syncthreads();
+}
+// Where chunk k's part is kept: NT * 16 rows of [D], and (reference, sum) pairs.
+__device__ __forceinline__ size_t part_of(const Args &a, int kvh, int group, int k) {
+    return (static_cast<size_t>(kvh) * a.groups + group) * (a.workers + a.n) + k;
+}
+
+// PAIR: q and out are f32, q and p travel as hi + lo pairs. NT: 16-row query tiles of a block. CUT: a block takes a
+// chunk of a request's keys, else all of them.
+template <class E, bool PAIR, int D, int NT, bool CUT>
+__global__ void __launch_bounds__(BT, NT == 1 ? 3 : NT == 2 ? 2 : 1) k_tree(Args a) {
     typedef typename Types<E>::v8 v8;
     typedef typename Types<E>::v4 v4;
     constexpr int KS = D / 32, DT = D / 16;                      // MFMA steps of a score, column tiles of O
@@ -121,28 +188,43 @@ __global__ void __launch_bounds__(BT) k_tree(Args a) {
     constexpr int JOIN = NW * NT * 16 * CDP * 4;
     __shared__ __align__(16) unsigned char sm[NW * VB > JOIN ? NW * VB : JOIN];
     __shared__ float s_ref[NW][NT * 16], s_sum[NW][NT * 16];
+    constexpr int QP = PAIR ? 2 : 1;
+    __shared__ u32x4_t s_q[QP * NT * KS * WAVE];      // the operands of q, a pair's hi before its lo
 
     const int wv = threadIdx.x >> 6, l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
     int id = blockIdx.x;
     const int kvh = id % a.hkv;
     id /= a.hkv;
-    const int group = id % a.groups;
-    id /= a.groups;
-    const int split = id % a.splits, req = id / a.splits;
-
-    const int c0 = gld(a.cu + req), c1 = min(gld(a.cu + req + 1), a.n_rows);
-    const int rows = min(c1 - c0, a.max_new);
+    const int group = id % a.groups, unit = id / a.groups;
     const int qrow0 = group * NT * 16;
-    if (qrow0 >= rows * a.g) return;                              // uniform: this request has fewer rows
-    const int64_t room = min(static_cast<int64_t>(a.blocks) * a.page.d, static_cast<int64_t>(INT32_MAX - 2 * KT));
-    const int past = static_cast<int>(min<int64_t>(max(gld(a.n_past + req), 0), room));
-    const int len = static_cast<int>(min<int64_t>(static_cast<int64_t>(past) + max(c1 - c0, 0), room));
-    const int t_end_all = (len + KT - 1) / KT;
-    const int t0 = split * a.tiles, t_end = split == a.splits - 1 ? t_end_all : min(t_end_all, t0 + a.tiles);
-    if (t0 >= t_end && split > 0) return;                         // the join counts the splits as this does
 
-    // this lane's query rows (one a tile): their operands, masks, and factor of the scores
-    v8 qh[NT][KS], ql[PAIR ? NT : 1][PAIR ? KS : 1];
+    int req = unit, t0 = 0, t_end;
+    bool whole = true;                                            // the block has all of the request's keys
+    Where wh;
+    if constexpr (CUT) {
+        __shared__ Chunks s_c;
+        lay_out(a, qrow0, s_c);
+        if (unit >= s_c.before[a.n]) return;
+        int lo = 0, hi = a.n;                                     // before[lo] <= unit < before[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (s_c.before[mid] <= unit) lo = mid;
+            else hi = mid;
+        }
+        req = lo;
+        wh = s_c.at[req];
+        const int n = s_c.before[req + 1] - s_c.before[req], k = unit - s_c.before[req], steps = s_c.steps[req];
+        whole = n == 1;
+        t0 = static_cast<int>(static_cast<int64_t>(steps) * k / n) * NW;
+        t_end = min((wh.len + KT - 1) / KT, static_cast<int>(static_cast<int64_t>(steps) * (k + 1) / n) * NW);
+    } else {
+        wh = where_is(a, req);
+        if (qrow0 >= wh.rows * a.g) return;                       // uniform: this request has fewer rows
+        t_end = (wh.len + KT - 1) / KT;
+    }
+    const int c0 = wh.c0, rows = wh.rows, past = wh.past, len = wh.len;
+
+    // this lane's query rows (one a tile): masks and factor of the scores; the operands into LDS
     uint64_t seen[NT];
     float fac[NT];
 #pragma unroll
@@ -169,27 +251,35 @@ __global__ void __launch_bounds__(BT) k_tree(Args a) {
             top = row_max(top);
             const int ex = top > 0.f && top < INFINITY ? ilogbf(top) : 0;
             fac[nt] = ldexpf(a.scale, ex);
+            if (wv == 0) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
+                for (int s = 0; s < KS; ++s) {
+                    v8 qhi, qlo;
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float y = ldexpf(x[s][hf][e], -ex);
-                        const E hi = static_cast<E>(y);
-                        qh[nt][s][4 * hf + e] = hi;
-                        ql[nt][s][4 * hf + e] = static_cast<E>(y - static_cast<float>(hi));
+                    for (int e = 0; e < 8; ++e) {
+                        const float y = ldexpf(a.flip ? -x[s][e >> 2][e & 3] : x[s][e >> 2][e & 3], -ex);
+                        qhi[e] = static_cast<E>(y);
+                        qlo[e] = static_cast<E>(y - static_cast<float>(qhi[e]));
                     }
+                    s_q[(nt * KS + s) * WAVE + l] = bits<u32x4_t>(qhi);
+                    s_q[((NT + nt) * KS + s) * WAVE + l] = bits<u32x4_t>(qlo);
+                }
+            }
         } else {
             const E *q = static_cast<const E *>(a.q) + at;
+            if (wv == 0) {
+                const uint32_t sign = a.flip ? 0x80008000u : 0u;
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-                qh[nt][s] = bits<v8>(on ? *(const NAVI_GLOBAL u32x4_t *) (q + 32 * s) : u32x4_t{0u, 0u, 0u, 0u});
+                for (int s = 0; s < KS; ++s)
+                    s_q[(nt * KS + s) * WAVE + l] = on ? *(const NAVI_GLOBAL u32x4_t *) (q + 32 * s) ^ sign : u32x4_t{0u, 0u, 0u, 0u};
+            }
         }
+        // a factor of 0 (all scores alike) as the least normal number: -inf, a place not seen, must stay -inf
+        fac[nt] = fmaxf(fac[nt], 1.17549435e-38f);
     }
 
     f32x4_t acc[NT][DT];
-    float ref[NT], sub[NT], sum[NT];                              // ref: the reference + SLACK; sub: reference - LIFT
+    float ref[NT], sub[NT], sum[NT];                          // ref: the reference + SLACK; sub: reference - LIFT
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         ref[nt] = NONE;
@@ -201,14 +291,14 @@ __global__ void __launch_bounds__(BT) k_tree(Args a) {
     unsigned char *buf = sm + wv * VB;
     const E *kb = static_cast<const E *>(a.k) + kvh * D + 8 * lg, *vb = static_cast<const E *>(a.v) + kvh * D + 8 * lg;
     const int32_t *table = a.table + static_cast<size_t>(req) * a.blocks;
-    // slot of key `key`, or -1 past the end and outside the pool
-    auto slot_of = [&](int key) {
-        const int b = div_by(a.page, key);
-        const int p = key < len ? gld(table + b) : -1;
-        return static_cast<unsigned>(p) < static_cast<unsigned>(a.n_pages) ? p * static_cast<int>(a.page.d) + key - b * static_cast<int>(a.page.d) : -1;
+    // page and place in it of key `key`; slot: its row, or -1 past the end and outside the pool
+    auto page_of = [&](int key) { return key < len ? gld(table + div_by(a.page, key)) : -1; };
+    auto slot_of = [&](int key, int p) {
+        return static_cast<unsigned>(p) < static_cast<unsigned>(a.n_pages)
+                   ? p * static_cast<int>(a.page.d) + key - div_by(a.page, key) * static_cast<int>(a.page.d) : -1;
     };
     u32x4_t kr[2][KS], vr[2][KS];
-    int slot[2];
+    int slot[2], page[2];
     auto load_kv = [&]() {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
@@ -223,15 +313,22 @@ __global__ void __launch_bounds__(BT) k_tree(Args a) {
     int t = t0 + wv;
     if (t < t_end) {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) slot[kt] = slot_of(t * KT + kt * 16 + lr);
+        for (int kt = 0; kt < 2; ++kt) page[kt] = page_of(t * KT + kt * 16 + lr);
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) slot[kt] = slot_of(t * KT + kt * 16 + lr, page[kt]);
         load_kv();
+        if (t + NW < t_end)                                   // pages are looked up two tiles ahead
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) page[kt] = page_of((t + NW) * KT + kt * 16 + lr);
     }
+    __syncthreads();                                              // the operands of q
     for (; t < t_end; t += NW) {
         // keys of this tile that exist (uniform), and whether any row may not see one
-        const uint32_t there = static_cast<uint32_t>(__ballot(slot[0] >= 0) & 0xFFFFu) | static_cast<uint32_t>(__ballot(slot[1] >= 0) & 0xFFFFu) << 16;
-        const bool tree_tile = (t + 1) * KT > past, masked = tree_tile || there != 0xFFFFFFFFu;
+        const uint32_t there =
+            static_cast<uint32_t>(__ballot(slot[0] >= 0) & 0xFFFFu) | static_cast<uint32_t>(__ballot(slot[1] >= 0) & 0xFFFFu) << 16;
+        const bool masked = (t + 1) * KT > past || there != 0xFFFFFFFFu;
         // V rows into LDS: 32-byte chunk i of key r at chunk i ^ (r & 7)
-        uint32_t special = 0;                                     // drafted keys with an infinity or NaN in V
+        uint32_t special = 0;                                 // drafted keys with an infinity or NaN in V
         if (masked) {
             bool sp[2] = {false, false};
 #pragma unroll
@@ -262,93 +359,129 @@ __global__ void __launch_bounds__(BT) k_tree(Args a) {
             }
         // scores
         f32x4_t sc[NT][2];
+        asm volatile("" ::: "memory");                        // or the operands would be kept in registers after all
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        // the operands of a step are read while the step before is multiplied
+        v8 qb[2][QP * NT];
+        auto load_q = [&](int s) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                f32x4_t z{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < QP * NT; ++i) qb[s & 1][i] = bits<v8>(s_q[(i * KS + s) * WAVE + l]);
+        };
+        load_q(0);
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    z = Types<E>::mfma(bits<v8>(kr[kt][s]), qh[nt][s], z);
-                    if constexpr (PAIR) z = Types<E>::mfma(bits<v8>(kr[kt][s]), ql[nt][s], z);
-                }
-                sc[nt][kt] = z;
-            }
+        for (int s = 0; s < KS; ++s) {
+            if (s + 1 < KS) load_q(s + 1);
+#pragma unroll
+            for (int i = 0; i < QP * NT; ++i)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) sc[i % NT][kt] = Types<E>::mfma(bits<v8>(kr[kt][s]), qb[s & 1][i], sc[i % NT][kt]);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, QP * NT, 0);          // LDS reads
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            __builtin_amdgcn_sched_group_barrier(0x100, QP * NT, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 2 * QP * NT, 0);  // MFMAs
+        }
         // the next tile's rows, in flight from here
-        const int spec_slot0 = slot[0], spec_slot1 = slot[1];
+        const int was0 = slot[0], was1 = slot[1];
         if (t + NW < t_end) {
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) slot[kt] = slot_of((t + NW) * KT + kt * 16 + lr);
+            for (int kt = 0; kt < 2; ++kt) slot[kt] = slot_of((t + NW) * KT + kt * 16 + lr, page[kt]);
             load_kv();
+            if (t + 2 * NW < t_end)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) page[kt] = page_of((t + 2 * NW) * KT + kt * 16 + lr);
         }
         // p
-        v8 ph[NT], pl[PAIR ? NT : 1];
-        float pf[NT][8];
+        if (masked) {
+            // bit k of `vis`: key k of the tile; the tile begins `ahead` positions after the first drafted one
+            const int ahead = t * KT - past;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                uint32_t vis = ahead >= 64 ? 0u : ahead >= 0 ? static_cast<uint32_t>(seen[nt] >> ahead)
+                             : ahead <= -KT ? ~0u : static_cast<uint32_t>(seen[nt] << -ahead) | ((1u << -ahead) - 1u);
+                vis = (vis & there) >> (4 * lg);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sc[nt][i >> 2][i & 3] = vis >> ((i >> 2) * 16 + (i & 3)) & 1u ? sc[nt][i >> 2][i & 3] : NONE;
+            }
+        }
+        // the reference follows where a score passes it by more than SLACK (one test for all query tiles, so
+        // that what follows is one straight run of instructions)
+        float top[NT];
+        bool passed = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float top = NONE;
+            top[nt] = NONE;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float x = sc[nt][i >> 2][i & 3] * fac[nt];
-                if (masked) {
-                    const int kin = (i >> 2) * 16 + 4 * lg + (i & 3), ahead = t * KT + kin - past;
-                    const bool vis = (there >> kin & 1) && (ahead < 0 || (ahead < 64 && (seen[nt] >> (ahead & 63) & 1)));
-                    x = vis ? x : NONE;
-                }
-                pf[nt][i] = x;
-                top = fmaxf(top, x);
-            }
-            if (__ballot(top > ref[nt])) {
-                const float mx = row_max(top);
-                if (mx > ref[nt]) {
-                    const float f = ref[nt] == NONE ? 0.f : __builtin_amdgcn_exp2f(ref[nt] - SLACK - mx);
-                    sum[nt] *= f;
+            for (int i = 0; i < 8; ++i) top[nt] = fmaxf(top[nt], sc[nt][i >> 2][i & 3]);
+            passed |= top[nt] * fac[nt] > ref[nt];
+        }
+        if (__ballot(passed)) {
 #pragma unroll
-                    for (int d = 0; d < DT; ++d) acc[nt][d] *= f;
-                    ref[nt] = mx + SLACK;
-                    sub[nt] = mx - LIFT;
-                }
-            }
+            for (int nt = 0; nt < NT; ++nt) {
+                const float mx = row_max(top[nt]) * fac[nt];
+                const bool up = mx > ref[nt];
+                const float f = !up ? 1.f : ref[nt] == NONE ? 0.f : __builtin_amdgcn_exp2f(ref[nt] - SLACK - mx);
+                sum[nt] *= f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float p = __builtin_amdgcn_exp2f(pf[nt][i] - sub[nt]);
-                sum[nt] += p;
-                pf[nt][i] = p;
-                const E hi = static_cast<E>(p);
-                ph[nt][i] = hi;
-                if constexpr (PAIR) pl[nt][i] = static_cast<E>(p - static_cast<float>(hi));
+                for (int d = 0; d < DT; ++d) acc[nt][d] *= f;
+                ref[nt] = up ? mx + SLACK : ref[nt];
+                sub[nt] = up ? mx - LIFT : sub[nt];
             }
         }
         // O^T += V^T P^T
+        v8 va[DT];
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-            v8 va;
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
                 const int r = kt * 16 + 4 * lg + (lr >> 2);
                 const v4 x = bits<v4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16(
                     (__attribute__((address_space(3))) s16x4 *) (buf + r * (D * 2) + ((d ^ (r & (DT - 1))) << 5) + ((lr & 3) << 3))));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) va[4 * kt + e] = x[e];
+                for (int e = 0; e < 4; ++e) va[d][4 * kt + e] = x[e];
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                acc[nt][d] = Types<E>::mfma(va, ph[nt], acc[nt][d]);
-                if constexpr (PAIR) acc[nt][d] = Types<E>::mfma(va, pl[nt], acc[nt][d]);
+        for (int nt = 0; nt < NT; ++nt) {
+            v8 ph, pl;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[nt][i >> 2][i & 3], fac[nt], -sub[nt]));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[nt][i >> 2][(i & 3) + 1], fac[nt], -sub[nt]));
+                sc[nt][i >> 2][i & 3] = p0;
+                sc[nt][i >> 2][(i & 3) + 1] = p1;
+                sum[nt] += p0 + p1;
+                if constexpr (PAIR) {
+                    // hi truncated, two at once; lo is the exact rest, rounded
+                    const auto hi = bits<half2_t>(__builtin_amdgcn_cvt_pkrtz(p0, p1));
+                    ph[i] = hi[0];
+                    ph[i + 1] = hi[1];
+                    pl[i] = static_cast<E>(p0 - static_cast<float>(hi[0]));
+                    pl[i + 1] = static_cast<E>(p1 - static_cast<float>(hi[1]));
+                } else {
+                    ph[i] = static_cast<E>(p0);
+                    ph[i + 1] = static_cast<E>(p1);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                acc[nt][d] = Types<E>::mfma(va[d], ph, acc[nt][d]);
+                if constexpr (PAIR) acc[nt][d] = Types<E>::mfma(va[d], pl, acc[nt][d]);
             }
         }
         // Drafted keys with an infinity or NaN in V (rare): zeros in the products above, since 0 times
         // one would reach the rows that do not see them; here only the rows that do see them add theirs.
         if (special) {
-            float *ps = reinterpret_cast<float *>(buf);           // [query row][key]
+            float *ps = reinterpret_cast<float *>(buf);       // [query row][key]
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) ps[(nt * 16 + lr) * KT + (i >> 2) * 16 + 4 * lg + (i & 3)] = pf[nt][i];
+                for (int i = 0; i < 8; ++i) ps[(nt * 16 + lr) * KT + (i >> 2) * 16 + 4 * lg + (i & 3)] = sc[nt][i >> 2][i & 3];
             __builtin_amdgcn_wave_barrier();
             for (uint32_t rest = special; rest; rest &= rest - 1) {
                 const int kin = __builtin_ctz(rest), ahead = t * KT + kin - past;
-                const int sl = __shfl(kin < 16 ? spec_slot0 : spec_slot1, kin & 15);
+                const int sl = __shfl(kin < 16 ? was0 : was1, kin & 15);
                 const E *vp = static_cast<const E *>(a.v) + static_cast<size_t>(max(sl, 0)) * a.ldkv + kvh * D + 4 * lg;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -375,7 +508,7 @@ __global__ void __launch_bounds__(BT) k_tree(Args a) {
             s_sum[wv][nt * 16 + lr] = sum[nt];
         }
     }
-    __syncthreads();                                              // and every wave is done with its buffer
+    __syncthreads();                                          // and every wave is done with its buffer
     float own[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -386,14 +519,15 @@ __global__ void __launch_bounds__(BT) k_tree(Args a) {
         own[nt] = ref[nt] == NONE ? 0.f : __builtin_amdgcn_exp2f(ref[nt] - m);
     }
     float *js = reinterpret_cast<float *>(sm);
+    const size_t part = CUT ? part_of(a, kvh, group, unit) * (NT * 16) : 0;
 #pragma unroll
-    for (int part = 0; part < NT; ++part) {                       // CD columns at a time
-        if (part) __syncthreads();
+    for (int cols = 0; cols < NT; ++cols) {                   // CD columns at a time
+        if (cols) __syncthreads();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int d = 0; d < DT / NT; ++d)
-                *reinterpret_cast<f32x4_t *>(js + (wv * NT * 16 + nt * 16 + lr) * CDP + d * 16 + 4 * lg) = acc[nt][part * (DT / NT) + d] * own[nt];
+                *reinterpret_cast<f32x4_t *>(js + (wv * NT * 16 + nt * 16 + lr) * CDP + d * 16 + 4 * lg) = acc[nt][cols * (DT / NT) + d] * own[nt];
         __syncthreads();
         for (int i = threadIdx.x; i < NT * 16 * (CD / 4); i += BT) {
             const int r = i / (CD / 4), c = i % (CD / 4) * 4, m = qrow0 + r, j = div_by(a.heads_per, m);
@@ -408,13 +542,12 @@ __global__ void __launch_bounds__(BT) k_tree(Args a) {
             float total = 0.f;
 #pragma unroll
             for (int w = 0; w < NW; ++w) total += s_ref[w][r] == NONE ? 0.f : s_sum[w][r] * __builtin_amdgcn_exp2f(s_ref[w][r] - mx);
-            const int head = kvh * a.g + m - j * a.g, col = part * CD + c;
-            if (a.splits > 1) {
-                const size_t at = (static_cast<size_t>(split) * a.n_rows + c0 + j) * (a.hkv * a.g) + head;
-                st4(a.po + at * D + col, o);
+            const int head = kvh * a.g + m - j * a.g, col = cols * CD + c;
+            if (CUT && !whole) {
+                st4(a.po + (part + r) * D + col, o);
                 if (col == 0) {
-                    gst(a.pm + 2 * at, mx);
-                    gst(a.pm + 2 * at + 1, total);
+                    gst(a.pm + 2 * (part + r), mx);
+                    gst(a.pm + 2 * (part + r) + 1, total);
                 }
             } else {
                 const float inv = mx == NONE ? 0.f : 1.f / total;
@@ -424,64 +557,104 @@ __global__ void __launch_bounds__(BT) k_tree(Args a) {
     }
 }
 
-// Joins the splits of every row in split order: block (head and column tile, row of the request, request).
+// Joins the parts of the requests that were cut, in their order: a wave takes a query row, D / 8 lanes its
+// columns and the others further parts. Block (request x kv head x group, rows).
 template <class E, bool PAIR, int D>
-__global__ void __launch_bounds__(BT) k_tree_join(Args a) {
-    const int req = blockIdx.z, j = blockIdx.y, heads = a.hkv * a.g;
-    const int c0 = gld(a.cu + req), c1 = min(gld(a.cu + req + 1), a.n_rows);
-    if (j >= c1 - c0) return;
-    const int i = blockIdx.x * BT + threadIdx.x, head = i / (D / 4), col = i % (D / 4) * 4;
-    if (head >= heads) return;
-    const int64_t room = min(static_cast<int64_t>(a.blocks) * a.page.d, static_cast<int64_t>(INT32_MAX - 2 * KT));
-    const int past = static_cast<int>(min<int64_t>(max(gld(a.n_past + req), 0), room));
-    const int len = static_cast<int>(min<int64_t>(static_cast<int64_t>(past) + (c1 - c0), room));
-    const int n = max(1, min(a.splits, ((len + KT - 1) / KT + a.tiles - 1) / a.tiles));
-    const size_t step = static_cast<size_t>(a.n_rows) * heads, at = static_cast<size_t>(c0 + j) * heads + head;
-    float m = NONE;
-    for (int s = 0; s < n; ++s) m = fmaxf(m, gld(a.pm + 2 * (s * step + at)));
-    f32x4_t o{0.f, 0.f, 0.f, 0.f};
-    float total = 0.f;
-    for (int s = 0; s < n; ++s) {
-        const float r = gld(a.pm + 2 * (s * step + at)), z = gld(a.pm + 2 * (s * step + at) + 1);
-        const f32x4_t x = ld4(a.po + (s * step + at) * D + col);
-        const float f = r == NONE ? 0.f : __builtin_amdgcn_exp2f(r - m);
-        total += f * z;
-        o += x * f;
+__global__ void __launch_bounds__(BT) k_tree_join(Args a, int nt16) {
+    constexpr int CL = D / 8, PL = WAVE / CL;
+    __shared__ Chunks seq;
+    const int l = threadIdx.x & 63, c = l % CL, pl = l / CL;
+    int id = blockIdx.x;
+    const int kvh = id % a.hkv;
+    id /= a.hkv;
+    const int group = id % a.groups, req = id / a.groups, qrow0 = group * nt16;
+    lay_out(a, qrow0, seq);
+    const int k0 = seq.before[req], k1 = seq.before[req + 1];
+    if (k1 - k0 < 2) return;                                      // a block had all of it and has stored it
+    const Where wh = seq.at[req];
+    const int left = min(nt16, wh.rows * a.g - qrow0);
+    for (int r = blockIdx.y * NW + (threadIdx.x >> 6); r < left; r += gridDim.y * NW) {
+        float m = NONE, sum = 0.f;
+        f32x4_t o[2] = {f32x4_t{0.f, 0.f, 0.f, 0.f}, f32x4_t{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll 4
+        for (int k = k0 + pl; k < k1; k += PL) {
+            const size_t at = part_of(a, kvh, group, k) * nt16 + r;
+            const float ref = gld(a.pm + 2 * at), z = gld(a.pm + 2 * at + 1);
+            const f32x4_t x0 = ld4(a.po + at * D + 8 * c), x1 = ld4(a.po + at * D + 8 * c + 4);
+            const float top = fmaxf(m, ref);
+            const float fo = m == NONE ? 0.f : __builtin_amdgcn_exp2f(m - top), fx = ref == NONE ? 0.f : __builtin_amdgcn_exp2f(ref - top);
+            m = top;
+            sum = sum * fo + z * fx;
+            o[0] = o[0] * fo + x0 * fx;
+            o[1] = o[1] * fo + x1 * fx;
+        }
+        float top = m;
+#pragma unroll
+        for (int x = CL; x < WAVE; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+        const float f = m == NONE ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        sum *= f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i >> 2][i & 3] *= f;
+#pragma unroll
+        for (int x = CL; x < WAVE; x <<= 1) {
+            sum += __shfl_xor(sum, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i >> 2][i & 3] += __shfl_xor(o[i >> 2][i & 3], x);
+        }
+        if (pl == 0) {
+            const int mrow = qrow0 + r, j = div_by(a.heads_per, mrow), head = kvh * a.g + mrow - j * a.g;
+            const float inv = top == NONE ? 0.f : 1.f / sum;
+            store_out<E, PAIR>(a, wh.c0 + j, head * D + 8 * c, a.hkv * a.g * D, o[0] * inv);
+            store_out<E, PAIR>(a, wh.c0 + j, head * D + 8 * c + 4, a.hkv * a.g * D, o[1] * inv);
+        }
     }
-    store_out<E, PAIR>(a, c0 + j, head * D + col, heads * D, o * (m == NONE ? 0.f : 1.f / total));
 }
 
-// How a call is cut: query tiles of a block, groups of them, splits of the keys and 32-key tiles of a split.
+// How a call is cut: query tiles of a block, groups of them, and blocks wanted for a kv head and group (0: one a request).
 struct Cut {
-    int nt, groups, splits, tiles;
+    int nt, groups, workers;
 };
 Cut cut_of(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys) {
     const int m = std::min(p.max_new, 64) * (h.n_head / h.n_kv_head);
     Cut c;
     c.nt = m <= 16 ? 1 : m <= 32 ? 2 : 4;
     c.groups = (m + 16 * c.nt - 1) / (16 * c.nt);
-    const int64_t units = static_cast<int64_t>(p.n_requests) * h.n_kv_head * c.groups;
-    const int all = (max_keys + KT - 1) / KT;
-    const int64_t want = std::max<int64_t>(1, 512 / units);
-    c.tiles = std::max(NW, static_cast<int>((all + want - 1) / want + NW - 1) / NW * NW);
-    c.splits = std::max(1, (all + c.tiles - 1) / c.tiles);
+    const int64_t heads = static_cast<int64_t>(h.n_kv_head) * c.groups;
+    const int steps = (max_keys + KT * NW - 1) / (KT * NW);
+    // A block a request where no request can be long and there are blocks for all CUs (32 requests of 1024 keys: 30.0 us,
+    // cut 33.2: the chunks and the join), or more requests than a block lays out. Else two blocks a CU, or the one that
+    // fits with four query tiles.
+    if (p.n_requests > MAXB || steps == 1 || (steps <= 16 && p.n_requests * heads >= 256)) {
+        c.workers = 0;
+        return c;
+    }
+    const int64_t blocks = c.nt == 4 ? 256 : 512;
+    c.workers = static_cast<int>(std::max<int64_t>(1, std::min((blocks + heads - 1) / heads, static_cast<int64_t>(steps) * p.n_requests)));
     return c;
 }
 
 size_t workspace(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys) {
     const Cut c = cut_of(p, h, max_keys);
-    if (c.splits == 1) return 0;
-    return static_cast<size_t>(c.splits) * p.n_rows * h.n_head * (h.head_dim + 2) * sizeof(float);
+    if (c.workers == 0) return 0;
+    return static_cast<size_t>(h.n_kv_head) * c.groups * (c.workers + p.n_requests) * (c.nt * 16) * (h.head_dim + 2) * sizeof(float);
+}
+
+template <class E, bool PAIR, int D, int NT>
+void launch_nt(const Args &a, const Cut &c, hipStream_t s) {
+    if (c.workers == 0) {
+        hipLaunchKernelGGL((k_tree<E, PAIR, D, NT, false>), dim3(static_cast<unsigned>(a.n) * a.groups * a.hkv), dim3(BT), 0, s, a);
+        return;
+    }
+    hipLaunchKernelGGL((k_tree<E, PAIR, D, NT, true>), dim3(static_cast<unsigned>(c.workers + a.n) * a.groups * a.hkv), dim3(BT), 0, s, a);
+    const unsigned units = static_cast<unsigned>(a.n) * a.groups * a.hkv;
+    hipLaunchKernelGGL((k_tree_join<E, PAIR, D>), dim3(units, std::max(1u, std::min(NT * 16u / NW, 1024u / units))), dim3(BT), 0, s, a, NT * 16);
 }
 
 template <class E, bool PAIR, int D>
 void launch_as(const Args &a, const Cut &c, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.n) * c.splits * c.groups * a.hkv));
-    if (c.nt == 1) hipLaunchKernelGGL((k_tree<E, PAIR, D, 1>), grid, dim3(BT), 0, s, a);
-    else if (c.nt == 2) hipLaunchKernelGGL((k_tree<E, PAIR, D, 2>), grid, dim3(BT), 0, s, a);
-    else hipLaunchKernelGGL((k_tree<E, PAIR, D, 4>), grid, dim3(BT), 0, s, a);
-    if (c.splits > 1)
-        hipLaunchKernelGGL((k_tree_join<E, PAIR, D>), dim3((a.hkv * a.g * (D / 4) + BT - 1) / BT, a.max_new, a.n), dim3(BT), 0, s, a);
+    if (c.nt == 1) launch_nt<E, PAIR, D, 1>(a, c, s);
+    else if (c.nt == 2) launch_nt<E, PAIR, D, 2>(a, c, s);
+    else launch_nt<E, PAIR, D, 4>(a, c, s);
 }
 
 void launch(const Call &x, hipStream_t s) {
@@ -494,7 +667,7 @@ void launch(const Call &x, hipStream_t s) {
     a.v = x.v;
     a.out = x.out;
     a.po = static_cast<float *>(x.ws);
-    a.pm = a.po ? a.po + static_cast<size_t>(c.splits) * p.n_rows * h.n_head * h.head_dim : nullptr;
+    a.pm = a.po ? a.po + static_cast<size_t>(h.n_kv_head) * c.groups * (c.workers + p.n_requests) * (c.nt * 16) * h.head_dim : nullptr;
     a.table = p.block_table;
     a.n_past = p.n_past;
     a.cu = p.cu_rows;
@@ -509,13 +682,13 @@ void launch(const Call &x, hipStream_t s) {
     a.ldq = x.ldq;
     a.ldkv = x.ldkv;
     a.ldo = x.ldo;
-    a.splits = c.splits;
-    a.tiles = c.tiles;
+    a.workers = c.workers;
     a.groups = c.groups;
     a.tiled = x.tiled;
     a.page = kv::make_div(static_cast<uint32_t>(p.page_size));
     a.heads_per = kv::make_div(static_cast<uint32_t>(a.g));
-    a.scale = x.scale * 1.44269504088896340736f;
+    a.flip = x.scale < 0.f;
+    a.scale = std::fabs(x.scale) * 1.44269504088896340736f;
     const bool pair = x.q_dtype == NAVI_DT_F32, bf = h.kv_dtype == NAVI_DT_BF16;
     if (h.head_dim == 128) {
         if (pair) launch_as<_Float16, true, 128>(a, c, s);
