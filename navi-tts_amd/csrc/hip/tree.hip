@@ -33,7 +33,14 @@ namespace tree {
 using kv::Div;
 using kv::div_by;
 
-constexpr int NW = 4, BT = NW * WAVE;  // waves of a block
+constexpr int NW = 4, BT = NW * WAVE;  // waves of a block of k_tree_join
+// Of k_tree: eight, more loads on their way, where a block has a whole request (32 requests of 1024 keys: 27.3 us, with four
+// 31.0); four, and twice as many blocks, where requests are cut (64 ragged ones of up to 8000 keys: 73 us, with eight 85).
+constexpr int alone_of(bool cut) { return cut ? 4 : 8; }
+// Of k_tree_rows, RW waves of which share their query rows' tiles: eight, one block a CU, so that half as many parts of
+// a cut request are stored and joined (64 drafted rows over 32768 keys: 57 us, with four 64); four where two waves share and
+// the registers allow two blocks a CU (64 requests x 24 rows over 8192 keys: 401 us, with eight 417).
+constexpr int waves_of(bool pair, int rw) { return rw == 2 && !pair ? 4 : 8; }
 constexpr int KT = 32;                 // keys of a wave's tile
 // p = 2^(s - reference + LIFT): at most 2^(SLACK + LIFT) = 2^14, inside f16, and f16's full precision down to
 // 2^-24 of the reference instead of 2^-14.
@@ -46,7 +53,7 @@ struct Args {
     float *po, *pm;                    // the parts of requests that are cut (part_of)
     const int32_t *table, *n_past, *cu;
     const uint64_t *mask;
-    int n, hkv, g, blocks, n_pages, n_rows, max_new, ldq, ldkv, ldo, workers, groups;
+    int n, hkv, g, blocks, n_pages, n_rows, max_new, ldq, ldkv, ldo, workers, groups, step;
     int tiled;                         // f32 out: in the tile layout of rows.h, heads * D wide
     int flip;                          // scale < 0: the scores' sign goes into q
     Div page, heads_per;               // heads_per: by g
@@ -128,7 +135,7 @@ __device__ __forceinline__ Where where_is(const Args &a, int req) {
 }
 
 // Requests of uneven length over evenly long chunks: with `workers` wanted blocks a kv head and query group, a chunk is
-// at most total / workers steps (of KT * NW keys), and a request is cut into as few even chunks of that as it takes:
+// at most total / workers steps (of a.step 32-key tiles), and a request is cut into as few even chunks of that as it takes:
 // at most workers + requests of them, in the requests' order.
 constexpr int MAXB = BT;               // most requests of a call that is cut
 struct Chunks {
@@ -138,276 +145,201 @@ struct Chunks {
     int red[NW];
     float sum[NW];
 };
-__device__ __forceinline__ int block_upto(int v, int *red) {
-    const int wv = threadIdx.x >> 6, upto = wave_incl_scan(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 63) red[wv] = upto;
-    __syncthreads();
-    int off = 0;
-#pragma unroll
-    for (int i = 0; i < NW - 1; ++i) off += i < wv ? red[i] : 0;
-    return off + upto;
+__device__ __forceinline__ int steps_of(const Args &a, const Where &w, int qrow0) {
+    const int tiles = w.rows * a.g > qrow0 ? (w.len + KT - 1) / KT : 0;
+    return (tiles + a.step - 1) / a.step;
 }
-__device__ __forceinline__ void lay_out(const Args &a, int qrow0, Chunks &q) {
-    const int t = threadIdx.x;
-    Where w{0, 0, 0, 0};
-    if (t < a.n) w = where_is(a, t);
-    const int steps = w.rows * a.g > qrow0 ? (w.len + KT * NW - 1) / (KT * NW) : 0;
+__device__ __forceinline__ int chunk_steps(const Args &a, float total) {
     // the steps in all, exact below 2^24; above (lengths out of all proportion) rounded up, so that the chunks stay as few
+    return max(total < 16777216.f ? (static_cast<int>(total) + a.workers - 1) / a.workers
+                                  : static_cast<int>(total * 1.001f / static_cast<float>(a.workers)) + 1, 1);
+}
+// The first BT threads have a request each; all of a block's threads call it.
+__device__ __forceinline__ void lay_out(const Args &a, int qrow0, Chunks &q) {
+    const int t = threadIdx.x, wv = t >> 6;
+    const bool own = t < a.n;
+    Where w{0, 0, 0, 0};
+    if (own) w = where_is(a, t);
+    const int steps = steps_of(a, w, qrow0);
+    if (a.n == 1) {                                               // nothing to add up
+        if (own) {
+            q.before[0] = 0;
+            const int most = chunk_steps(a, static_cast<float>(steps));
+            q.before[1] = (steps + most - 1) / most;
+            q.steps[0] = steps;
+            q.at[0] = w;
+        }
+        __syncthreads();
+        return;
+    }
     const float part = wave_sum(static_cast<float>(steps));
-    if ((t & 63) == 0) q.sum[t >> 6] = part;
+    if ((t & 63) == 0 && wv < NW) q.sum[wv] = part;
     __syncthreads();
     float total = 0.f;
 #pragma unroll
     for (int i = 0; i < NW; ++i) total += q.sum[i];
-    const int most = max(total < 16777216.f ? (static_cast<int>(total) + a.workers - 1) / a.workers
-                                            : static_cast<int>(total * 1.001f / static_cast<float>(a.workers)) + 1, 1);
-    const int chunks = block_upto((steps + most - 1) / most, q.red);
+    const int most = chunk_steps(a, total), upto = wave_incl_scan((steps + most - 1) / most);
+    if ((t & 63) == 63 && wv < NW) q.red[wv] = upto;
+    __syncthreads();
+    int off = 0;
+#pragma unroll
+    for (int i = 0; i < NW - 1; ++i) off += i < wv ? q.red[i] : 0;
     if (t == 0) q.before[0] = 0;
-    if (t < a.n) {
-        q.before[t + 1] = chunks;
+    if (own) {
+        q.before[t + 1] = off + upto;
         q.steps[t] = steps;
         q.at[t] = w;
     }
     __syncthreads();
 }
-// Where chunk k's part is kept: NT * 16 rows of [D], and (reference, sum) pairs.
+// Where chunk k's part is kept: the group's rows of [D], and (reference, sum) pairs.
 __device__ __forceinline__ size_t part_of(const Args &a, int kvh, int group, int k) {
     return (static_cast<size_t>(kvh) * a.groups + group) * (a.workers + a.n) + k;
 }
 
-// PAIR: q and out are f32, q and p travel as hi + lo pairs. NT: 16-row query tiles of a block. CUT: a block takes a
-// chunk of a request's keys, else all of them.
-template <class E, bool PAIR, int D, int NT, bool CUT>
-__global__ void __launch_bounds__(BT, NT == 1 ? 3 : NT == 2 ? 2 : 1) k_tree(Args a) {
-    typedef typename Types<E>::v8 v8;
-    typedef typename Types<E>::v4 v4;
-    constexpr int KS = D / 32, DT = D / 16;                      // MFMA steps of a score, column tiles of O
-    constexpr int VB = KT * D * 2 > NT * 16 * KT * 4 ? KT * D * 2 : NT * 16 * KT * 4;   // a wave's buffer, bytes
-    constexpr int CD = D / NT, CDP = CD + 4;                     // columns joined at a time, padded
-    constexpr int JOIN = NW * NT * 16 * CDP * 4;
-    __shared__ __align__(16) unsigned char sm[NW * VB > JOIN ? NW * VB : JOIN];
-    __shared__ float s_ref[NW][NT * 16], s_sum[NW][NT * 16];
-    constexpr int QP = PAIR ? 2 : 1;
-    __shared__ u32x4_t s_q[QP * NT * KS * WAVE];      // the operands of q, a pair's hi before its lo
-
-    const int wv = threadIdx.x >> 6, l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+// A block's share of the work: a request, its tiles t0 .. t_end - 1, and whether these are all it has.
+struct Share {
+    Where at;
+    int kvh, group, unit, req, t0, t_end;
+    bool whole, none;
+};
+template <bool CUT>
+__device__ __forceinline__ Share share_of(const Args &a, int group_rows) {
+    Share s;
     int id = blockIdx.x;
-    const int kvh = id % a.hkv;
+    s.kvh = id % a.hkv;
     id /= a.hkv;
-    const int group = id % a.groups, unit = id / a.groups;
-    const int qrow0 = group * NT * 16;
-
-    int req = unit, t0 = 0, t_end;
-    bool whole = true;                                            // the block has all of the request's keys
-    Where wh;
+    s.group = id % a.groups;
+    s.unit = s.req = id / a.groups;
+    s.t0 = 0;
+    s.whole = true;
     if constexpr (CUT) {
-        __shared__ Chunks s_c;
-        lay_out(a, qrow0, s_c);
-        if (unit >= s_c.before[a.n]) return;
+        __shared__ Chunks c;
+        lay_out(a, s.group * group_rows, c);
+        s.none = s.unit >= c.before[a.n];
+        if (s.none) return s;
         int lo = 0, hi = a.n;                                     // before[lo] <= unit < before[hi]
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (s_c.before[mid] <= unit) lo = mid;
+            if (c.before[mid] <= s.unit) lo = mid;
             else hi = mid;
         }
-        req = lo;
-        wh = s_c.at[req];
-        const int n = s_c.before[req + 1] - s_c.before[req], k = unit - s_c.before[req], steps = s_c.steps[req];
-        whole = n == 1;
-        t0 = static_cast<int>(static_cast<int64_t>(steps) * k / n) * NW;
-        t_end = min((wh.len + KT - 1) / KT, static_cast<int>(static_cast<int64_t>(steps) * (k + 1) / n) * NW);
+        s.req = lo;
+        s.at = c.at[lo];
+        const int n = c.before[lo + 1] - c.before[lo], k = s.unit - c.before[lo], steps = c.steps[lo];
+        s.whole = n == 1;
+        s.t0 = static_cast<int>(static_cast<int64_t>(steps) * k / n) * a.step;
+        s.t_end = min((s.at.len + KT - 1) / KT, static_cast<int>(static_cast<int64_t>(steps) * (k + 1) / n) * a.step);
     } else {
-        wh = where_is(a, req);
-        if (qrow0 >= wh.rows * a.g) return;                       // uniform: this request has fewer rows
-        t_end = (wh.len + KT - 1) / KT;
+        s.at = where_is(a, s.req);
+        s.none = s.group * group_rows >= s.at.rows * a.g;         // this request has fewer rows
+        s.t_end = (s.at.len + KT - 1) / KT;
     }
-    const int c0 = wh.c0, rows = wh.rows, past = wh.past, len = wh.len;
+    return s;
+}
 
-    // this lane's query rows (one a tile): masks and factor of the scores; the operands into LDS
+// The pages of a request: page_of a position and, from its page, the row of the pool (slot_of): -1 where there is none.
+struct Pages {
+    const int32_t *table;
+    int limit;                         // positions from here on are not the block's
+    const Args &a;
+    __device__ __forceinline__ int page_of(int key) const { return key < limit ? gld(table + div_by(a.page, key)) : -1; }
+    __device__ __forceinline__ int slot_of(int key, int page) const {
+        return static_cast<unsigned>(page) < static_cast<unsigned>(a.n_pages)
+                   ? page * static_cast<int>(a.page.d) + key - div_by(a.page, key) * static_cast<int>(a.page.d) : -1;
+    }
+};
+
+// V rows of a tile in LDS: 32-byte piece i of key r at piece i ^ (r & (D / 16 - 1)), so that the rows that a
+// transposing load touches spread over the banks. The address of 16-byte half `h` of piece i.
+template <int D>
+__device__ __forceinline__ unsigned char *v_at(unsigned char *buf, int r, int i, int h) {
+    return buf + r * (D * 2) + ((i ^ (r & (D / 16 - 1))) << 5) + (h << 4);
+}
+
+// A wave's query rows, 16 a tile; lane l has row l % 16 of each: mask, factor of the scores, and the running
+// reference (ref: + SLACK; sub: - LIFT), sum and O^T (columns 16 d + 4 (l / 16) ..).
+template <class E, bool PAIR, int D, int NT>
+struct Rows {
+    typedef typename Types<E>::v8 v8;
+    typedef typename Types<E>::v4 v4;
+    static constexpr int KS = D / 32, DT = D / 16, QP = PAIR ? 2 : 1;   // MFMA steps of a score, column tiles of O
+    f32x4_t acc[NT][DT];
+    float ref[NT], sub[NT], sum[NT], fac[NT];
     uint64_t seen[NT];
-    float fac[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int m = qrow0 + nt * 16 + lr, j = div_by(a.heads_per, m);
-        const bool on = j < rows;
-        seen[nt] = on ? gld(a.mask + c0 + j) : 0;
-        fac[nt] = a.scale;
-        const size_t at = static_cast<size_t>(c0 + (on ? j : 0)) * a.ldq + static_cast<size_t>(kvh * a.g + (on ? m - j * a.g : 0)) * D + 8 * lg;
+
+    // Query row m of the request's (m < 0: none): its operands, a pair's hi before its lo, and the factor of its scores.
+    static __device__ __forceinline__ float operands(const Args &a, const Share &s, int m, v8 (&q)[QP * KS]) {
+        const int lg = (threadIdx.x & 63) >> 4, j = div_by(a.heads_per, max(m, 0));
+        const bool on = m >= 0 && j < s.at.rows;
+        const size_t at = static_cast<size_t>(s.at.c0 + (on ? j : 0)) * a.ldq + static_cast<size_t>(s.kvh * a.g + (on ? m - j * a.g : 0)) * D + 8 * lg;
+        float f = a.scale;
         if constexpr (PAIR) {
             // q times a power of two that puts the row's largest value into [1, 2): pairs keep 22 bits of it
             // whatever its range; the scores get the inverse
-            const float *q = static_cast<const float *>(a.q) + at;
+            const float *p = static_cast<const float *>(a.q) + at;
             f32x4_t x[KS][2];
             float top = 0.f;
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
+            for (int k = 0; k < KS; ++k)
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    x[s][hf] = on ? ld4(q + 32 * s + 4 * hf) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+                for (int h = 0; h < 2; ++h) {
+                    x[k][h] = on ? ld4(p + 32 * k + 4 * h) : f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[s][hf][e]));
+                    for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[k][h][e]));
                 }
             top = row_max(top);
             const int ex = top > 0.f && top < INFINITY ? ilogbf(top) : 0;
-            fac[nt] = ldexpf(a.scale, ex);
-            if (wv == 0) {
+            f = ldexpf(a.scale, ex);
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    v8 qhi, qlo;
+            for (int k = 0; k < KS; ++k)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float y = ldexpf(a.flip ? -x[s][e >> 2][e & 3] : x[s][e >> 2][e & 3], -ex);
-                        qhi[e] = static_cast<E>(y);
-                        qlo[e] = static_cast<E>(y - static_cast<float>(qhi[e]));
-                    }
-                    s_q[(nt * KS + s) * WAVE + l] = bits<u32x4_t>(qhi);
-                    s_q[((NT + nt) * KS + s) * WAVE + l] = bits<u32x4_t>(qlo);
+                for (int e = 0; e < 8; ++e) {
+                    const float y = ldexpf(a.flip ? -x[k][e >> 2][e & 3] : x[k][e >> 2][e & 3], -ex);
+                    q[k][e] = static_cast<E>(y);
+                    q[KS + k][e] = static_cast<E>(y - static_cast<float>(q[k][e]));
                 }
-            }
         } else {
-            const E *q = static_cast<const E *>(a.q) + at;
-            if (wv == 0) {
-                const uint32_t sign = a.flip ? 0x80008000u : 0u;
+            const E *p = static_cast<const E *>(a.q) + at;
+            const uint32_t sign = a.flip ? 0x80008000u : 0u;
 #pragma unroll
-                for (int s = 0; s < KS; ++s)
-                    s_q[(nt * KS + s) * WAVE + l] = on ? *(const NAVI_GLOBAL u32x4_t *) (q + 32 * s) ^ sign : u32x4_t{0u, 0u, 0u, 0u};
-            }
+            for (int k = 0; k < KS; ++k) q[k] = bits<v8>(on ? *(const NAVI_GLOBAL u32x4_t *) (p + 32 * k) ^ sign : u32x4_t{0u, 0u, 0u, 0u});
         }
         // a factor of 0 (all scores alike) as the least normal number: -inf, a place not seen, must stay -inf
-        fac[nt] = fmaxf(fac[nt], 1.17549435e-38f);
+        return fmaxf(f, 1.17549435e-38f);
     }
 
-    f32x4_t acc[NT][DT];
-    float ref[NT], sub[NT], sum[NT];                          // ref: the reference + SLACK; sub: reference - LIFT
+    __device__ __forceinline__ void start(const Args &a, const Share &s, int qrow0) {
+        const int lr = threadIdx.x & 15;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        ref[nt] = NONE;
-        sub[nt] = sum[nt] = 0.f;
+        for (int nt = 0; nt < NT; ++nt) {
+            const int j = div_by(a.heads_per, qrow0 + nt * 16 + lr);
+            seen[nt] = j < s.at.rows ? gld(a.mask + s.at.c0 + j) : 0;
+            ref[nt] = NONE;
+            sub[nt] = sum[nt] = 0.f;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[nt][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            for (int d = 0; d < DT; ++d) acc[nt][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
     }
 
-    unsigned char *buf = sm + wv * VB;
-    const E *kb = static_cast<const E *>(a.k) + kvh * D + 8 * lg, *vb = static_cast<const E *>(a.v) + kvh * D + 8 * lg;
-    const int32_t *table = a.table + static_cast<size_t>(req) * a.blocks;
-    // page and place in it of key `key`; slot: its row, or -1 past the end and outside the pool
-    auto page_of = [&](int key) { return key < len ? gld(table + div_by(a.page, key)) : -1; };
-    auto slot_of = [&](int key, int p) {
-        return static_cast<unsigned>(p) < static_cast<unsigned>(a.n_pages)
-                   ? p * static_cast<int>(a.page.d) + key - div_by(a.page, key) * static_cast<int>(a.page.d) : -1;
-    };
-    u32x4_t kr[2][KS], vr[2][KS];
-    int slot[2], page[2];
-    auto load_kv = [&]() {
+    // -inf for the scores of keys that a row does not see. Bit k of `there`: key k of the tile exists; the tile begins
+    // `ahead` positions after the first drafted one.
+    __device__ __forceinline__ void hide(f32x4_t (&sc)[NT][2], uint32_t there, int ahead) {
+        const int lg = (threadIdx.x & 63) >> 4;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            const size_t at = static_cast<size_t>(max(slot[kt], 0)) * a.ldkv;
+        for (int nt = 0; nt < NT; ++nt) {
+            uint32_t vis = ahead >= 64 ? 0u : ahead >= 0 ? static_cast<uint32_t>(seen[nt] >> ahead)
+                         : ahead <= -KT ? ~0u : static_cast<uint32_t>(seen[nt] << -ahead) | ((1u << -ahead) - 1u);
+            vis = (vis & there) >> (4 * lg);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                kr[kt][s] = *(const NAVI_GLOBAL u32x4_t *) (kb + at + 32 * s);
-                vr[kt][s] = *(const NAVI_GLOBAL u32x4_t *) (vb + at + 32 * s);
-            }
+            for (int i = 0; i < 8; ++i) sc[nt][i >> 2][i & 3] = vis >> ((i >> 2) * 16 + (i & 3)) & 1u ? sc[nt][i >> 2][i & 3] : NONE;
         }
-    };
-    int t = t0 + wv;
-    if (t < t_end) {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) page[kt] = page_of(t * KT + kt * 16 + lr);
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) slot[kt] = slot_of(t * KT + kt * 16 + lr, page[kt]);
-        load_kv();
-        if (t + NW < t_end)                                   // pages are looked up two tiles ahead
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) page[kt] = page_of((t + NW) * KT + kt * 16 + lr);
     }
-    __syncthreads();                                              // the operands of q
-    for (; t < t_end; t += NW) {
-        // keys of this tile that exist (uniform), and whether any row may not see one
-        const uint32_t there =
-            static_cast<uint32_t>(__ballot(slot[0] >= 0) & 0xFFFFu) | static_cast<uint32_t>(__ballot(slot[1] >= 0) & 0xFFFFu) << 16;
-        const bool masked = (t + 1) * KT > past || there != 0xFFFFFFFFu;
-        // V rows into LDS: 32-byte chunk i of key r at chunk i ^ (r & 7)
-        uint32_t special = 0;                                 // drafted keys with an infinity or NaN in V
-        if (masked) {
-            bool sp[2] = {false, false};
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    if (slot[kt] < 0) vr[kt][s] = u32x4_t{0u, 0u, 0u, 0u};
-                    if (t * KT + kt * 16 + lr >= past) sp[kt] |= any_special<E>(vr[kt][s]);
-                }
-            uint64_t b0 = __ballot(sp[0]), b1 = __ballot(sp[1]);
-            if (b0 | b1) {
-                b0 |= b0 >> 32;
-                b1 |= b1 >> 32;
-                special = static_cast<uint32_t>((b0 | b0 >> 16) & 0xFFFFu) | static_cast<uint32_t>((b1 | b1 >> 16) & 0xFFFFu) << 16;
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-                    if (special >> (kt * 16 + lr) & 1)
-#pragma unroll
-                        for (int s = 0; s < KS; ++s) vr[kt][s] = u32x4_t{0u, 0u, 0u, 0u};
-            }
-        }
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const int r = kt * 16 + lr, ch = 2 * s + (lg >> 1);
-                *reinterpret_cast<u32x4_t *>(buf + r * (D * 2) + ((ch ^ (r & (DT - 1))) << 5) + ((lg & 1) << 4)) = vr[kt][s];
-            }
-        // scores
-        f32x4_t sc[NT][2];
-        asm volatile("" ::: "memory");                        // or the operands would be kept in registers after all
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        // the operands of a step are read while the step before is multiplied
-        v8 qb[2][QP * NT];
-        auto load_q = [&](int s) {
-#pragma unroll
-            for (int i = 0; i < QP * NT; ++i) qb[s & 1][i] = bits<v8>(s_q[(i * KS + s) * WAVE + l]);
-        };
-        load_q(0);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            if (s + 1 < KS) load_q(s + 1);
-#pragma unroll
-            for (int i = 0; i < QP * NT; ++i)
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt) sc[i % NT][kt] = Types<E>::mfma(bits<v8>(kr[kt][s]), qb[s & 1][i], sc[i % NT][kt]);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x100, QP * NT, 0);          // LDS reads
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            __builtin_amdgcn_sched_group_barrier(0x100, QP * NT, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 2 * QP * NT, 0);  // MFMAs
-        }
-        // the next tile's rows, in flight from here
-        const int was0 = slot[0], was1 = slot[1];
-        if (t + NW < t_end) {
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) slot[kt] = slot_of((t + NW) * KT + kt * 16 + lr, page[kt]);
-            load_kv();
-            if (t + 2 * NW < t_end)
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt) page[kt] = page_of((t + 2 * NW) * KT + kt * 16 + lr);
-        }
-        // p
-        if (masked) {
-            // bit k of `vis`: key k of the tile; the tile begins `ahead` positions after the first drafted one
-            const int ahead = t * KT - past;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                uint32_t vis = ahead >= 64 ? 0u : ahead >= 0 ? static_cast<uint32_t>(seen[nt] >> ahead)
-                             : ahead <= -KT ? ~0u : static_cast<uint32_t>(seen[nt] << -ahead) | ((1u << -ahead) - 1u);
-                vis = (vis & there) >> (4 * lg);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sc[nt][i >> 2][i & 3] = vis >> ((i >> 2) * 16 + (i & 3)) & 1u ? sc[nt][i >> 2][i & 3] : NONE;
-            }
-        }
-        // the reference follows where a score passes it by more than SLACK (one test for all query tiles, so
-        // that what follows is one straight run of instructions)
+
+    // Scores to p, in place, and O^T += V^T P^T. One test for all query tiles whether a score passes its reference
+    // by more than SLACK, so that the rest is one straight run of instructions.
+    __device__ __forceinline__ void add(f32x4_t (&sc)[NT][2], unsigned char *buf) {
+        const int l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
         float top[NT];
         bool passed = false;
 #pragma unroll
@@ -430,15 +362,13 @@ __global__ void __launch_bounds__(BT, NT == 1 ? 3 : NT == 2 ? 2 : 1) k_tree(Args
                 sub[nt] = up ? mx - LIFT : sub[nt];
             }
         }
-        // O^T += V^T P^T
         v8 va[DT];
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
-                const int r = kt * 16 + 4 * lg + (lr >> 2);
                 const v4 x = bits<v4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s16x4 *) (buf + r * (D * 2) + ((d ^ (r & (DT - 1))) << 5) + ((lr & 3) << 3))));
+                    (__attribute__((address_space(3))) s16x4 *) (v_at<D>(buf, kt * 16 + 4 * lg + (lr >> 2), d, 0) + ((lr & 3) << 3))));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) va[d][4 * kt + e] = x[e];
             }
@@ -470,115 +400,413 @@ __global__ void __launch_bounds__(BT, NT == 1 ? 3 : NT == 2 ? 2 : 1) k_tree(Args
                 if constexpr (PAIR) acc[nt][d] = Types<E>::mfma(va[d], pl, acc[nt][d]);
             }
         }
-        // Drafted keys with an infinity or NaN in V (rare): zeros in the products above, since 0 times
-        // one would reach the rows that do not see them; here only the rows that do see them add theirs.
-        if (special) {
-            float *ps = reinterpret_cast<float *>(buf);       // [query row][key]
+    }
+
+    // Drafted keys with an infinity or NaN in V (rare; bits `special` of the tile): zeros in the products of add, since 0
+    // times one would reach the rows that do not see them. Here the rows that do see them add theirs; sc: p.
+    __device__ __forceinline__ void add_special(const f32x4_t (&sc)[NT][2], uint32_t special, int tile, const Share &s, const Pages &pg) {
+        const int l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+        for (; special; special &= special - 1) {
+            const int kin = __builtin_ctz(special), key = tile * KT + kin, ahead = key - s.at.past;
+            const int slot = pg.slot_of(key, pg.page_of(key));
+            const E *vp = static_cast<const E *>(pg.a.v) + static_cast<size_t>(max(slot, 0)) * pg.a.ldkv + s.kvh * D + 4 * lg;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+                float p = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) ps[(nt * 16 + lr) * KT + (i >> 2) * 16 + 4 * lg + (i & 3)] = sc[nt][i >> 2][i & 3];
-            __builtin_amdgcn_wave_barrier();
-            for (uint32_t rest = special; rest; rest &= rest - 1) {
-                const int kin = __builtin_ctz(rest), ahead = t * KT + kin - past;
-                const int sl = __shfl(kin < 16 ? was0 : was1, kin & 15);
-                const E *vp = static_cast<const E *>(a.v) + static_cast<size_t>(max(sl, 0)) * a.ldkv + kvh * D + 4 * lg;
+                for (int i = 0; i < 8; ++i) p = (kin >> 4) * 4 + (kin & 3) == i ? sc[nt][i >> 2][i & 3] : p;
+                p = __shfl(p, lr + 16 * ((kin & 15) >> 2));
+                const bool vis = ahead >= 0 && ahead < 64 && (seen[nt] >> (ahead & 63) & 1);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    if (!(ahead < 64 && (seen[nt] >> (ahead & 63) & 1))) continue;
-                    const float p = ps[(nt * 16 + lr) * KT + kin];
+                for (int d = 0; d < DT; ++d) {
+                    const v4 x = bits<v4>(*(const NAVI_GLOBAL u32x2_t *) (vp + 16 * d));
 #pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        const v4 x = bits<v4>(*(const NAVI_GLOBAL u32x2_t *) (vp + 16 * d));
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[nt][d][e] = fmaf(p, static_cast<float>(x[e]), acc[nt][d][e]);
-                    }
+                    for (int e = 0; e < 4; ++e) acc[nt][d][e] = vis ? fmaf(p, static_cast<float>(x[e]), acc[nt][d][e]) : acc[nt][d][e];
                 }
             }
-            __builtin_amdgcn_wave_barrier();
         }
     }
 
-    // join the four waves: reference = the greatest, sums and rows scaled to it
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        sum[nt] = row_sum(sum[nt]);
-        if (lg == 0) {
-            s_ref[wv][nt * 16 + lr] = ref[nt];
-            s_sum[wv][nt * 16 + lr] = sum[nt];
+    // Row r of the group, columns col ..: stored, or kept as the chunk's part.
+    static __device__ __forceinline__ void finish(const Args &a, const Share &s, int group_rows, int r, int col, f32x4_t o, float m, float total) {
+        const int q = s.group * group_rows + r, j = div_by(a.heads_per, q);
+        if (j >= s.at.rows) return;
+        if (!s.whole) {
+            const size_t at = part_of(a, s.kvh, s.group, s.unit) * group_rows + r;
+            st4(a.po + at * D + col, o);
+            if (col == 0) {
+                gst(a.pm + 2 * at, m);
+                gst(a.pm + 2 * at + 1, total);
+            }
+        } else {
+            store_out<E, PAIR>(a, s.at.c0 + j, (s.kvh * a.g + q - j * a.g) * D + col, a.hkv * a.g * D, o * (m == NONE ? 0.f : 1.f / total));
         }
     }
-    __syncthreads();                                          // and every wave is done with its buffer
-    float own[NT];
+};
+
+// Up to 32 query rows: every wave has all of them and works alone on its own tiles, every W-th of the block's, with K from
+// memory in operand form and its own V buffer, no barrier until the end; then the W results are joined in LDS.
+// CUT: a block takes a chunk of a request's keys, else all of them.
+template <class E, bool PAIR, int D, int NT, bool CUT>
+__global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) k_tree(Args a) {
+    constexpr int W = alone_of(CUT);
+    typedef Rows<E, PAIR, D, NT> R;
+    typedef typename R::v8 v8;
+    constexpr int KS = R::KS, DT = R::DT, QP = R::QP, VB = KT * D * 2, DP = D + 4;
+    constexpr int JOIN = W * NT * 16 * DP * 4, QB = QP * NT * KS * WAVE * 16;
+    __shared__ __align__(16) unsigned char sm[W * VB + QB > JOIN ? W * VB + QB : JOIN];
+    __shared__ float s_fac[NT * 16], s_ref[W][NT * 16], s_sum[W][NT * 16];
+    const int wv = threadIdx.x >> 6, l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+    const Share s = share_of<CUT>(a, NT * 16);
+    if (s.none) return;
+    const int qrow0 = s.group * NT * 16;
+    const Pages pg{a.table + static_cast<size_t>(s.req) * a.blocks, s.at.len, a};
+
+    u32x4_t kr[2][KS], vr[2][KS];
+    int slot[2], page[2];
+    const E *kb = static_cast<const E *>(a.k) + s.kvh * D + 8 * lg, *vb = static_cast<const E *>(a.v) + s.kvh * D + 8 * lg;
+    auto look_up = [&](int t) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) page[kt] = pg.page_of(t * KT + kt * 16 + lr);
+    };
+    auto load = [&](int t) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            slot[kt] = pg.slot_of(t * KT + kt * 16 + lr, page[kt]);
+            const size_t at = static_cast<size_t>(max(slot[kt], 0)) * a.ldkv;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                kr[kt][k] = *(const NAVI_GLOBAL u32x4_t *) (kb + at + 32 * k);
+                vr[kt][k] = *(const NAVI_GLOBAL u32x4_t *) (vb + at + 32 * k);
+            }
+        }
+    };
+    int t = s.t0 + wv;
+    if (t < s.t_end) look_up(t);
+    R rows;
+    rows.start(a, s, qrow0);
+    if (t < s.t_end) {
+        load(t);
+        if (t + W < s.t_end) look_up(t + W);                    // pages are looked up two tiles ahead
+    }
+    // the operands of q into LDS, a wave a query tile
+    u32x4_t *s_q = reinterpret_cast<u32x4_t *>(sm + W * VB);
+    if (wv < NT) {
+        v8 q[QP * KS];
+        const float f = R::operands(a, s, qrow0 + wv * 16 + lr, q);
+#pragma unroll
+        for (int i = 0; i < QP * KS; ++i) s_q[((i / KS * NT + wv) * KS + i % KS) * WAVE + l] = bits<u32x4_t>(q[i]);
+        if (lg == 0) s_fac[wv * 16 + lr] = f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) rows.fac[nt] = s_fac[nt * 16 + lr];
+
+    unsigned char *buf = sm + wv * VB;
+    for (; t < s.t_end; t += W) {
+        // keys of this tile that exist (uniform), and whether any row may not see one
+        const uint32_t there =
+            static_cast<uint32_t>(__ballot(slot[0] >= 0) & 0xFFFFu) | static_cast<uint32_t>(__ballot(slot[1] >= 0) & 0xFFFFu) << 16;
+        const bool masked = (t + 1) * KT > s.at.past || there != 0xFFFFFFFFu;
+        uint32_t special = 0;                                     // drafted keys with an infinity or NaN in V
+        if (masked) {
+            bool sp[2] = {false, false};
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    if (slot[kt] < 0) vr[kt][k] = u32x4_t{0u, 0u, 0u, 0u};
+                    if (t * KT + kt * 16 + lr >= s.at.past) sp[kt] |= any_special<E>(vr[kt][k]);
+                }
+            uint64_t b0 = __ballot(sp[0]), b1 = __ballot(sp[1]);
+            if (b0 | b1) {
+                b0 |= b0 >> 32;
+                b1 |= b1 >> 32;
+                special = static_cast<uint32_t>((b0 | b0 >> 16) & 0xFFFFu) | static_cast<uint32_t>((b1 | b1 >> 16) & 0xFFFFu) << 16;
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) vr[kt][k] = special >> (kt * 16 + lr) & 1 ? u32x4_t{0u, 0u, 0u, 0u} : vr[kt][k];
+            }
+        }
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int k = 0; k < KS; ++k) *reinterpret_cast<u32x4_t *>(v_at<D>(buf, kt * 16 + lr, 2 * k + (lg >> 1), lg & 1)) = vr[kt][k];
+        // scores; the operands of a step are read while the step before is multiplied
+        f32x4_t sc[NT][2];
+        asm volatile("" ::: "memory");                            // or the operands would be kept in registers after all
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        v8 qb[2][QP * NT];
+        auto load_q = [&](int k) {
+#pragma unroll
+            for (int i = 0; i < QP * NT; ++i) qb[k & 1][i] = bits<v8>(s_q[(i * KS + k) * WAVE + l]);
+        };
+        load_q(0);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            if (k + 1 < KS) load_q(k + 1);
+#pragma unroll
+            for (int i = 0; i < QP * NT; ++i)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) sc[i % NT][kt] = Types<E>::mfma(bits<v8>(kr[kt][k]), qb[k & 1][i], sc[i % NT][kt]);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, QP * NT, 0);          // LDS reads
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x100, QP * NT, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 2 * QP * NT, 0);  // MFMAs
+        }
+        // the next tile's rows, in flight from here
+        if (t + W < s.t_end) {
+            load(t + W);
+            if (t + 2 * W < s.t_end) look_up(t + 2 * W);
+        }
+        if (masked) rows.hide(sc, there, t * KT - s.at.past);
+        rows.add(sc, buf);
+        if (special) rows.add_special(sc, special, t, s, pg);
+    }
+
+    // join the waves: reference = the greatest, sums and rows scaled to it
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        rows.sum[nt] = row_sum(rows.sum[nt]);
+        if (lg == 0) {
+            s_ref[wv][nt * 16 + lr] = rows.ref[nt];
+            s_sum[wv][nt * 16 + lr] = rows.sum[nt];
+        }
+    }
+    __syncthreads();                                              // and every wave is done with its buffer
+    float *js = reinterpret_cast<float *>(sm);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int r = nt * 16 + lr;
         float m = s_ref[0][r];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) m = fmaxf(m, s_ref[w][r]);
-        own[nt] = ref[nt] == NONE ? 0.f : __builtin_amdgcn_exp2f(ref[nt] - m);
+        for (int w = 1; w < W; ++w) m = fmaxf(m, s_ref[w][r]);
+        const float own = rows.ref[nt] == NONE ? 0.f : __builtin_amdgcn_exp2f(rows.ref[nt] - m);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_t *>(js + (wv * NT * 16 + r) * DP + d * 16 + 4 * lg) = rows.acc[nt][d] * own;
     }
-    float *js = reinterpret_cast<float *>(sm);
-    const size_t part = CUT ? part_of(a, kvh, group, unit) * (NT * 16) : 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < NT * 16 * (D / 4); i += W * WAVE) {
+        const int r = i / (D / 4), c = i % (D / 4) * 4;
+        f32x4_t o = *reinterpret_cast<f32x4_t *>(js + r * DP + c);
+        float m = s_ref[0][r], total = 0.f;
 #pragma unroll
-    for (int cols = 0; cols < NT; ++cols) {                   // CD columns at a time
-        if (cols) __syncthreads();
+        for (int w = 1; w < W; ++w) {
+            o += *reinterpret_cast<f32x4_t *>(js + (w * NT * 16 + r) * DP + c);
+            m = fmaxf(m, s_ref[w][r]);
+        }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int w = 0; w < W; ++w) total += s_ref[w][r] == NONE ? 0.f : s_sum[w][r] * __builtin_amdgcn_exp2f(s_ref[w][r] - m);
+        R::finish(a, s, NT * 16, r, c, o, m, total);
+    }
+}
+
+// More than 32 query rows: a wave has 32 of them (RW waves the block's 32 RW), and the RW waves share the K and V tiles, which
+// they bring into LDS together: the cache is read once for 64 or 128 rows. KW such teams take every KW-th tile. Two
+// buffers: a tile is written while the one before is multiplied and the one after is on its way from memory; one barrier a tile.
+template <class E, bool PAIR, int D, int RW, bool CUT>
+__global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args a) {
+    constexpr int NT = 2, RWV = waves_of(PAIR, RW), KW = RWV / RW;
+    typedef Rows<E, PAIR, D, NT> R;
+    typedef typename R::v8 v8;
+    constexpr int KS = R::KS, DT = R::DT, QP = R::QP, RB = D * 2, TB = KT * RB, DP = D + 4;
+    constexpr int LPR = RB / 16, RPI = WAVE / LPR, KPW = KT / RW, SI = KPW / RPI;   // lanes a row, rows a load, keys a wave, its loads
+    static_assert(KW * RW == RWV && SI * RPI * RW == KT, "");
+    constexpr int BUFS = 2 * KW * 2 * TB, JOIN = (KW - 1) * RW * 32 * DP * 4;
+    __shared__ __align__(16) unsigned char sm[BUFS > JOIN ? BUFS : JOIN];
+    // the operands of q stay in registers, but a pair's lo, which would not fit: in LDS, a copy for all teams
+    __shared__ u32x4_t s_lo[PAIR ? RW * NT * KS * WAVE : 1];
+    __shared__ uint32_t s_there[2][KW][RW], s_special[2][KW][RW];
+    __shared__ float s_ref[RWV][NT * 16], s_sum[RWV][NT * 16];
+    const int wv = threadIdx.x >> 6, l = threadIdx.x & 63, lr = l & 15, lg = l >> 4, rw = wv % RW, kw = wv / RW;
+    const Share s = share_of<CUT>(a, RW * 32);
+    if (s.none) return;
+    const int qrow0 = s.group * RW * 32 + rw * 32;
+    const Pages pg{a.table + static_cast<size_t>(s.req) * a.blocks, min(s.at.len, s.t_end * KT), a};
+
+    // staging: this lane's 16 bytes of rows rw KPW + i RPI + l / LPR of the tile
+    const int c = l % LPR, r0 = rw * KPW + l / LPR;
+    u32x4_t kr[SI], vr[SI];
+    int slot[SI], page[SI];
+    const E *kb = static_cast<const E *>(a.k) + s.kvh * D + 8 * c, *vb = static_cast<const E *>(a.v) + s.kvh * D + 8 * c;
+    auto look_up = [&](int t) {
 #pragma unroll
-            for (int d = 0; d < DT / NT; ++d)
-                *reinterpret_cast<f32x4_t *>(js + (wv * NT * 16 + nt * 16 + lr) * CDP + d * 16 + 4 * lg) = acc[nt][cols * (DT / NT) + d] * own[nt];
-        __syncthreads();
-        for (int i = threadIdx.x; i < NT * 16 * (CD / 4); i += BT) {
-            const int r = i / (CD / 4), c = i % (CD / 4) * 4, m = qrow0 + r, j = div_by(a.heads_per, m);
-            if (j >= rows) continue;
-            f32x4_t o = *reinterpret_cast<f32x4_t *>(js + r * CDP + c);
-            float mx = s_ref[0][r];
+        for (int i = 0; i < SI; ++i) page[i] = pg.page_of(t * KT + r0 + i * RPI);
+    };
+    auto load = [&](int t) {
 #pragma unroll
-            for (int w = 1; w < NW; ++w) {
-                o += *reinterpret_cast<f32x4_t *>(js + (w * NT * 16 + r) * CDP + c);
-                mx = fmaxf(mx, s_ref[w][r]);
-            }
-            float total = 0.f;
+        for (int i = 0; i < SI; ++i) {
+            slot[i] = pg.slot_of(t * KT + r0 + i * RPI, page[i]);
+            const size_t at = static_cast<size_t>(max(slot[i], 0)) * a.ldkv;
+            kr[i] = *(const NAVI_GLOBAL u32x4_t *) (kb + at);
+            vr[i] = *(const NAVI_GLOBAL u32x4_t *) (vb + at);
+        }
+    };
+    auto bits_of = [&](uint64_t b, int i) {                       // a ballot over load i's rows as bits of the tile's keys
+        uint32_t x = 0;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) total += s_ref[w][r] == NONE ? 0.f : s_sum[w][r] * __builtin_amdgcn_exp2f(s_ref[w][r] - mx);
-            const int head = kvh * a.g + m - j * a.g, col = cols * CD + c;
-            if (CUT && !whole) {
-                st4(a.po + (part + r) * D + col, o);
-                if (col == 0) {
-                    gst(a.pm + 2 * (part + r), mx);
-                    gst(a.pm + 2 * (part + r) + 1, total);
+        for (int r = 0; r < RPI; ++r) x |= static_cast<uint32_t>((b >> (r * LPR) & ((uint64_t(1) << LPR) - 1)) != 0) << r;
+        return x << (rw * KPW + i * RPI);
+    };
+    auto put = [&](int b, int t) {
+        unsigned char *kd = sm + (b * KW + kw) * 2 * TB, *vd = kd + TB;
+        uint32_t there = 0, special = 0;
+#pragma unroll
+        for (int i = 0; i < SI; ++i) {
+            const uint64_t ok = __ballot(slot[i] >= 0);
+            there |= bits_of(ok, i);
+            if (ok != ~uint64_t(0) || (t + 1) * KT > s.at.past) {
+                vr[i] = slot[i] < 0 ? u32x4_t{0u, 0u, 0u, 0u} : vr[i];
+                const uint64_t sp = __ballot(t * KT + r0 + i * RPI >= s.at.past && any_special<E>(vr[i]));
+                if (sp) {
+                    const uint32_t x = bits_of(sp, i);
+                    special |= x;
+                    vr[i] = x >> (r0 + i * RPI) & 1 ? u32x4_t{0u, 0u, 0u, 0u} : vr[i];
                 }
-            } else {
-                const float inv = mx == NONE ? 0.f : 1.f / total;
-                store_out<E, PAIR>(a, c0 + j, head * D + col, a.hkv * a.g * D, o * inv);
             }
+            const int r = r0 + i * RPI;
+            *reinterpret_cast<u32x4_t *>(kd + r * RB + ((c ^ (r & (LPR - 1))) << 4)) = kr[i];
+            *reinterpret_cast<u32x4_t *>(v_at<D>(vd, r, c >> 1, c & 1)) = vr[i];
+        }
+        if (l == 0) {
+            s_there[b][kw][rw] = there;
+            s_special[b][kw][rw] = special;
+        }
+    };
+
+    int t = s.t0 + kw;
+    const int turns = (s.t_end - s.t0 + KW - 1) / KW;             // the same for all waves: past its tiles a team has none there
+    look_up(t);
+    R rows;
+    rows.start(a, s, qrow0);
+    load(t);
+    look_up(t + KW);
+    v8 q[NT][KS];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        v8 x[QP * KS];
+        rows.fac[nt] = R::operands(a, s, qrow0 + nt * 16 + lr, x);
+#pragma unroll
+        for (int i = 0; i < QP * KS; ++i)
+            if (i < KS) q[nt][i] = x[i];
+            else if (kw == 0) s_lo[((rw * NT + nt) * KS + i - KS) * WAVE + l] = bits<u32x4_t>(x[i]);
+    }
+    put(0, t);
+    load(t + KW);
+    look_up(t + 2 * KW);
+    for (int turn = 0; turn < turns; ++turn, t += KW) {
+        const int b = turn & 1;
+        __syncthreads();                                          // tile t is in LDS, and tile t - KW has been used
+        if (turn + 1 < turns) {
+            put(b ^ 1, t + KW);
+            load(t + 2 * KW);
+            look_up(t + 3 * KW);
+        }
+        uint32_t there = 0, special = 0;
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            there |= s_there[b][kw][i];
+            special |= s_special[b][kw][i];
+        }
+        there = __builtin_amdgcn_readfirstlane(there);
+        special = __builtin_amdgcn_readfirstlane(special);
+        unsigned char *kd = sm + (b * KW + kw) * 2 * TB;
+        f32x4_t sc[NT][2];
+        if constexpr (PAIR) asm volatile("" ::: "memory");          // or lo would be kept in registers after all
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            v8 kf[2];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                const int r = kt * 16 + lr;
+                kf[kt] = bits<v8>(*reinterpret_cast<u32x4_t *>(kd + r * RB + (((4 * k + lg) ^ (r & (LPR - 1))) << 4)));
+            }
+#pragma unroll
+            for (int p = 0; p < QP; ++p)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const v8 x = p == 0 ? q[nt][k] : bits<v8>(s_lo[((rw * NT + nt) * KS + k) * WAVE + l]);
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt) sc[nt][kt] = Types<E>::mfma(kf[kt], x, sc[nt][kt]);
+                }
+        }
+        if ((t + 1) * KT > s.at.past || there != 0xFFFFFFFFu) rows.hide(sc, there, t * KT - s.at.past);
+        rows.add(sc, kd + TB);
+        if (special) rows.add_special(sc, special, t, s, pg);
+    }
+
+    // join the teams' results through LDS: reference = the greatest, sums and rows scaled to it; the first team adds and stores
+    float *js = reinterpret_cast<float *>(sm);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        rows.sum[nt] = row_sum(rows.sum[nt]);
+        if (lg == 0) {
+            s_ref[wv][nt * 16 + lr] = rows.ref[nt];
+            s_sum[wv][nt * 16 + lr] = rows.sum[nt];
         }
     }
+    __syncthreads();                                              // and every wave is done with the buffers
+    float m[NT], total[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = nt * 16 + lr;
+        m[nt] = s_ref[rw][r];
+#pragma unroll
+        for (int w = 1; w < KW; ++w) m[nt] = fmaxf(m[nt], s_ref[w * RW + rw][r]);
+        total[nt] = 0.f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+            const float x = s_ref[w * RW + rw][r];
+            total[nt] += x == NONE ? 0.f : s_sum[w * RW + rw][r] * __builtin_amdgcn_exp2f(x - m[nt]);
+        }
+        const float own = rows.ref[nt] == NONE ? 0.f : __builtin_amdgcn_exp2f(rows.ref[nt] - m[nt]);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            rows.acc[nt][d] *= own;
+            if (kw > 0) *reinterpret_cast<f32x4_t *>(js + (((kw - 1) * RW + rw) * 32 + r) * DP + d * 16 + 4 * lg) = rows.acc[nt][d];
+        }
+    }
+    __syncthreads();
+    if (kw > 0) return;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            f32x4_t o = rows.acc[nt][d];
+#pragma unroll
+            for (int w = 1; w < KW; ++w) o += *reinterpret_cast<f32x4_t *>(js + (((w - 1) * RW + rw) * 32 + nt * 16 + lr) * DP + d * 16 + 4 * lg);
+            R::finish(a, s, RW * 32, rw * 32 + nt * 16 + lr, d * 16 + 4 * lg, o, m[nt], total[nt]);
+        }
 }
 
 // Joins the parts of the requests that were cut, in their order: a wave takes a query row, D / 8 lanes its
 // columns and the others further parts. Block (request x kv head x group, rows).
 template <class E, bool PAIR, int D>
-__global__ void __launch_bounds__(BT) k_tree_join(Args a, int nt16) {
+__global__ void __launch_bounds__(BT) k_tree_join(Args a, int group_rows) {
     constexpr int CL = D / 8, PL = WAVE / CL;
     __shared__ Chunks seq;
     const int l = threadIdx.x & 63, c = l % CL, pl = l / CL;
     int id = blockIdx.x;
     const int kvh = id % a.hkv;
     id /= a.hkv;
-    const int group = id % a.groups, req = id / a.groups, qrow0 = group * nt16;
+    const int group = id % a.groups, req = id / a.groups, qrow0 = group * group_rows;
     lay_out(a, qrow0, seq);
     const int k0 = seq.before[req], k1 = seq.before[req + 1];
     if (k1 - k0 < 2) return;                                      // a block had all of it and has stored it
     const Where wh = seq.at[req];
-    const int left = min(nt16, wh.rows * a.g - qrow0);
+    const int left = min(group_rows, wh.rows * a.g - qrow0);
     for (int r = blockIdx.y * NW + (threadIdx.x >> 6); r < left; r += gridDim.y * NW) {
         float m = NONE, sum = 0.f;
         f32x4_t o[2] = {f32x4_t{0.f, 0.f, 0.f, 0.f}, f32x4_t{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll 4
         for (int k = k0 + pl; k < k1; k += PL) {
-            const size_t at = part_of(a, kvh, group, k) * nt16 + r;
+            const size_t at = part_of(a, kvh, group, k) * group_rows + r;
             const float ref = gld(a.pm + 2 * at), z = gld(a.pm + 2 * at + 1);
             const f32x4_t x0 = ld4(a.po + at * D + 8 * c), x1 = ld4(a.po + at * D + 8 * c + 4);
             const float top = fmaxf(m, ref);
@@ -610,64 +838,75 @@ __global__ void __launch_bounds__(BT) k_tree_join(Args a, int nt16) {
     }
 }
 
-// How a call is cut: query tiles of a block, groups of them, and blocks wanted for a kv head and group (0: one a request).
+// How a call is cut: query tiles and, above 32 query rows, waves that share them (waves 1: none share), rows of a group and
+// groups, and blocks wanted for a kv head and group (0: one a request).
 struct Cut {
-    int nt, groups, workers;
+    int tiles, waves, rows, groups, workers, step;
 };
-Cut cut_of(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys) {
+Cut cut_of(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys, bool pair) {
     const int m = std::min(p.max_new, 64) * (h.n_head / h.n_kv_head);
     Cut c;
-    c.nt = m <= 16 ? 1 : m <= 32 ? 2 : 4;
-    c.groups = (m + 16 * c.nt - 1) / (16 * c.nt);
+    c.tiles = m <= 16 ? 1 : 2;
+    c.waves = m <= 32 ? 1 : m <= 64 ? 2 : 4;
+    c.rows = 16 * c.tiles * c.waves;
+    c.groups = (m + c.rows - 1) / c.rows;
     const int64_t heads = static_cast<int64_t>(h.n_kv_head) * c.groups;
-    const int steps = (max_keys + KT * NW - 1) / (KT * NW);
-    // A block a request where no request can be long and there are blocks for all CUs (32 requests of 1024 keys: 30.0 us,
-    // cut 33.2: the chunks and the join), or more requests than a block lays out. Else two blocks a CU, or the one that
-    // fits with four query tiles.
-    if (p.n_requests > MAXB || steps == 1 || (steps <= 16 && p.n_requests * heads >= 256)) {
+    const int waves = c.waves == 1 ? alone_of(true) : waves_of(pair, c.waves);
+    c.step = waves / c.waves;                           // tiles of a block's turn
+    const int steps = (max_keys + KT * c.step - 1) / (KT * c.step);
+    // A block a request where no request can be long and there are blocks for all CUs (32 requests of 1024 keys: 27.3 us,
+    // cut 33.3: the chunks and the join), or more requests than a block lays out. Else enough blocks for all waves of the CUs.
+    if (p.n_requests > MAXB || steps == 1 || (max_keys <= 2048 && p.n_requests * heads >= 256)) {
         c.workers = 0;
         return c;
     }
-    const int64_t blocks = c.nt == 4 ? 256 : 512;
+    const int64_t blocks = 2048 / waves;                           // two waves a SIMD
     c.workers = static_cast<int>(std::max<int64_t>(1, std::min((blocks + heads - 1) / heads, static_cast<int64_t>(steps) * p.n_requests)));
     return c;
 }
 
-size_t workspace(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys) {
-    const Cut c = cut_of(p, h, max_keys);
-    if (c.workers == 0) return 0;
-    return static_cast<size_t>(h.n_kv_head) * c.groups * (c.workers + p.n_requests) * (c.nt * 16) * (h.head_dim + 2) * sizeof(float);
+// Floats of the parts' rows (then two for each row).
+size_t part_rows(const navi_kv_pages &p, const navi_kv_heads &h, const Cut &c) {
+    return c.workers == 0 ? 0 : static_cast<size_t>(h.n_kv_head) * c.groups * (c.workers + p.n_requests) * c.rows;
 }
 
-template <class E, bool PAIR, int D, int NT>
-void launch_nt(const Args &a, const Cut &c, hipStream_t s) {
-    if (c.workers == 0) {
-        hipLaunchKernelGGL((k_tree<E, PAIR, D, NT, false>), dim3(static_cast<unsigned>(a.n) * a.groups * a.hkv), dim3(BT), 0, s, a);
-        return;
-    }
-    hipLaunchKernelGGL((k_tree<E, PAIR, D, NT, true>), dim3(static_cast<unsigned>(c.workers + a.n) * a.groups * a.hkv), dim3(BT), 0, s, a);
-    const unsigned units = static_cast<unsigned>(a.n) * a.groups * a.hkv;
-    hipLaunchKernelGGL((k_tree_join<E, PAIR, D>), dim3(units, std::max(1u, std::min(NT * 16u / NW, 1024u / units))), dim3(BT), 0, s, a, NT * 16);
+size_t workspace(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys) {
+    // q's type is not known here: enough for either
+    return std::max(part_rows(p, h, cut_of(p, h, max_keys, false)), part_rows(p, h, cut_of(p, h, max_keys, true))) * (h.head_dim + 2) * sizeof(float);
+}
+
+template <class E, bool PAIR, int D, bool CUT>
+void launch_cut(const Args &a, const Cut &c, hipStream_t s) {
+    const dim3 rbt(static_cast<unsigned>(waves_of(PAIR, c.waves) * WAVE));
+    const dim3 grid(static_cast<unsigned>(CUT ? c.workers + a.n : a.n) * a.groups * a.hkv);
+    const dim3 abt(alone_of(CUT) * WAVE);
+    if (c.tiles == 1) hipLaunchKernelGGL((k_tree<E, PAIR, D, 1, CUT>), grid, abt, 0, s, a);
+    else if (c.waves == 1) hipLaunchKernelGGL((k_tree<E, PAIR, D, 2, CUT>), grid, abt, 0, s, a);
+    else if (c.waves == 2) hipLaunchKernelGGL((k_tree_rows<E, PAIR, D, 2, CUT>), grid, rbt, 0, s, a);
+    else hipLaunchKernelGGL((k_tree_rows<E, PAIR, D, 4, CUT>), grid, rbt, 0, s, a);
 }
 
 template <class E, bool PAIR, int D>
 void launch_as(const Args &a, const Cut &c, hipStream_t s) {
-    if (c.nt == 1) launch_nt<E, PAIR, D, 1>(a, c, s);
-    else if (c.nt == 2) launch_nt<E, PAIR, D, 2>(a, c, s);
-    else launch_nt<E, PAIR, D, 4>(a, c, s);
+    if (c.workers == 0) return launch_cut<E, PAIR, D, false>(a, c, s);
+    launch_cut<E, PAIR, D, true>(a, c, s);
+    const unsigned units = static_cast<unsigned>(a.n) * a.groups * a.hkv;
+    hipLaunchKernelGGL((k_tree_join<E, PAIR, D>), dim3(units, std::max(1u, std::min(static_cast<unsigned>(c.rows / NW), 1024u / units))), dim3(BT), 0, s,
+                       a, c.rows);
 }
 
 void launch(const Call &x, hipStream_t s) {
     const navi_kv_pages &p = *x.pages;
     const navi_kv_heads &h = *x.heads;
-    const Cut c = cut_of(p, h, x.max_keys);
+    const bool pair = x.q_dtype == NAVI_DT_F32, bf = h.kv_dtype == NAVI_DT_BF16;
+    const Cut c = cut_of(p, h, x.max_keys, pair);
     Args a{};
     a.q = x.q;
     a.k = x.k;
     a.v = x.v;
     a.out = x.out;
     a.po = static_cast<float *>(x.ws);
-    a.pm = a.po ? a.po + static_cast<size_t>(h.n_kv_head) * c.groups * (c.workers + p.n_requests) * (c.nt * 16) * h.head_dim : nullptr;
+    a.pm = a.po ? a.po + part_rows(p, h, c) * h.head_dim : nullptr;
     a.table = p.block_table;
     a.n_past = p.n_past;
     a.cu = p.cu_rows;
@@ -683,13 +922,13 @@ void launch(const Call &x, hipStream_t s) {
     a.ldkv = x.ldkv;
     a.ldo = x.ldo;
     a.workers = c.workers;
+    a.step = c.step;
     a.groups = c.groups;
     a.tiled = x.tiled;
     a.page = kv::make_div(static_cast<uint32_t>(p.page_size));
     a.heads_per = kv::make_div(static_cast<uint32_t>(a.g));
     a.flip = x.scale < 0.f;
     a.scale = std::fabs(x.scale) * 1.44269504088896340736f;
-    const bool pair = x.q_dtype == NAVI_DT_F32, bf = h.kv_dtype == NAVI_DT_BF16;
     if (h.head_dim == 128) {
         if (pair) launch_as<_Float16, true, 128>(a, c, s);
         else if (bf) launch_as<__bf16, false, 128>(a, c, s);
