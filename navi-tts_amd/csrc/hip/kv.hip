@@ -58,26 +58,36 @@ constexpr int REC_ENDED = 1, REC_REFUSED = 2, REC_BAD = 4;
 
 constexpr int PT = 1024, PW = PT / WAVE;   // the planning block: 16 waves
 
-// Exclusive prefix sum over the block's threads; *total the whole sum. red: PW values of LDS.
-__device__ __forceinline__ int64_t block_before(int64_t v, int64_t *red, int64_t &total) {
+// Exclusive prefix sums of x and y over the block's threads, and their totals. red: PW pairs of LDS.
+struct Two {
+    int64_t x, y;
+};
+__device__ __forceinline__ Two block_before(Two v, Two *red, Two &total) {
     const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-    int64_t x = v;
+    Two s = v;
 #pragma unroll
     for (int o = 1; o < WAVE; o <<= 1) {
-        const int64_t y = __shfl_up(static_cast<long long>(x), o);
-        if (l >= o) x += y;
+        const int64_t x = __shfl_up(static_cast<long long>(s.x), o), y = __shfl_up(static_cast<long long>(s.y), o);
+        if (l >= o) {
+            s.x += x;
+            s.y += y;
+        }
     }
     __syncthreads();                                  // red's readers of the call before are done
-    if (l == 63) red[w] = x;
+    if (l == 63) red[w] = s;
     __syncthreads();
-    int64_t before = 0;
-    total = 0;
+    Two before{0, 0};
+    total = Two{0, 0};
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
-        if (i < w) before += red[i];
-        total += red[i];
+        if (i < w) {
+            before.x += red[i].x;
+            before.y += red[i].y;
+        }
+        total.x += red[i].x;
+        total.y += red[i].y;
     }
-    return before + x - v;
+    return Two{before.x + s.x - v.x, before.y + s.y - v.y};
 }
 
 // The page of block b of a request: kept from its table, or taken from the stack (whose top part was
@@ -144,107 +154,131 @@ __device__ __forceinline__ void fill_request(const PlanArgs &a, int i, int part,
 }
 
 // One block plans all requests: row offsets, the checks, the stack; FILL: the tables and rows too, a
-// wave a request at a time. Thread t takes requests t, t + PT, ...: a request's values meet their
-// neighbours' in the prefix sums only, so they are read again in each pass rather than held.
+// wave a request at a time. Thread t has requests t R .. t R + R - 1 (R = 1 up to PT requests, whose
+// lengths then stay in registers); it is bound by the latencies of its rounds of loads, barriers and sums, so
+// these are few: 256 requests with trees 13 us with the fill, 21 when every check read its request's record from memory.
 template <bool FILL>
 __global__ void __launch_bounds__(PT) k_plan(PlanArgs a) {
-    __shared__ int64_t red[PW];
-    __shared__ int s_top;
+    __shared__ Two red[PW];
+    __shared__ int s_top, s_list;
+    __shared__ int4 list[PT];                         // of a round: row offset, rows, parents checked?; then the pages that go back
+    __shared__ bool s_bad[PT];
     const int tid = threadIdx.x, wv = tid >> 6, l = tid & 63;
+    const int R = (a.n + PT - 1) / PT, i0 = tid * R;
     const int64_t room = min(static_cast<int64_t>(a.blocks) * a.page.d, static_cast<int64_t>(INT32_MAX));
+    const int free_in = gld(a.free_in);
+    struct Lengths {
+        int past, add, held;
+    };
+    auto lengths = [&](int i) {
+        return i < a.n ? Lengths{gld(a.n_past + i), gld(a.n_new + i), gld(a.held_in + i)} : Lengths{0, 0, 0};
+    };
+    const Lengths first = lengths(i0);
+    auto own = [&](int k) { return k == 0 ? first : lengths(i0 + k); };
     // rows: offsets, and which lengths are in range
-    int64_t rows = 0, total;
-    for (int i0 = 0; i0 < a.n; i0 += PT) {
-        const int i = i0 + tid;
-        int past = 0, add = 0, held = 0;
+    Two total, v{0, 0};
+    for (int k = 0; k < R; ++k) v.x += max(own(k).add, 0);
+    int64_t at = block_before(v, red, total).x;
+    if (tid == 0) {
+        gst(a.cu + a.n, static_cast<int>(min(total.x, static_cast<int64_t>(a.n_rows))));
+        s_top = s_list = 0;
+    }
+    int flags0 = 0;                                   // of this thread's first request; the others' are in their records
+    for (int k = 0; k < R; ++k) {
+        const int i = i0 + k;
+        const Lengths x = own(k);
+        const int count = max(x.add, 0);
+        const bool bad = x.past < 0 || x.held < 0 || x.held > a.blocks || x.add > a.max_new || at + count > a.n_rows ||
+                         (x.add >= 0 && static_cast<int64_t>(x.past) + count > room);
+        const int flags = (x.add < 0 ? REC_ENDED : 0) | (bad ? REC_BAD : 0);
+        const int c0 = static_cast<int>(min(at, static_cast<int64_t>(a.n_rows)));
         if (i < a.n) {
-            past = gld(a.n_past + i);
-            add = gld(a.n_new + i);
-            held = gld(a.held_in + i);
-        }
-        const int count = max(add, 0);
-        const int64_t at = rows + block_before(count, red, total);
-        rows += total;
-        if (i < a.n) {
-            const bool bad = past < 0 || held < 0 || held > a.blocks || add > a.max_new || at + count > a.n_rows ||
-                             (add >= 0 && static_cast<int64_t>(past) + count > room);
-            gst(a.cu + i, static_cast<int>(min(at, static_cast<int64_t>(a.n_rows))));
+            gst(a.cu + i, c0);
             gst(a.status + i, bad ? 2 : 0);
-            a.rec[i] = int4{held, 0, 0, (add < 0 ? REC_ENDED : 0) | (bad ? REC_BAD : 0)};
+            if (k > 0) a.rec[i] = int4{x.held, 0, 0, flags};
         }
-    }
-    if (tid == 0) gst(a.cu + a.n, static_cast<int>(min(rows, static_cast<int64_t>(a.n_rows))));
-    __threadfence_block();
-    __syncthreads();
-    // parents come before their rows: a wave a request, a lane a row
-    if (a.parent) {
-        for (int i = wv; i < a.n; i += PW) {
-            if (a.rec[i].w & (REC_BAD | REC_ENDED)) continue;
-            const int c0 = gld(a.cu + i), count = gld(a.cu + i + 1) - c0;
-            const int p = l < count ? gld(a.parent + c0 + l) : -1;
-            if (__ballot(p < -1 || p >= l) != 0 && l == 0) {
-                gst(a.status + i, 3);
-                a.rec[i].w |= REC_BAD;
-            }
-        }
-        __threadfence_block();
-        __syncthreads();
-    }
-    // the ended requests' pages go onto the stack, a wave a request
-    int top = min(max(gld(a.free_in), 0), a.n_pages);
-    for (int i0 = 0; i0 < a.n; i0 += PT) {
-        const int i = i0 + tid;
-        int back = 0;
-        if (i < a.n) {
-            const int4 r = a.rec[i];
-            if ((r.w & (REC_ENDED | REC_BAD)) == REC_ENDED) back = r.x;
-        }
-        const int64_t before = block_before(back, red, total);
-        if (i < a.n && back > 0) a.rec[i].z = static_cast<int>(min(top + before, static_cast<int64_t>(a.n_pages)));
-        if (total > 0) {
-            __threadfence_block();
+        if (k == 0) flags0 = flags;
+        at += count;
+        // parents come before their rows: a wave eight requests at a time, a lane a row
+        if (a.parent) {
+            list[tid] = int4{c0, i < a.n && flags == 0 ? count : 0, 0, 0};
+            s_bad[tid] = false;
             __syncthreads();
-            for (int k = i0 + wv; k < min(a.n, i0 + PT); k += PW) {
-                const int4 r = a.rec[k];
-                if ((r.w & (REC_ENDED | REC_BAD)) != REC_ENDED) continue;
-                for (int b = l; b < r.x && r.z + b < a.n_pages; b += WAVE)
-                    gst(a.free_pages + r.z + b, gld(a.table_in + static_cast<size_t>(k) * a.blocks + b));
+            const int used = min(PT, (a.n - k + R - 1) / R);      // threads with a request in this round
+            for (int t0 = wv * 8; t0 < used; t0 += PW * 8) {
+                int p[8], n[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int4 q = t0 + u < used ? list[t0 + u] : int4{0, 0, 0, 0};
+                    n[u] = q.y;
+                    p[u] = l < q.y ? gld(a.parent + q.x + l) : -1;
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (__ballot(p[u] < -1 || p[u] >= l) != 0 && n[u] > 0 && l == 0) s_bad[t0 + u] = true;
+            }
+            __syncthreads();
+            if (i < a.n && s_bad[tid]) {
+                gst(a.status + i, 3);
+                if (k == 0) flags0 |= REC_BAD;
+                else a.rec[i].w |= REC_BAD;
             }
         }
-        top = static_cast<int>(min(top + total, static_cast<int64_t>(a.n_pages)));
     }
-    // pages taken, in order, as long as they last
-    int64_t asked = 0;
-    int taken_all = 0;
-    if (tid == 0) s_top = 0;
-    for (int i0 = 0; i0 < a.n; i0 += PT) {
-        const int i = i0 + tid;
-        int4 r{0, 0, 0, REC_BAD};
-        int64_t want = 0;
-        if (i < a.n) {
-            r = a.rec[i];
-            if (!(r.w & (REC_BAD | REC_ENDED))) {
-                const int len = gld(a.n_past + i) + max(gld(a.n_new + i), 0);       // <= room
-                want = max((len > 0 ? div_by(a.page, len - 1) + 1 : 0) - r.x, 0);
-            }
+    // pages that ended requests give back, and pages that the others need
+    auto flags_of = [&](int k) { return k == 0 ? flags0 : a.rec[i0 + k].w; };
+    auto back_and_want = [&](int k) {
+        Two r{0, 0};
+        if (i0 + k >= a.n) return r;
+        const Lengths x = own(k);
+        const int f = flags_of(k);
+        if ((f & (REC_ENDED | REC_BAD)) == REC_ENDED) r.x = x.held;
+        else if (!(f & (REC_ENDED | REC_BAD))) {
+            const int len = x.past + max(x.add, 0);               // <= room
+            r.y = max((len > 0 ? div_by(a.page, len - 1) + 1 : 0) - x.held, 0);
         }
-        const int64_t off = asked + block_before(want, red, total);
-        asked += total;
-        const bool refused = want > 0 && off + want > top;
+        return r;
+    };
+    v = Two{0, 0};
+    for (int k = 0; k < R; ++k) {
+        const Two r = back_and_want(k);
+        v.x += r.x;
+        v.y += r.y;
+    }
+    Two off = block_before(v, red, total);
+    const int below = min(max(free_in, 0), a.n_pages);            // the stack's top before, and with the pages given back
+    const int top = static_cast<int>(min(below + total.x, static_cast<int64_t>(a.n_pages)));
+    for (int k = 0; k < R; ++k) {
+        const int i = i0 + k;
+        const Two r = back_and_want(k);
         if (i < a.n) {
-            const int taken = refused ? 0 : static_cast<int>(want);
+            const int held = own(k).held, f = flags_of(k);
+            const bool refused = r.y > 0 && off.y + r.y > top;
+            const int taken = refused ? 0 : static_cast<int>(r.y);
             if (refused) gst(a.status + i, 1);
-            if (!(r.w & (REC_BAD | REC_ENDED)))
-                a.rec[i] = int4{r.x, taken, static_cast<int>(max<int64_t>(top - 1 - off, 0)), r.w | (refused ? REC_REFUSED : 0)};
-            gst(a.held + i, (r.w & (REC_ENDED | REC_BAD)) == REC_ENDED ? 0 : r.x + taken);
+            a.rec[i] = int4{held, taken, static_cast<int>(max<int64_t>(top - 1 - off.y, 0)), f | (refused ? REC_REFUSED : 0)};
+            gst(a.held + i, (f & (REC_ENDED | REC_BAD)) == REC_ENDED ? 0 : held + taken);
             // the granted requests' pages lie without gaps below the top
-            if (taken > 0) atomicMax(&s_top, static_cast<int>(off) + taken);
+            if (taken > 0) atomicMax(&s_top, static_cast<int>(off.y) + taken);
+            if (r.x > 0) list[atomicAdd(&s_list, 1)] = int4{i, static_cast<int>(min(below + off.x, static_cast<int64_t>(a.n_pages))), held, 0};
+        }
+        off.x += r.x;
+        off.y += r.y;
+        if (total.x > 0) {                                        // onto the stack, a wave a request (in places that do not
+            __syncthreads();                                      // depend on the list's order)
+            for (int e = wv; e < s_list; e += PW) {
+                const int4 q = list[e];
+                for (int b = l; b < q.z && q.y + b < a.n_pages; b += WAVE)
+                    gst(a.free_pages + q.y + b, gld(a.table_in + static_cast<size_t>(q.x) * a.blocks + b));
+            }
+            __syncthreads();
+            if (tid == 0) s_list = 0;
+            __syncthreads();
         }
     }
     __threadfence_block();
     __syncthreads();
-    taken_all = s_top;
-    if (tid == 0) gst(a.n_free, top - taken_all);
+    if (tid == 0) gst(a.n_free, top - s_top);
     if constexpr (FILL)
         for (int i = wv; i < a.n; i += PW) fill_request(a, i, 0, 1, l, WAVE);
 }
