@@ -51,6 +51,7 @@ struct Args {
     const void *q, *k, *v;
     void *out;
     float *po, *pm;                    // the parts of requests that are cut (part_of)
+    int32_t *first;                    // and each group's chunks before every request [groups][n + 1]
     const int32_t *table, *n_past, *cu;
     const uint64_t *mask;
     int n, hkv, g, blocks, n_pages, n_rows, max_new, ldq, ldkv, ldo, workers, groups, step;
@@ -216,6 +217,8 @@ __device__ __forceinline__ Share share_of(const Args &a, int group_rows) {
     if constexpr (CUT) {
         __shared__ Chunks c;
         lay_out(a, s.group * group_rows, c);
+        if (s.unit == 0 && s.kvh == 0)                            // for the join
+            for (int i = threadIdx.x; i <= a.n; i += blockDim.x) gst(a.first + s.group * (a.n + 1) + i, c.before[i]);
         s.none = s.unit >= c.before[a.n];
         if (s.none) return s;
         int lo = 0, hi = a.n;                                     // before[lo] <= unit < before[hi]
@@ -654,20 +657,24 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
     };
     auto put = [&](int b, int t) {
         unsigned char *kd = sm + (b * KW + kw) * 2 * TB, *vd = kd + TB;
-        uint32_t there = 0, special = 0;
+        // all of them there and cached: seen by all rows
+        bool plain = (t + 1) * KT <= s.at.past;
+#pragma unroll
+        for (int i = 0; i < SI; ++i) plain = plain && slot[i] >= 0;
+        uint32_t there = ((KPW < 32 ? 1u << (KPW & 31) : 0u) - 1u) << (rw * KPW), special = 0;
+        if (__ballot(!plain)) {
+            there = 0;
+#pragma unroll
+            for (int i = 0; i < SI; ++i) {
+                there |= bits_of(__ballot(slot[i] >= 0), i);
+                vr[i] = slot[i] < 0 ? u32x4_t{0u, 0u, 0u, 0u} : vr[i];
+                const uint32_t x = bits_of(__ballot(t * KT + r0 + i * RPI >= s.at.past && any_special<E>(vr[i])), i);
+                special |= x;
+                vr[i] = x >> (r0 + i * RPI) & 1 ? u32x4_t{0u, 0u, 0u, 0u} : vr[i];
+            }
+        }
 #pragma unroll
         for (int i = 0; i < SI; ++i) {
-            const uint64_t ok = __ballot(slot[i] >= 0);
-            there |= bits_of(ok, i);
-            if (ok != ~uint64_t(0) || (t + 1) * KT > s.at.past) {
-                vr[i] = slot[i] < 0 ? u32x4_t{0u, 0u, 0u, 0u} : vr[i];
-                const uint64_t sp = __ballot(t * KT + r0 + i * RPI >= s.at.past && any_special<E>(vr[i]));
-                if (sp) {
-                    const uint32_t x = bits_of(sp, i);
-                    special |= x;
-                    vr[i] = x >> (r0 + i * RPI) & 1 ? u32x4_t{0u, 0u, 0u, 0u} : vr[i];
-                }
-            }
             const int r = r0 + i * RPI;
             *reinterpret_cast<u32x4_t *>(kd + r * RB + ((c ^ (r & (LPR - 1))) << 4)) = kr[i];
             *reinterpret_cast<u32x4_t *>(v_at<D>(vd, r, c >> 1, c & 1)) = vr[i];
@@ -790,16 +797,14 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
 template <class E, bool PAIR, int D>
 __global__ void __launch_bounds__(BT) k_tree_join(Args a, int group_rows) {
     constexpr int CL = D / 8, PL = WAVE / CL;
-    __shared__ Chunks seq;
     const int l = threadIdx.x & 63, c = l % CL, pl = l / CL;
     int id = blockIdx.x;
     const int kvh = id % a.hkv;
     id /= a.hkv;
     const int group = id % a.groups, req = id / a.groups, qrow0 = group * group_rows;
-    lay_out(a, qrow0, seq);
-    const int k0 = seq.before[req], k1 = seq.before[req + 1];
+    const int k0 = gld(a.first + group * (a.n + 1) + req), k1 = gld(a.first + group * (a.n + 1) + req + 1);
     if (k1 - k0 < 2) return;                                      // a block had all of it and has stored it
-    const Where wh = seq.at[req];
+    const Where wh = where_is(a, req);
     const int left = min(group_rows, wh.rows * a.g - qrow0);
     for (int r = blockIdx.y * NW + (threadIdx.x >> 6); r < left; r += gridDim.y * NW) {
         float m = NONE, sum = 0.f;
@@ -865,14 +870,20 @@ Cut cut_of(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys, bool pa
     return c;
 }
 
-// Floats of the parts' rows (then two for each row).
+// Rows of the parts: the workspace has head_dim floats for each, then two for each, then the first chunks.
 size_t part_rows(const navi_kv_pages &p, const navi_kv_heads &h, const Cut &c) {
     return c.workers == 0 ? 0 : static_cast<size_t>(h.n_kv_head) * c.groups * (c.workers + p.n_requests) * c.rows;
 }
 
 size_t workspace(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys) {
     // q's type is not known here: enough for either
-    return std::max(part_rows(p, h, cut_of(p, h, max_keys, false)), part_rows(p, h, cut_of(p, h, max_keys, true))) * (h.head_dim + 2) * sizeof(float);
+    size_t need = 0;
+    for (const bool pair : {false, true}) {
+        const Cut c = cut_of(p, h, max_keys, pair);
+        if (c.workers > 0)
+            need = std::max(need, part_rows(p, h, c) * (h.head_dim + 2) * sizeof(float) + static_cast<size_t>(c.groups) * (p.n_requests + 1) * sizeof(int32_t));
+    }
+    return need;
 }
 
 template <class E, bool PAIR, int D, bool CUT>
@@ -906,7 +917,10 @@ void launch(const Call &x, hipStream_t s) {
     a.v = x.v;
     a.out = x.out;
     a.po = static_cast<float *>(x.ws);
-    a.pm = a.po ? a.po + part_rows(p, h, c) * h.head_dim : nullptr;
+    if (a.po) {
+        a.pm = a.po + part_rows(p, h, c) * h.head_dim;
+        a.first = reinterpret_cast<int32_t *>(a.pm + 2 * part_rows(p, h, c));
+    }
     a.table = p.block_table;
     a.n_past = p.n_past;
     a.cu = p.cu_rows;
