@@ -51,10 +51,10 @@ struct Args {
     const void *q, *k, *v;
     void *out;
     float *po, *pm;                    // the parts of requests that are cut (part_of)
-    int32_t *first;                    // and each group's chunks before every request [groups][n + 1]
+    uint32_t *first;                   // and each group's chunks before every request [groups][n + 1]
     const int32_t *table, *n_past, *cu;
     const uint64_t *mask;
-    int n, hkv, g, blocks, n_pages, n_rows, max_new, ldq, ldkv, ldo, workers, groups, step;
+    int n, hkv, g, blocks, n_pages, n_rows, max_new, ldq, ldkv, ldo, workers, groups, step, parts;
     int tiled;                         // f32 out: in the tile layout of rows.h, heads * D wide
     int flip;                          // scale < 0: the scores' sign goes into q
     Div page, heads_per;               // heads_per: by g
@@ -137,10 +137,11 @@ __device__ __forceinline__ Where where_is(const Args &a, int req) {
 
 // Requests of uneven length over evenly long chunks: with `workers` wanted blocks a kv head and query group, a chunk is
 // at most total / workers steps (of a.step 32-key tiles), and a request is cut into as few even chunks of that as it takes:
-// at most workers + requests of them, in the requests' order.
+// at most workers + requests of them, in the requests' order. At most `workers` requests are longer than a chunk, so that
+// the chunks of cut requests, whose parts are kept, are at most 2 workers.
 constexpr int MAXB = BT;               // most requests of a call that is cut
 struct Chunks {
-    int before[MAXB + 1];              // chunks before request i
+    uint32_t before[MAXB + 1];         // before request i: all chunks, and << 16 those of cut requests
     int steps[MAXB];
     Where at[MAXB];
     int red[NW];
@@ -155,6 +156,10 @@ __device__ __forceinline__ int chunk_steps(const Args &a, float total) {
     return max(total < 16777216.f ? (static_cast<int>(total) + a.workers - 1) / a.workers
                                   : static_cast<int>(total * 1.001f / static_cast<float>(a.workers)) + 1, 1);
 }
+__device__ __forceinline__ uint32_t chunks_of(int steps, int most) {
+    const uint32_t n = static_cast<uint32_t>((steps + most - 1) / most);
+    return n > 1 ? n << 16 | n : n;
+}
 // The first BT threads have a request each; all of a block's threads call it.
 __device__ __forceinline__ void lay_out(const Args &a, int qrow0, Chunks &q) {
     const int t = threadIdx.x, wv = t >> 6;
@@ -165,8 +170,7 @@ __device__ __forceinline__ void lay_out(const Args &a, int qrow0, Chunks &q) {
     if (a.n == 1) {                                               // nothing to add up
         if (own) {
             q.before[0] = 0;
-            const int most = chunk_steps(a, static_cast<float>(steps));
-            q.before[1] = (steps + most - 1) / most;
+            q.before[1] = chunks_of(steps, chunk_steps(a, static_cast<float>(steps)));
             q.steps[0] = steps;
             q.at[0] = w;
         }
@@ -179,7 +183,7 @@ __device__ __forceinline__ void lay_out(const Args &a, int qrow0, Chunks &q) {
     float total = 0.f;
 #pragma unroll
     for (int i = 0; i < NW; ++i) total += q.sum[i];
-    const int most = chunk_steps(a, total), upto = wave_incl_scan((steps + most - 1) / most);
+    const int upto = wave_incl_scan(static_cast<int>(chunks_of(steps, chunk_steps(a, total))));
     if ((t & 63) == 63 && wv < NW) q.red[wv] = upto;
     __syncthreads();
     int off = 0;
@@ -187,21 +191,21 @@ __device__ __forceinline__ void lay_out(const Args &a, int qrow0, Chunks &q) {
     for (int i = 0; i < NW - 1; ++i) off += i < wv ? q.red[i] : 0;
     if (t == 0) q.before[0] = 0;
     if (own) {
-        q.before[t + 1] = off + upto;
+        q.before[t + 1] = static_cast<uint32_t>(off + upto);
         q.steps[t] = steps;
         q.at[t] = w;
     }
     __syncthreads();
 }
-// Where chunk k's part is kept: the group's rows of [D], and (reference, sum) pairs.
+// Where a cut chunk's part is kept: the group's rows of [D], and (reference, sum) pairs.
 __device__ __forceinline__ size_t part_of(const Args &a, int kvh, int group, int k) {
-    return (static_cast<size_t>(kvh) * a.groups + group) * (a.workers + a.n) + k;
+    return (static_cast<size_t>(kvh) * a.groups + group) * a.parts + k;
 }
 
 // A block's share of the work: a request, its tiles t0 .. t_end - 1, and whether these are all it has.
 struct Share {
     Where at;
-    int kvh, group, unit, req, t0, t_end;
+    int kvh, group, req, t0, t_end, part;
     bool whole, none;
 };
 template <bool CUT>
@@ -211,26 +215,29 @@ __device__ __forceinline__ Share share_of(const Args &a, int group_rows) {
     s.kvh = id % a.hkv;
     id /= a.hkv;
     s.group = id % a.groups;
-    s.unit = s.req = id / a.groups;
-    s.t0 = 0;
+    const int unit = id / a.groups;
+    s.req = unit;
+    s.t0 = s.part = 0;
     s.whole = true;
     if constexpr (CUT) {
         __shared__ Chunks c;
         lay_out(a, s.group * group_rows, c);
-        if (s.unit == 0 && s.kvh == 0)                            // for the join
+        if (unit == 0 && s.kvh == 0)                            // for the join
             for (int i = threadIdx.x; i <= a.n; i += blockDim.x) gst(a.first + s.group * (a.n + 1) + i, c.before[i]);
-        s.none = s.unit >= c.before[a.n];
+        auto before = [&](int i) { return static_cast<int>(c.before[i] & 0xFFFFu); };
+        s.none = unit >= before(a.n);
         if (s.none) return s;
         int lo = 0, hi = a.n;                                     // before[lo] <= unit < before[hi]
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (c.before[mid] <= s.unit) lo = mid;
+            if (before(mid) <= unit) lo = mid;
             else hi = mid;
         }
         s.req = lo;
         s.at = c.at[lo];
-        const int n = c.before[lo + 1] - c.before[lo], k = s.unit - c.before[lo], steps = c.steps[lo];
+        const int n = before(lo + 1) - before(lo), k = unit - before(lo), steps = c.steps[lo];
         s.whole = n == 1;
+        s.part = static_cast<int>(c.before[lo] >> 16) + k;
         s.t0 = static_cast<int>(static_cast<int64_t>(steps) * k / n) * a.step;
         s.t_end = min((s.at.len + KT - 1) / KT, static_cast<int>(static_cast<int64_t>(steps) * (k + 1) / n) * a.step);
     } else {
@@ -435,7 +442,7 @@ struct Rows {
         const int q = s.group * group_rows + r, j = div_by(a.heads_per, q);
         if (j >= s.at.rows) return;
         if (!s.whole) {
-            const size_t at = part_of(a, s.kvh, s.group, s.unit) * group_rows + r;
+            const size_t at = part_of(a, s.kvh, s.group, s.part) * group_rows + r;
             st4(a.po + at * D + col, o);
             if (col == 0) {
                 gst(a.pm + 2 * at, m);
@@ -802,8 +809,9 @@ __global__ void __launch_bounds__(BT) k_tree_join(Args a, int group_rows) {
     const int kvh = id % a.hkv;
     id /= a.hkv;
     const int group = id % a.groups, req = id / a.groups, qrow0 = group * group_rows;
-    const int k0 = gld(a.first + group * (a.n + 1) + req), k1 = gld(a.first + group * (a.n + 1) + req + 1);
-    if (k1 - k0 < 2) return;                                      // a block had all of it and has stored it
+    const uint32_t b0 = gld(a.first + group * (a.n + 1) + req), b1 = gld(a.first + group * (a.n + 1) + req + 1);
+    const int k0 = static_cast<int>(b0 >> 16), k1 = static_cast<int>(b1 >> 16);
+    if (k0 == k1) return;                                         // a block had all of it and has stored it
     const Where wh = where_is(a, req);
     const int left = min(group_rows, wh.rows * a.g - qrow0);
     for (int r = blockIdx.y * NW + (threadIdx.x >> 6); r < left; r += gridDim.y * NW) {
@@ -846,7 +854,7 @@ __global__ void __launch_bounds__(BT) k_tree_join(Args a, int group_rows) {
 // How a call is cut: query tiles and, above 32 query rows, waves that share them (waves 1: none share), rows of a group and
 // groups, and blocks wanted for a kv head and group (0: one a request).
 struct Cut {
-    int tiles, waves, rows, groups, workers, step;
+    int tiles, waves, rows, groups, workers, step, parts;
 };
 Cut cut_of(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys, bool pair) {
     const int m = std::min(p.max_new, 64) * (h.n_head / h.n_kv_head);
@@ -862,17 +870,18 @@ Cut cut_of(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys, bool pa
     // A block a request where no request can be long and there are blocks for all CUs (32 requests of 1024 keys: 27.3 us,
     // cut 33.3: the chunks and the join), or more requests than a block lays out. Else enough blocks for all waves of the CUs.
     if (p.n_requests > MAXB || steps == 1 || (max_keys <= 2048 && p.n_requests * heads >= 256)) {
-        c.workers = 0;
+        c.workers = c.parts = 0;
         return c;
     }
     const int64_t blocks = 2048 / waves;                           // two waves a SIMD
     c.workers = static_cast<int>(std::max<int64_t>(1, std::min((blocks + heads - 1) / heads, static_cast<int64_t>(steps) * p.n_requests)));
+    c.parts = std::min(c.workers + p.n_requests, 2 * c.workers);
     return c;
 }
 
 // Rows of the parts: the workspace has head_dim floats for each, then two for each, then the first chunks.
-size_t part_rows(const navi_kv_pages &p, const navi_kv_heads &h, const Cut &c) {
-    return c.workers == 0 ? 0 : static_cast<size_t>(h.n_kv_head) * c.groups * (c.workers + p.n_requests) * c.rows;
+size_t part_rows(const navi_kv_heads &h, const Cut &c) {
+    return static_cast<size_t>(h.n_kv_head) * c.groups * c.parts * c.rows;
 }
 
 size_t workspace(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys) {
@@ -881,7 +890,7 @@ size_t workspace(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys) {
     for (const bool pair : {false, true}) {
         const Cut c = cut_of(p, h, max_keys, pair);
         if (c.workers > 0)
-            need = std::max(need, part_rows(p, h, c) * (h.head_dim + 2) * sizeof(float) + static_cast<size_t>(c.groups) * (p.n_requests + 1) * sizeof(int32_t));
+            need = std::max(need, part_rows(h, c) * (h.head_dim + 2) * sizeof(float) + static_cast<size_t>(c.groups) * (p.n_requests + 1) * sizeof(int32_t));
     }
     return need;
 }
@@ -918,8 +927,8 @@ void launch(const Call &x, hipStream_t s) {
     a.out = x.out;
     a.po = static_cast<float *>(x.ws);
     if (a.po) {
-        a.pm = a.po + part_rows(p, h, c) * h.head_dim;
-        a.first = reinterpret_cast<int32_t *>(a.pm + 2 * part_rows(p, h, c));
+        a.pm = a.po + part_rows(h, c) * h.head_dim;
+        a.first = reinterpret_cast<uint32_t *>(a.pm + 2 * part_rows(h, c));
     }
     a.table = p.block_table;
     a.n_past = p.n_past;
@@ -937,6 +946,7 @@ void launch(const Call &x, hipStream_t s) {
     a.ldo = x.ldo;
     a.workers = c.workers;
     a.step = c.step;
+    a.parts = c.parts;
     a.groups = c.groups;
     a.tiled = x.tiled;
     a.page = kv::make_div(static_cast<uint32_t>(p.page_size));

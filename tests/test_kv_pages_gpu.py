@@ -247,6 +247,24 @@ def test_split_over_blocks(kind, past, nodes):
     assert torch.equal(a, s.attend(128 ** -0.5)), "the same call twice"
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [2, 33, 255, 256, 257, 300])
+def test_many_requests(kind, n):
+    """Up to 256 requests are cut into chunks, more are not; some long, some short, some without rows."""
+    rng = np.random.default_rng(n)
+    reqs = [(int(np.exp(rng.uniform(0, 8))) if i % 50 == 1 else int(rng.integers(0, 60)), random_tree(rng, int(rng.integers(0, 4)))) for i in range(n)]
+    reqs[0] = (4000, [-1, 0])
+    Step(reqs, kind=kind, heads=2, kv_heads=1, dim=64, page=16, seed=n).fill().check()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,dim,nodes,past", [(64, 2, 64, 5, 70), (32, 1, 128, 9, 600), (48, 1, 64, 64, 33), (8, 8, 64, 33, 4000), (6, 2, 128, 43, 1500)])
+def test_large_groups_and_row_counts(kind, heads, kv, dim, nodes, past):
+    """Query rows that fill several groups of 128, or leave the last of them nearly empty."""
+    rng = np.random.default_rng(past)
+    Step([(past, random_tree(rng, nodes)), (past // 3, random_tree(rng, 2))], kind=kind, heads=heads, kv_heads=kv, dim=dim, seed=past).fill().check()
+
+
 @pytest.mark.parametrize("past", [40, 700])
 def test_more_keys_than_announced(past):
     s = Step([(past, [-1, 0, 0]), (3, [-1])], heads=4, kv_heads=2, seed=past).fill()
