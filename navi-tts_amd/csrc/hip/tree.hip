@@ -467,6 +467,16 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
     __shared__ __align__(16) unsigned char sm[W * VB + QB > JOIN ? W * VB + QB : JOIN];
     __shared__ float s_fac[NT * 16], s_ref[W][NT * 16], s_sum[W][NT * 16];
     const int wv = threadIdx.x >> 6, l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+    // uncut, the first tile's pages do not wait for the request's lengths: a round of memory latency less
+    int ahead[2];
+    if constexpr (!CUT) {
+        const int req = static_cast<int>(blockIdx.x) / a.hkv / a.groups;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            const int b = div_by(a.page, wv * KT + kt * 16 + lr);
+            ahead[kt] = b < a.blocks ? gld(a.table + static_cast<size_t>(req) * a.blocks + b) : -1;
+        }
+    }
     const Share s = share_of<CUT>(a, NT * 16);
     if (s.none) return;
     const int qrow0 = s.group * NT * 16;
@@ -492,7 +502,12 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
         }
     };
     int t = s.t0 + wv;
-    if (t < s.t_end) look_up(t);
+    if constexpr (CUT) {
+        if (t < s.t_end) look_up(t);
+    } else {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) page[kt] = t * KT + kt * 16 + lr < s.at.len ? ahead[kt] : -1;
+    }
     R rows;
     rows.start(a, s, qrow0);
     if (t < s.t_end) {
@@ -867,9 +882,10 @@ Cut cut_of(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys, bool pa
     const int waves = c.waves == 1 ? alone_of(true) : waves_of(pair, c.waves);
     c.step = waves / c.waves;                           // tiles of a block's turn
     const int steps = (max_keys + KT * c.step - 1) / (KT * c.step);
-    // A block a request where no request can be long and there are blocks for all CUs (32 requests of 1024 keys: 27.3 us,
-    // cut 33.3: the chunks and the join), or more requests than a block lays out. Else enough blocks for all waves of the CUs.
-    if (p.n_requests > MAXB || steps == 1 || (max_keys <= 2048 && p.n_requests * heads >= 256)) {
+    // A block a request where no request can be long enough to share (one row of 16 heads over 256 keys: 9.3 us, cut 10.6; over
+    // 512: 12.4 and 10.6), or moderately long with blocks for all CUs (32 requests of 1024 keys: 26.6 us, cut 33.3: the chunks
+    // and the join), or for more requests than a block lays out. Else enough blocks for all waves of the CUs.
+    if (p.n_requests > MAXB || steps == 1 || (c.waves == 1 && max_keys <= 384) || (max_keys <= 2048 && p.n_requests * heads >= 256)) {
         c.workers = c.parts = 0;
         return c;
     }
