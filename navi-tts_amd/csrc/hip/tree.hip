@@ -13,13 +13,19 @@
 //  * V^T's operand is V read from LDS through the transposing load (ds_read_b64_tr_b16: in a
 //    16-lane group lane 4r + c fetches columns 4c.. of key r and gets column `lane`, keys 0..3). V rows sit
 //    in LDS with their 32-byte chunks XORed by the key, so that the 16 rows such a load touches
-//    spread over all banks. K goes from memory to registers in operand form.
-//  * A wave works alone on its own 32-key tiles (every fourth of the block's range), with its own V buffer
-//    and no barrier until its range ends; then the block's four partial results are joined in LDS.
+//    spread over all banks.
+//  * Up to 32 query rows (k_tree) a wave works alone on its own 32-key tiles, every W-th of the block's range, with K from
+//    memory in operand form, its own V buffer and no barrier until its range ends; then the waves' results are joined in
+//    LDS. 32 requests with one row each over 1024 keys take 26.6 us, 5.07 TB/s: the cache's bytes at the rate of a large
+//    read (5.6 TB/s here) are 24.
+//  * Above (k_tree_rows) two or four waves with 32 rows each share the K and V tiles, which go through LDS in two buffers with
+//    one barrier a tile. 64 requests x 24 rows (48 query rows) over 8192 keys 415 us, 5.2 TB/s; without the products 385.
+//    64 f32 rows (128 query rows) over 32768 keys 59 us: 39 us for every further 32768 keys, which with the pairs' doubled
+//    products are 880 TFLOP/s, and 20 us for the start, the parts' 17 MB and the join.
 //  * Softmax against a reference value that moves only when a score passes it by more than SLACK: the
 //    rescaling, and the maximum over lanes that it needs, are off the common path. exp2 with the scale folded in.
-//  * Few requests: a request's keys are split over several blocks, whose partial results (unnormalised sums,
-//    reference, sum) a second kernel joins in split order.
+//  * Requests are cut into even chunks over the blocks, however uneven their lengths (lay_out): 64 requests of lengths spread from
+//    1 to 8000 72 us, uncut 151. A second kernel joins the chunks' results (unnormalised sums, reference, sum) in their order.
 #include "dev_common.h"
 #include "tile_layout.h"
 #include "tree.h"
@@ -34,8 +40,8 @@ using kv::Div;
 using kv::div_by;
 
 constexpr int NW = 4, BT = NW * WAVE;  // waves of a block of k_tree_join
-// Of k_tree: eight, more loads on their way, where a block has a whole request (32 requests of 1024 keys: 27.3 us, with four
-// 31.0); four, and twice as many blocks, where requests are cut (64 ragged ones of up to 8000 keys: 73 us, with eight 85).
+// Of k_tree: eight, more loads on their way, where a block has a whole request (32 requests of 1024 keys: 26.6 us, with four
+// 31.0); four, and twice as many blocks, where requests are cut (64 ragged ones of up to 8000 keys: 72 us, with eight 85).
 constexpr int alone_of(bool cut) { return cut ? 4 : 8; }
 // Of k_tree_rows, RW waves of which share their query rows' tiles: eight, one block a CU, so that half as many parts of
 // a cut request are stored and joined (64 drafted rows over 32768 keys: 57 us, with four 64); four where two waves share and
@@ -883,9 +889,11 @@ Cut cut_of(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys, bool pa
     c.step = waves / c.waves;                           // tiles of a block's turn
     const int steps = (max_keys + KT * c.step - 1) / (KT * c.step);
     // A block a request where no request can be long enough to share (one row of 16 heads over 256 keys: 9.3 us, cut 10.6; over
-    // 512: 12.4 and 10.6), or moderately long with blocks for all CUs (32 requests of 1024 keys: 26.6 us, cut 33.3: the chunks
-    // and the join), or for more requests than a block lays out. Else enough blocks for all waves of the CUs.
-    if (p.n_requests > MAXB || steps == 1 || (c.waves == 1 && max_keys <= 384) || (max_keys <= 2048 && p.n_requests * heads >= 256)) {
+    // 512: 12.4 and 10.6); where there are blocks for all CUs and no request is so long that an uneven one would cost more than
+    // the chunks and the join (one row of 32 requests, all alike and of lengths spread down to one: of 1000 keys 26.4 and 20.7 us,
+    // cut 30.7 and 14.8; of 1400 39.7 and 26.2, cut 45.6 and 19.4; of 2000 56.5 and 35.8, cut 61.8 and 23.6); and for more
+    // requests than a block lays out. Else enough blocks for all waves of the CUs.
+    if (p.n_requests > MAXB || steps == 1 || (c.waves == 1 && max_keys <= 384) || (max_keys <= 1280 && p.n_requests * heads >= 256)) {
         c.workers = c.parts = 0;
         return c;
     }
