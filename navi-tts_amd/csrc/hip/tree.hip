@@ -133,7 +133,7 @@ struct Where {
 __device__ __forceinline__ Where where_is(const Args &a, int req) {
     const int64_t room = min(static_cast<int64_t>(a.blocks) * a.page.d, static_cast<int64_t>(INT32_MAX - 4 * KT * NW));
     Where w;
-    w.c0 = gld(a.cu + req);
+    w.c0 = max(gld(a.cu + req), 0);
     const int count = max(min(gld(a.cu + req + 1), a.n_rows) - w.c0, 0);
     w.rows = min(count, a.max_new);
     w.past = static_cast<int>(min<int64_t>(max(gld(a.n_past + req), 0), room));

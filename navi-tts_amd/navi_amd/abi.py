@@ -799,8 +799,7 @@ def kv_commit(pages: KvPages, k, v, ld_kv: int, path: int, max_path: int, accept
               stream: int | None = None):
     """navi_kv_commit: the accepted rows of each request moved into place in every layer; k, v: one address a layer."""
     n = len(k)
-    kp, vp = (C.c_void_p * n)(*k), (C.c_void_p * n)(*v)
-    view = KvView(n, pages.n_pages * pages.page_size, ld_kv, C.cast(kp, C.POINTER(C.c_void_p)), C.cast(vp, C.POINTER(C.c_void_p)))
+    view = KvView(n, pages.n_pages * pages.page_size, ld_kv, (C.c_void_p * n)(*k), (C.c_void_p * n)(*v))
     err = C.create_string_buffer(256)
     _check(lib().navi_kv_commit(pages, view, path, max_path, accept, n_past, status, stream, err, 256), err)
 

@@ -353,6 +353,20 @@ def test_lengths_out_of_range_stay_in_the_table():
     assert bool(torch.isfinite(out[2 ** 31 - 1]).all())
 
 
+def test_fewer_rows_than_the_requests_have():
+    """n_rows below cu_rows' end: the rows past it are neither read nor written."""
+    s = Step([(40, [-1, 0, 0, 0]), (10, [-1, 0, 1])], heads=4, kv_heads=2).fill()
+    want, tol = s.expect(0.1)
+    s.device()
+    s.n_rows = 5
+    q, k, v = s.q[:5].cuda(), s.k.cuda(), s.v.cuda()
+    out = torch.full((7, 512), 7.0, dtype=torch.float16, device="cuda")
+    abi.tree_attention(s.pages(), s.layout(), q.data_ptr(), 1, 512, k.data_ptr(), v.data_ptr(), s.ld, 0.1, s.max_keys, out.data_ptr(), 512, None, 0, stream=stream())
+    torch.cuda.synchronize()
+    got = out.cpu().double().numpy().reshape(7, 4, 128)
+    assert (np.abs(got - want) <= tol)[:5].all() and (got[5:] == 7).all()
+
+
 def test_rows_past_four_gigabytes():
     """Slots whose byte offset passes 32 bits and whose element offset passes 31."""
     heads, kv, dim, page, rows = 16, 8, 128, 16, 2_200_000 // 16 * 16
