@@ -310,10 +310,11 @@ typedef struct {
  *      outside 0 .. max_blocks, or rows past n_rows
  *   3  a parent that does not come before its row
  * A request with a status other than 0 keeps its pages and takes none; its rows get slot -1 (and
- * position and mask 0 unless the status is 1). row_mask bit a is set for the row's ancestors and itself; without
- * d_parent, for rows 0 .. min(own index, 63). Table entries past the held pages are -1; entries of row_*
- * past the last request's rows are left as they were. d_held, d_free and pages->block_table may be
- * d_held_in, d_free_in and d_table_in. d_scratch: 4 * n_requests words. */
+ * position and mask 0 unless the status is 1), and their attention holds nothing of use. row_mask bit a
+ * is set for the row's ancestors and itself; without d_parent, for rows 0 .. min(own index, 63). Table
+ * entries past the held pages are -1; entries of row_* past the last request's rows are left as they
+ * were. d_held, d_free and pages->block_table may be d_held_in, d_free_in and d_table_in. d_scratch: 4 *
+ * n_requests words, 16-byte aligned, for this call alone until it is done. */
 navi_status navi_kv_plan(const navi_kv_pages *pages, const int32_t *d_n_new, const int32_t *d_parent, const int32_t *d_table_in,
                          const int32_t *d_held_in, const int32_t *d_free_in, int32_t *d_free_pages, int32_t *d_held,
                          int32_t *d_free, int32_t *d_status, int32_t *d_scratch, void *stream, char *err, size_t errlen);
@@ -337,7 +338,7 @@ navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *head
  * infinities and NaN included; a position whose page is outside the pool is not seen; a row that sees
  * nothing gets zeros. Rows past cu_rows[n_requests] and past max_new of a request are left as they were.
  * max_keys: the most positions a request may reach (n_past + rows), by which the work is split; longer
- * requests are still right, but slow. d_ws: navi_tree_workspace(...) bytes, 16-byte aligned, for this call
+ * requests are still right, but slow. n_requests * n_head < 2^23. d_ws: navi_tree_workspace(...) bytes, 16-byte aligned, for this call
  * alone until it is done: calls that may overlap need a workspace each. Alignment as navi_kv_append. */
 navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads *heads, const void *d_q, int32_t q_dtype, int32_t ldq,
                                 const void *d_k, const void *d_v, int32_t ld_kv, float scale, int32_t max_keys, void *d_out,
@@ -347,7 +348,7 @@ size_t navi_tree_workspace(const navi_kv_pages *pages, const navi_kv_heads *head
 /* The accepted rows of each request moved into place in every layer of `kv` (n_layer, max_pos >= the pool's rows, kv_dim the
  * row stride, a multiple of 8): with path = d_path[i][0 .. d_accept[i] - 1] (stride max_path <= 64), the indexes of accepted rows within
  * the request's step in ascending order, position n_past[i] + j takes the K and V of position n_past[i] + path[j].
- * d_n_past_out[i] = n_past[i] + d_accept[i] (not the array n_past itself). d_status[i]: 0, or 2 where d_accept[i] is outside
+ * d_n_past_out[i] = n_past[i] + d_accept[i]. d_n_past_out and d_status are none of the call's inputs. d_status[i]: 0, or 2 where d_accept[i] is outside
  * 0 .. max_path, the path does not ascend or leaves the request's rows, or a page is outside the pool: nothing is moved and
  * d_n_past_out[i] = n_past[i]. Pages past the new length stay with the request. */
 navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, const int32_t *d_path, int32_t max_path,
@@ -359,8 +360,9 @@ navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, c
  * every row's post-norm hidden in d_hidden f32 [n_rows][hidden] and its logits in d_logits f32 [n_rows][vocab]
  * (NULL: not computed). kv: the pool (n_layer, kv_dim and at least n_pages * page_size rows as navi_talker_kv's), or NULL: the
  * talker's own cache, whose max_positions rows are then the pages. n_rows <= max_prompt_tokens, max_new <= 64.
- * max_keys as in navi_tree_attention, at most max_positions; positions past it get no K and V. Rows that belong to no
- * request hold nothing of use. Errors as navi_talker_prefill.
+ * max_keys as in navi_tree_attention, at most max_positions; rows at positions past max_positions get no K and V. Rows of no
+ * request, or of one that the plan refused, are taken as zeros, so that they do not fail the call; their results hold
+ * nothing of use. Errors as navi_talker_prefill.
  * Runs on the library stream (plan on it too) and is synchronous; navi_talker_last_ms is its device time. */
 navi_status navi_talker_verify(navi_talker *t, const navi_kv_view *kv, const navi_kv_pages *pages, int32_t max_keys, const float *d_rows,
                                float *d_hidden, float *d_logits, char *err, size_t errlen);

@@ -56,9 +56,9 @@ struct OnDevice {
 navi_status check_pages(const char *who, const navi_kv_pages *p, char *err, size_t errlen);
 navi_status check_heads(const char *who, const navi_kv_heads *h, int ld_kv, char *err, size_t errlen);
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-// Rows of `type` elements with stride ld >= width start on 16 bytes.
-inline bool rows_ok(const void *p, int type, int ld, long width) {
-    return p && aligned16(p) && ld >= width && ld % (type == NAVI_DT_F32 ? 4 : 8) == 0;
+// `rows` rows (of none: p may be null) of `type` elements with stride ld >= width start on 16 bytes.
+inline bool rows_ok(const void *p, int rows, int type, int ld, long width) {
+    return (p || rows == 0) && aligned16(p) && ld >= width && ld % (type == NAVI_DT_F32 ? 4 : 8) == 0;
 }
 
 } // namespace kv

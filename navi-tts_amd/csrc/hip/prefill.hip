@@ -502,6 +502,18 @@ __global__ void __launch_bounds__(BT) k_tiled_rows_norm(const float *x, const fl
     st4(y + static_cast<size_t>(blockIdx.x) * H + i, o);
 }
 
+// Rows of a planned step that are no request's (past cu[n], or without a slot): zeros in the residual stream, and in the
+// attention's output, which is not written for all of them, so that nothing they hold reaches the f16-range check. Row = block,
+// of att up to the last tile's 16.
+__global__ void __launch_bounds__(BT) k_unowned(float *x, int T, int H, float *att, int QD, const int32_t *cu, int n, const int32_t *slot) {
+    const int r = blockIdx.x;
+    if (r < min(gld(cu + n), T) && gld(slot + r) >= 0) return;
+    const f32x4_t zero{0.f, 0.f, 0.f, 0.f};
+    if (r < T)
+        for (int i = threadIdx.x * 4; i < H; i += BT * 4) st4(x + rows::pk_a(r, i, H), zero);
+    for (int i = threadIdx.x * 4; i < QD; i += BT * 4) st4(att + rows::pk_a(r, i, QD), zero);
+}
+
 } // namespace pf
 } // namespace navi_amd
 
@@ -1090,8 +1102,8 @@ navi_status navi_talker_verify(navi_talker *t, const navi_kv_view *kv, const nav
     NAVI_TRY_HIP(hipEventRecord(t->ev0, s), err, errlen);
     rows::tile_rows(d_rows, T, H, t->x, s, t->flag);
     t->flag_set = true;
-    // rows that belong to no request are not written by the attention: zeros, not what a prefill left there
-    NAVI_TRY_HIP(hipMemsetAsync(t->att, 0, static_cast<size_t>((T + 15) / 16 * 16) * t->QD * sizeof(float), s), err, errlen);
+    hipLaunchKernelGGL(k_unowned, dim3((T + 15) / 16 * 16), dim3(BT), 0, s, t->x, T, H, t->att, t->QD, pages->cu_rows, pages->n_requests,
+                       pages->row_slot);
     for (int l = 0; l < t->L; ++l) {
         const LayerW &w = t->layers[l];
         bool ok = rows::launch_rows_pk(rows::EPI_PLAIN, true, t->x, T, H, w.ln1, t->eps, w.qkv_t, QKVW, t->part, QKVW, t->flag, s);
@@ -1099,7 +1111,7 @@ navi_status navi_talker_verify(navi_talker *t, const navi_kv_view *kv, const nav
                             t->q, NAVI_DT_F32, t->QD, s, err, errlen);
         if (st != NAVI_OK) return st;
         tree::launch({pages, &heads, t->q, kv->k[l], kv->v[l], t->att, t->tree_ws, t->tree_bytes, NAVI_DT_F32, t->QD, t->KVD, t->QD, max_keys,
-                      1.f / std::sqrt(static_cast<float>(HD)), true}, s);
+                      1.f / std::sqrt(static_cast<float>(HD)), true, true}, s);
         ok = ok && rows::launch_rows_pk(rows::EPI_RESID, false, t->att, T, t->QD, nullptr, 0.f, w.o_t, H, t->x, 0, t->flag, s) &&
              rows::launch_rows_pk(rows::EPI_SWIGLU, true, t->x, T, H, w.ln2, t->eps, w.gu_t, t->F, t->h, 0, t->flag, s) &&
              rows::launch_rows_pk(rows::EPI_RESID, false, t->h, T, t->F, nullptr, 0.f, w.d_t, H, t->x, 0, t->flag, s);

@@ -58,7 +58,7 @@ struct Args {
     void *out;
     float *po, *pm;                    // the parts of requests that are cut (part_of)
     uint32_t *first;                   // and each group's chunks before every request [groups][n + 1]
-    const int32_t *table, *n_past, *cu;
+    const int32_t *table, *n_past, *cu, *slot;   // slot: null, or rows with slot < 0 see no row of the step
     const uint64_t *mask;
     int n, hkv, g, blocks, n_pages, n_rows, max_new, ldq, ldkv, ldo, workers, groups, step, parts;
     int tiled;                         // f32 out: in the tile layout of rows.h, heads * D wide
@@ -330,7 +330,7 @@ struct Rows {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int j = div_by(a.heads_per, qrow0 + nt * 16 + lr);
-            seen[nt] = j < s.at.rows ? gld(a.mask + s.at.c0 + j) : 0;
+            seen[nt] = j < s.at.rows && (!a.slot || gld(a.slot + s.at.c0 + j) >= 0) ? gld(a.mask + s.at.c0 + j) : 0;
             ref[nt] = NONE;
             sub[nt] = sum[nt] = 0.f;
 #pragma unroll
@@ -957,6 +957,7 @@ void launch(const Call &x, hipStream_t s) {
     a.table = p.block_table;
     a.n_past = p.n_past;
     a.cu = p.cu_rows;
+    a.slot = x.slots ? p.row_slot : nullptr;
     a.mask = p.row_mask;
     a.n = p.n_requests;
     a.hkv = h.n_kv_head;
@@ -1017,7 +1018,7 @@ navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads 
         set_err(err, errlen, "tree_attention: up to %d rows a request; at most 64", pages->max_new);
         return NAVI_ERR_INVALID;
     }
-    if (!kv::rows_ok(d_q, q_dtype, ldq, width) || !kv::rows_ok(d_out, q_dtype, ldo, width) || !d_k || !d_v || !kv::aligned16(d_k) ||
+    if (!kv::rows_ok(d_q, pages->n_rows, q_dtype, ldq, width) || !kv::rows_ok(d_out, pages->n_rows, q_dtype, ldo, width) || !d_k || !d_v || !kv::aligned16(d_k) ||
         !kv::aligned16(d_v)) {
         set_err(err, errlen, "tree_attention: a null or misaligned pointer, or a stride too small (ldq %d, ldo %d)", ldq, ldo);
         return NAVI_ERR_INVALID;
@@ -1026,7 +1027,8 @@ navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads 
         set_err(err, errlen, "tree_attention: max_keys %d out of range", max_keys);
         return NAVI_ERR_INVALID;
     }
-    if (static_cast<int64_t>(pages->n_requests) * heads->n_head * 64 > INT32_MAX) {
+    // at most n_requests * n_head blocks of 512 threads, and a launch has less than 2^32
+    if (static_cast<int64_t>(pages->n_requests) * heads->n_head * 512 > UINT32_MAX) {
         set_err(err, errlen, "tree_attention: %d requests of %d heads are too many for one call", pages->n_requests, heads->n_head);
         return NAVI_ERR_INVALID;
     }
@@ -1038,7 +1040,8 @@ navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads 
     kv::OnDevice dev;
     if ((st = dev.enter(stream, "tree_attention", err, errlen)) != NAVI_OK) return st;
     if (pages->n_rows == 0) return NAVI_OK;
-    tree::launch({pages, heads, d_q, d_k, d_v, d_out, d_ws, ws_bytes, q_dtype, ldq, ld_kv, ldo, max_keys, scale, false}, static_cast<hipStream_t>(stream));
+    tree::launch({pages, heads, d_q, d_k, d_v, d_out, d_ws, ws_bytes, q_dtype, ldq, ld_kv, ldo, max_keys, scale, false, false},
+                 static_cast<hipStream_t>(stream));
     NAVI_TRY_HIP(hipGetLastError(), err, errlen);
     return NAVI_OK;
 }

@@ -207,6 +207,27 @@ def test_append_over_its_own_input_and_without_rows():
     torch.cuda.synchronize()
 
 
+def test_a_step_without_rows():
+    """All requests have ended: their pages go back, the row arrays and the rows may be null, nothing else is written."""
+    n, blocks = 3, 4
+    table, held, free, stack = i32(range(12)), i32([4, 0, 2]), i32([0]), i32([TOUCH] * 12)
+    past, new, cu, status, scratch = i32([60, 0, 17]), i32([-1, -1, -1]), i32([7] * 4), i32([7] * 3), i32([0] * 12)
+    pages = abi.KvPages(n, 16, 12, blocks, 0, 8, table.data_ptr(), past.data_ptr(), cu.data_ptr(), None, None, None)
+    abi.kv_plan(pages, n_new=new.data_ptr(), table_in=table.data_ptr(), held_in=held.data_ptr(), free_in=free.data_ptr(), free_pages=stack.data_ptr(),
+                held=held.data_ptr(), free=free.data_ptr(), status=status.data_ptr(), scratch=scratch.data_ptr(), stream=stream())
+    heads = abi.KvHeads(4, 2, 64, abi.DT_BF16)
+    k = torch.ones(12 * 16, 128, device="cuda").bfloat16()
+    abi.kv_append(pages, heads, None, 0, 512, k.data_ptr(), k.data_ptr(), 128, None, 0, 256, stream=stream())
+    ws = torch.empty(max(16, abi.tree_workspace(pages, heads, 640)), dtype=torch.uint8, device="cuda")
+    abi.tree_attention(pages, heads, None, abi.DT_BF16, 256, k.data_ptr(), k.data_ptr(), 128, 1.0, 640, None, 256, ws.data_ptr(), ws.numel(), stream=stream())
+    path, accept, out, st = i32([0] * 3), i32([0] * 3), i32([-5] * 3), i32([9] * 3)
+    abi.kv_commit(pages, [k.data_ptr()], [k.data_ptr()], 128, path.data_ptr(), 1, accept.data_ptr(), out.data_ptr(), st.data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    assert table.tolist() == [-1] * 12 and held.tolist() == [0] * 3 and free.tolist() == [6]
+    assert stack.tolist()[:6] == [0, 1, 2, 3, 8, 9] and cu.tolist() == [0] * 4 and status.tolist() == [0] * 3
+    assert out.tolist() == past.tolist() and st.tolist() == [0] * 3 and bool((k == 1).all())
+
+
 # ---- attention -------------------------------------------------------------------------------------
 
 KINDS = ["f32", "f16", "bf16"]

@@ -80,6 +80,14 @@ def test_append_refuses_more_rows_than_a_grid_holds():
     refused(4, *a, **k)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_launches_of_2_to_32_threads_are_refused(dim):
+    """Append: dim / 8 threads a head; attention: 512 threads a request and head."""
+    a, k = _append(pages(n_rows=(1 << 32) // (dim // 8) // 32), heads(head_dim=dim))
+    assert "too many" in refused(4, *a, **k)
+    assert "too many" in refused(4, *_attend(pages(n_requests=1 << 14), heads(n_head=512, n_kv_head=8, head_dim=dim), ldq=1 << 16, ldo=1 << 16))
+
+
 def _attend(pages_=None, heads_=None, q=P, qt=0, ldq=2048, k=P, v=P, ld=1024, keys=64, out=P, ldo=2048, ws=P, size=1 << 40):
     return abi.tree_attention, pages_ or pages(), heads_ or heads(), q, qt, ldq, k, v, ld, 1.0, keys, out, ldo, ws, size
 
@@ -113,6 +121,16 @@ def test_commit_refuses(kw):
     d = dict(k=[P], v=[P], ld=1024, path=P, max_path=4, accept=P, n_past=P + 64, status=P)
     d.update(kw)
     refused(4, abi.kv_commit, pages(), d["k"], d["v"], d["ld"], d["path"], d["max_path"], d["accept"], d["n_past"], d["status"])
+
+
+@pytest.mark.parametrize("name,other", [(a, b) for a in ("n_past", "status") for b in ("past", "cu", "table", "path", "accept")] + [("n_past", "status")])
+def test_commit_refuses_results_over_inputs(name, other):
+    """Other blocks read the inputs until the launch ends: in place would be a race."""
+    at = dict(table=P, past=P + 64, cu=P + 128, path=P + 192, accept=P + 256, n_past=P + 320, status=P + 384)
+    at[name] = at[other]
+    p = pages()
+    p.block_table, p.n_past, p.cu_rows = at["table"], at["past"], at["cu"]
+    assert "inputs" in refused(4, abi.kv_commit, p, [P], [P], 1024, at["path"], 4, at["accept"], at["n_past"], at["status"])
 
 
 def test_commit_refuses_a_cache_smaller_than_the_pool():

@@ -1,6 +1,9 @@
 """navi_talker_verify over planned steps against the CPU oracle: a prompt prefilled into the talker's own cache and one
 taken in as a chain of rows, trees of drafted rows on both, the accepted rows committed, and the next step on what
 was committed. Bars as the prefill's: 2e-2 max abs and cosine > 0.9995 against the oracle's rows."""
+import ctypes as C
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 import torch
@@ -38,13 +41,13 @@ class Pool:
         self.table, self.held, self.free, self.stack = i32(table), i32([len(taken.get(i, [])) for i in range(n)]), i32([len(rest)]), i32(rest + [0] * (self.n_pages - len(rest)))
         self.past = i32([0] * n)
 
-    def step(self, trees, rows, kv=None, logits=True, spare=0):
+    def step(self, trees, rows, kv=None, logits=True, spare=0, spare_value=0., status=None):
         abi, new = self.abi, [len(t) for t in trees]
         R = sum(new) + spare
         self.cu, self.slot, self.pos, self.status = i32([0] * (self.n + 1)), i32([-1] * R), i32([0] * R), i32([0] * self.n)
         self.mask, scratch = torch.zeros(R, dtype=torch.int64, device="cuda"), i32([0] * 4 * self.n)
         d_new, d_par = i32(new), i32([p for t in trees for p in t] + [0] * spare)
-        d_rows = torch.cat([torch.from_numpy(np.concatenate(rows).astype(np.float32)), torch.zeros(spare, 1024)]).cuda()
+        d_rows = torch.cat([torch.from_numpy(np.concatenate(rows).astype(np.float32)), torch.full((spare, 1024), spare_value)]).cuda()
         hid, lg = torch.zeros(R, 1024, device="cuda"), torch.zeros(R, self.t.params.talker.vocab, device="cuda")
         self.pages = abi.KvPages(self.n, PAGE, self.n_pages, self.blocks, R, 64, *(x.data_ptr() for x in (self.table, self.past, self.cu, self.slot, self.pos, self.mask)))
         torch.cuda.synchronize()
@@ -52,7 +55,7 @@ class Pool:
                     free_in=self.free.data_ptr(), free_pages=self.stack.data_ptr(), held=self.held.data_ptr(), free=self.free.data_ptr(),
                     status=self.status.data_ptr(), scratch=scratch.data_ptr(), stream=abi.lib().navi_device_stream())
         self.t.verify(self.pages, self.blocks * PAGE, d_rows.data_ptr(), hid.data_ptr(), lg.data_ptr() if logits else None, kv=kv)
-        assert self.status.tolist() == [0] * self.n
+        assert self.status.tolist() == (status or [0] * self.n)
         return hid.cpu().numpy(), lg.cpu().numpy()
 
     def commit(self, paths, kv):
@@ -143,6 +146,37 @@ def test_a_row_does_not_depend_on_the_other_requests(side):
         h2, _ = Pool(abi, talker, 1, {}).step([t], [xi], kv=kv, logits=False)
         assert np.array_equal(h, h2)
         at += len(t)
+
+
+def test_a_refused_request_and_padding_do_not_spoil_the_others(side):
+    """A pool whose unwritten rows are NaN, a request that gets no page while it holds a part of one, rows of no request that are NaN:
+    the other request's results are those it has alone, and the call succeeds."""
+    abi, _, talker, _ = side
+    L, rng = talker.kv.n_layer, np.random.default_rng(8)
+    pool = torch.full((2, L, 512, 1024), float("nan"), dtype=torch.float16, device="cuda")
+    pool[:, :, 16:19] = 0.25                                   # request 1: three cached rows on page 1
+    kv = SimpleNamespace(view=abi.KvView(L, 512, 1024, *((C.c_void_p * L)(*(pool[i, l].data_ptr() for l in range(L))) for i in range(2))))
+    x = [rng.standard_normal((n, 1024)).astype(np.float32) for n in (5, 20)]
+    trees = [[-1, 0, 1, 1, 2], [j - 1 for j in range(20)]]
+    p = Pool(abi, talker, 2, {1: [1]})
+    p.past.copy_(i32([0, 3]))
+    p.free.copy_(i32([1]))                                       # one page: the first request's
+    h, l = p.step(trees, x, kv=kv, spare=3, spare_value=float("nan"), status=[0, 1])
+    assert torch.isnan(pool[:, :, 19:32]).all() and p.slot.tolist()[5:25] == [-1] * 20
+    alone_h, alone_l = Pool(abi, talker, 1, {}).step(trees[:1], x[:1], kv=abi.KvCache(L, 512, 1024))
+    assert np.abs(h[:5] - alone_h).max() < 1e-3 and np.abs(l[:5] - alone_l).max() < 1e-3
+
+
+def test_verify_of_the_most_rows(side):
+    """128 rows, the handle's most: two requests' chains of 64, each against the chain's rows one request at a time."""
+    abi, _, talker, _ = side
+    rng = np.random.default_rng(9)
+    x = [rng.standard_normal((64, 1024)).astype(np.float32) for _ in range(2)]
+    kv, chain = abi.KvCache(talker.kv.n_layer, 512, 1024), [j - 1 for j in range(64)]
+    h, l = Pool(abi, talker, 2, {}).step([chain, chain], x, kv=kv)
+    for i in range(2):
+        h1, l1 = Pool(abi, talker, 1, {}).step([chain], [x[i]], kv=kv)
+        assert np.abs(h[64 * i:64 * i + 64] - h1).max() < TOL_ABS and np.abs(l[64 * i:64 * i + 64] - l1).max() < TOL_ABS
 
 
 def test_verify_after_a_long_prefill_and_refusals(side):
