@@ -158,9 +158,10 @@ __device__ __forceinline__ int steps_of(const Args &a, const Where &w, int qrow0
     return (tiles + a.step - 1) / a.step;
 }
 __device__ __forceinline__ int chunk_steps(const Args &a, float total) {
-    // the steps in all, exact below 2^24; above (lengths out of all proportion) rounded up, so that the chunks stay as few
+    // the steps in all, exact below 2^24; above (lengths out of all proportion) rounded up, so that the chunks stay as few, and
+    // at most 2^30, more than a request has
     return max(total < 16777216.f ? (static_cast<int>(total) + a.workers - 1) / a.workers
-                                  : static_cast<int>(total * 1.001f / static_cast<float>(a.workers)) + 1, 1);
+                                  : static_cast<int>(min(total * 1.001f / static_cast<float>(a.workers), 1073741824.f)) + 1, 1);
 }
 __device__ __forceinline__ uint32_t chunks_of(int steps, int most) {
     const uint32_t n = static_cast<uint32_t>((steps + most - 1) / most);
