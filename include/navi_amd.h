@@ -339,7 +339,7 @@ navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *head
  * nothing gets zeros. Rows past cu_rows[n_requests] and past max_new of a request are left as they were.
  * max_keys: the most positions a request may reach (n_past + rows), by which the work is split; longer
  * requests are still right, but slow. n_requests * n_head < 2^23. d_ws: navi_tree_workspace(...) bytes, 16-byte aligned, for this call
- * alone until it is done: calls that may overlap need a workspace each. Alignment as navi_kv_append. */
+ * alone until it is done: calls that may overlap need a workspace each. d_out may be d_q with the same stride. Alignment as navi_kv_append. */
 navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads *heads, const void *d_q, int32_t q_dtype, int32_t ldq,
                                 const void *d_k, const void *d_v, int32_t ld_kv, float scale, int32_t max_keys, void *d_out,
                                 int32_t ldo, void *d_ws, size_t ws_bytes, void *stream, char *err, size_t errlen);

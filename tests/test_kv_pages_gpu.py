@@ -627,6 +627,48 @@ def test_on_another_stream_and_the_library_stream():
         want = got
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_over_its_own_queries(kind):
+    """d_out = d_q: one row, groups of many, cut and uncut."""
+    rng = np.random.default_rng(3)
+    for reqs in ([(70, [-1])], [(40, random_tree(rng, 24)), (3, [-1])], [(2500, random_tree(rng, 9))], [(1800, random_tree(rng, 64)), (9, [-1, 0])]):
+        s = Step(reqs, kind=kind, spare_rows=1).fill()
+        want = s.check()
+        s.device()
+        q = torch.full((s.n_rows, s.heads * s.dim), 7.0, dtype=s.q.dtype)
+        q[:s.rows] = s.q
+        q = q.cuda()
+        size = abi.tree_workspace(s.pages(), s.layout(), s.max_keys)
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        abi.tree_attention(s.pages(), s.layout(), q.data_ptr(), TYPE[kind][1], q.shape[1], s.d_k.data_ptr(), s.d_v.data_ptr(), s.ld, s.dim ** -0.5, s.max_keys,
+                           q.data_ptr(), q.shape[1], ws.data_ptr(), size, stream=stream())
+        torch.cuda.synchronize()
+        assert torch.equal(q.cpu(), want)
+
+
+def test_two_streams_at_once():
+    """Two servers' steps on a stream each, enqueued in turn without a wait, workspaces and scratch their own."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    servers = [Server(seed=i) for i in (11, 12)]
+    alone = [Server(seed=i) for i in (11, 12)]
+    for s in (*servers, *alone):
+        seeded(s, 5, [60] * s.n)
+    torch.cuda.synchronize()
+    for s in alone:
+        s.plan(streams[0].cuda_stream)
+        for _ in range(6):
+            s.layer(streams[0].cuda_stream)
+        s.commit(streams[0].cuda_stream)
+        torch.cuda.synchronize()
+    for part in ("plan", *["layer"] * 6, "commit"):
+        for s, st in zip(servers, streams):
+            getattr(s, part)(st.cuda_stream)
+    torch.cuda.synchronize()
+    for a, b in zip(servers, alone):
+        for name in ("out", "k", "v", "table", "held", "free", "slot", "pos", "mask", "cu", "new_past"):
+            assert torch.equal(torch.nan_to_num(getattr(a, name).float()), torch.nan_to_num(getattr(b, name).float())), name
+
+
 def test_graphs_replayed_between_eager_work():
     """Two captured graphs (a workspace each) replayed in turn, with eager steps and synchronizations between the replays."""
     eager, a, b = Server(seed=4), Server(seed=4), Server(seed=4)
