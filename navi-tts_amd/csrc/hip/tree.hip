@@ -16,7 +16,7 @@
 //    spread over all banks.
 //  * Up to 32 query rows (k_tree) a wave works alone on its own 32-key tiles, every W-th of the block's range, with K from
 //    memory in operand form, its own V buffer and no barrier until its range ends; then the waves' results are joined in
-//    LDS. 32 requests with one row each over 1024 keys take 26.6 us, 5.07 TB/s: the cache's bytes at the rate of a large
+//    LDS. 32 requests with one row each over 1024 keys take 25.7 us, 5.24 TB/s: the cache's bytes at the rate of a large
 //    read (5.6 TB/s here) are 24.
 //  * Above (k_tree_rows) two or four waves with 32 rows each share the K and V tiles, which go through LDS in two buffers with
 //    one barrier a tile. 64 requests x 24 rows (48 query rows) over 8192 keys 415 us, 5.2 TB/s; without the products 385.
@@ -25,7 +25,7 @@
 //  * Softmax against a reference value that moves only when a score passes it by more than SLACK: the
 //    rescaling, and the maximum over lanes that it needs, are off the common path. exp2 with the scale folded in.
 //  * Requests are cut into even chunks over the blocks, however uneven their lengths (lay_out): 64 requests of lengths spread from
-//    1 to 8000 72 us, uncut 151. A second kernel joins the chunks' results (unnormalised sums, reference, sum) in their order.
+//    1 to 8000 70 us, uncut 143. A second kernel joins the chunks' results (unnormalised sums, reference, sum) in their order.
 #include "dev_common.h"
 #include "tile_layout.h"
 #include "tree.h"
@@ -40,8 +40,8 @@ using kv::Div;
 using kv::div_by;
 
 constexpr int NW = 4, BT = NW * WAVE;  // waves of a block of k_tree_join
-// Of k_tree: eight, more loads on their way, where a block has a whole request (32 requests of 1024 keys: 26.6 us, with four
-// 31.0); four, and twice as many blocks, where requests are cut (64 ragged ones of up to 8000 keys: 72 us, with eight 85).
+// Of k_tree: eight, more loads on their way, where a block has a whole request (32 requests of 1024 keys: 25.7 us, with four
+// 27.0); four, and twice as many blocks, where requests are cut (64 ragged ones of up to 8000 keys: 70 us, with eight 86).
 constexpr int alone_of(bool cut) { return cut ? 4 : 8; }
 // Of k_tree_rows, RW waves of which share their query rows' tiles: eight, one block a CU, so that half as many parts of
 // a cut request are stored and joined (64 drafted rows over 32768 keys: 57 us, with four 64); four where two waves share and
@@ -285,23 +285,32 @@ struct Rows {
     float ref[NT], sub[NT], sum[NT], fac[NT];
     uint64_t seen[NT];
 
-    // Query row m of the request's (m < 0: none): its operands, a pair's hi before its lo, and the factor of its scores.
-    static __device__ __forceinline__ float operands(const Args &a, const Share &s, int m, v8 (&q)[QP * KS]) {
-        const int lg = (threadIdx.x & 63) >> 4, j = div_by(a.heads_per, max(m, 0));
-        const bool on = m >= 0 && j < s.at.rows;
+    // Query row m of the request's as it stands in memory (past its rows: zeros), loaded; then its operands, a pair's hi
+    // before its lo, and the factor of its scores.
+    struct Raw {
+        u32x4_t x[QP * KS];
+    };
+    static __device__ __forceinline__ void fetch(const Args &a, const Share &s, int m, Raw &r) {
+        const int lg = (threadIdx.x & 63) >> 4, j = div_by(a.heads_per, m);
+        const bool on = j < s.at.rows;
         const size_t at = static_cast<size_t>(s.at.c0 + (on ? j : 0)) * a.ldq + static_cast<size_t>(s.kvh * a.g + (on ? m - j * a.g : 0)) * D + 8 * lg;
+        const unsigned char *p = static_cast<const unsigned char *>(a.q) + at * 2 * QP;
+#pragma unroll
+        for (int i = 0; i < QP * KS; ++i)
+            r.x[i] = on ? *(const NAVI_GLOBAL u32x4_t *) (p + 64 * QP * (i / QP) + 16 * (i % QP)) : u32x4_t{0u, 0u, 0u, 0u};
+    }
+    static __device__ __forceinline__ float operands(const Args &a, const Raw &r, v8 (&q)[QP * KS]) {
         float f = a.scale;
         if constexpr (PAIR) {
             // q times a power of two that puts the row's largest value into [1, 2): pairs keep 22 bits of it
             // whatever its range; the scores get the inverse
-            const float *p = static_cast<const float *>(a.q) + at;
             f32x4_t x[KS][2];
             float top = 0.f;
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    x[k][h] = on ? ld4(p + 32 * k + 4 * h) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+                    x[k][h] = bits<f32x4_t>(r.x[2 * k + h]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[k][h][e]));
                 }
@@ -317,10 +326,9 @@ struct Rows {
                     q[KS + k][e] = static_cast<E>(y - static_cast<float>(q[k][e]));
                 }
         } else {
-            const E *p = static_cast<const E *>(a.q) + at;
             const uint32_t sign = a.flip ? 0x80008000u : 0u;
 #pragma unroll
-            for (int k = 0; k < KS; ++k) q[k] = bits<v8>(on ? *(const NAVI_GLOBAL u32x4_t *) (p + 32 * k) ^ sign : u32x4_t{0u, 0u, 0u, 0u});
+            for (int k = 0; k < KS; ++k) q[k] = bits<v8>(r.x[k] ^ sign);
         }
         // a factor of 0 (all scores alike) as the least normal number: -inf, a place not seen, must stay -inf
         return fmaxf(f, 1.17549435e-38f);
@@ -502,11 +510,12 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
             slot[kt] = pg.slot_of(t * KT + kt * 16 + lr, page[kt]);
             const size_t at = static_cast<size_t>(max(slot[kt], 0)) * a.ldkv;
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                kr[kt][k] = *(const NAVI_GLOBAL u32x4_t *) (kb + at + 32 * k);
-                vr[kt][k] = *(const NAVI_GLOBAL u32x4_t *) (vb + at + 32 * k);
-            }
+            for (int k = 0; k < KS; ++k) kr[kt][k] = *(const NAVI_GLOBAL u32x4_t *) (kb + at + 32 * k);
         }
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int k = 0; k < KS; ++k) vr[kt][k] = *(const NAVI_GLOBAL u32x4_t *) (vb + static_cast<size_t>(max(slot[kt], 0)) * a.ldkv + 32 * k);
     };
     int t = s.t0 + wv;
     if constexpr (CUT) {
@@ -515,6 +524,9 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) page[kt] = t * KT + kt * 16 + lr < s.at.len ? ahead[kt] : -1;
     }
+    // q before K and V, which a wait for it would otherwise include (one row over 256 keys: 8.7 us, after them 10.2)
+    typename R::Raw raw;
+    if (wv < NT) R::fetch(a, s, qrow0 + wv * 16 + lr, raw);
     R rows;
     rows.start(a, s, qrow0);
     if (t < s.t_end) {
@@ -525,7 +537,7 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
     u32x4_t *s_q = reinterpret_cast<u32x4_t *>(sm + W * VB);
     if (wv < NT) {
         v8 q[QP * KS];
-        const float f = R::operands(a, s, qrow0 + wv * 16 + lr, q);
+        const float f = R::operands(a, raw, q);
 #pragma unroll
         for (int i = 0; i < QP * KS; ++i) s_q[((i / KS * NT + wv) * KS + i % KS) * WAVE + l] = bits<u32x4_t>(q[i]);
         if (lg == 0) s_fac[wv * 16 + lr] = f;
@@ -539,6 +551,32 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
         // keys of this tile that exist (uniform), and whether any row may not see one
         const uint32_t there =
             static_cast<uint32_t>(__ballot(slot[0] >= 0) & 0xFFFFu) | static_cast<uint32_t>(__ballot(slot[1] >= 0) & 0xFFFFu) << 16;
+        // scores, for which V need not have arrived (it is loaded after K: 32 requests of 1024 keys 26.6 us when V came to LDS first);
+        // the operands of a step are read while the step before is multiplied
+        f32x4_t sc[NT][2];
+        asm volatile("" ::: "memory");                            // or the operands would be kept in registers after all
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        v8 qb[2][QP * NT];
+        auto load_q = [&](int k) {
+#pragma unroll
+            for (int i = 0; i < QP * NT; ++i) qb[k & 1][i] = bits<v8>(s_q[(i * KS + k) * WAVE + l]);
+        };
+        load_q(0);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            if (k + 1 < KS) load_q(k + 1);
+#pragma unroll
+            for (int i = 0; i < QP * NT; ++i)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) sc[i % NT][kt] = Types<E>::mfma(bits<v8>(kr[kt][k]), qb[k & 1][i], sc[i % NT][kt]);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, QP * NT, 0);          // LDS reads
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x100, QP * NT, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 2 * QP * NT, 0);  // MFMAs
+        }
         const bool masked = (t + 1) * KT > s.at.past || there != 0xFFFFFFFFu;
         uint32_t special = 0;                                     // drafted keys with an infinity or NaN in V
         if (masked) {
@@ -565,31 +603,6 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int k = 0; k < KS; ++k) *reinterpret_cast<u32x4_t *>(v_at<D>(buf, kt * 16 + lr, 2 * k + (lg >> 1), lg & 1)) = vr[kt][k];
-        // scores; the operands of a step are read while the step before is multiplied
-        f32x4_t sc[NT][2];
-        asm volatile("" ::: "memory");                            // or the operands would be kept in registers after all
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        v8 qb[2][QP * NT];
-        auto load_q = [&](int k) {
-#pragma unroll
-            for (int i = 0; i < QP * NT; ++i) qb[k & 1][i] = bits<v8>(s_q[(i * KS + k) * WAVE + l]);
-        };
-        load_q(0);
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            if (k + 1 < KS) load_q(k + 1);
-#pragma unroll
-            for (int i = 0; i < QP * NT; ++i)
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt) sc[i % NT][kt] = Types<E>::mfma(bits<v8>(kr[kt][k]), qb[k & 1][i], sc[i % NT][kt]);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x100, QP * NT, 0);          // LDS reads
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            __builtin_amdgcn_sched_group_barrier(0x100, QP * NT, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 2 * QP * NT, 0);  // MFMAs
-        }
         // the next tile's rows, in flight from here
         if (t + W < s.t_end) {
             load(t + W);
@@ -725,7 +738,9 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         v8 x[QP * KS];
-        rows.fac[nt] = R::operands(a, s, qrow0 + nt * 16 + lr, x);
+        typename R::Raw raw;
+        R::fetch(a, s, qrow0 + nt * 16 + lr, raw);
+        rows.fac[nt] = R::operands(a, raw, x);
 #pragma unroll
         for (int i = 0; i < QP * KS; ++i)
             if (i < KS) q[nt][i] = x[i];
@@ -889,10 +904,10 @@ Cut cut_of(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys, bool pa
     const int waves = c.waves == 1 ? alone_of(true) : waves_of(pair, c.waves);
     c.step = waves / c.waves;                           // tiles of a block's turn
     const int steps = (max_keys + KT * c.step - 1) / (KT * c.step);
-    // A block a request where no request can be long enough to share (one row of 16 heads over 256 keys: 9.3 us, cut 10.6; over
-    // 512: 12.4 and 10.6); where there are blocks for all CUs and no request is so long that an uneven one would cost more than
-    // the chunks and the join (one row of 32 requests, all alike and of lengths spread down to one: of 1000 keys 26.4 and 20.7 us,
-    // cut 30.7 and 14.8; of 1400 39.7 and 26.2, cut 45.6 and 19.4; of 2000 56.5 and 35.8, cut 61.8 and 23.6); and for more
+    // A block a request where no request can be long enough to share (one row of 16 heads over 256 keys: 8.3 us, cut 10.5; over
+    // 512: 11.6 and 10.4); where there are blocks for all CUs and no request is so long that an uneven one would cost more than
+    // the chunks and the join (one row of 32 requests, all alike and of lengths spread down to one: of 1000 keys 25.7 and 19.5 us,
+    // cut 30.5 and 14.5; of 1400 38.6 and 24.7, cut 45.4 and 19.4; of 2000 54.2 and 33.9, cut 59.2 and 22.6); and for more
     // requests than a block lays out. Else enough blocks for all waves of the CUs.
     if (p.n_requests > MAXB || steps == 1 || (c.waves == 1 && max_keys <= 384) || (max_keys <= 1280 && p.n_requests * heads >= 256)) {
         c.workers = c.parts = 0;
