@@ -5,7 +5,6 @@ A step of a server: every request has `n_past` rows in a pool of pages and takes
 token) or a tree of drafted tokens. The head layouts are the talker's (16 / 8 heads x 128), the codec transformer's
 (16 / 16 x 64) and common grouped ones. Lengths follow from the case; values, page orders and trees from the seed.
 """
-import functools
 import math
 import random
 import sys
@@ -207,7 +206,6 @@ def run(s):
         return {"plan": _plan, "append": _append, "attention": _attention, "commit": _commit}[op](s)
 
 
-@functools.cache
 def _abi():
     at = str(Path(__file__).resolve().parent.parent / "navi-tts_amd")
     if at not in sys.path:
