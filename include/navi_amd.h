@@ -334,7 +334,8 @@ navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *head
  * to the step's rows a of its request with bit a of row_mask[r], at positions n_past[i] + a (the step's K and V are in
  * the pages): out = softmax(scale q . K) V per head, heads grouped n_head / n_kv_head to a kv head. max_new <= 64; one
  * row a request is ordinary single-token decode. d_q and d_out have one type: the pool's, or f32 over an f16
- * pool (q and the probabilities then travel as f16 hi + lo pairs). What a row does not see has no influence,
+ * pool (q then travels as f16 hi + lo pairs; the probabilities travel as pairs of the pool's type whatever q's, so that a
+ * result is off by its own rounding, not by theirs). What a row does not see has no influence,
  * infinities and NaN included; a position whose page is outside the pool is not seen; a row that sees
  * nothing gets zeros. Rows past cu_rows[n_requests] and past max_new of a request are left as they were.
  * max_keys: the most positions a request may reach (n_past + rows), by which the work is split; longer
