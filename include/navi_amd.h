@@ -287,6 +287,7 @@ typedef struct {                       /* a step's requests and rows on a pool o
     int32_t *row_slot;                 /* [n_rows]: the row's slot in the pool, -1 none */
     int32_t *row_pos;                  /* [n_rows]: the row's position: n_past + its depth in the tree */
     uint64_t *row_mask;                /* [n_rows]: bit a: the row sees row a of its request's step */
+    const int32_t *status;             /* [n_requests]: the step's d_status of navi_kv_plan, for navi_kv_commit; NULL: not given */
 } navi_kv_pages;
 
 typedef struct {
@@ -349,9 +350,12 @@ size_t navi_tree_workspace(const navi_kv_pages *pages, const navi_kv_heads *head
 /* The accepted rows of each request moved into place in every layer of `kv` (n_layer, max_pos >= the pool's rows, kv_dim the
  * row stride, a multiple of 8): with path = d_path[i][0 .. d_accept[i] - 1] (stride max_path <= 64), the indexes of accepted rows within
  * the request's step in ascending order, position n_past[i] + j takes the K and V of position n_past[i] + path[j].
- * d_n_past_out[i] = n_past[i] + d_accept[i]. d_n_past_out and d_status are none of the call's inputs. d_status[i]: 0, or 2 where d_accept[i] is outside
- * 0 .. max_path, the path does not ascend or leaves the request's rows, or a page is outside the pool: nothing is moved and
- * d_n_past_out[i] = n_past[i]. Pages past the new length stay with the request. */
+ * d_n_past_out[i] = n_past[i] + d_accept[i]. d_n_past_out and d_status are none of the call's inputs. d_status[i]: 0, or 2 where
+ * d_accept[i] is outside 0 .. max_path, the path does not ascend or leaves the request's rows, a page of these, or of the request's
+ * last row, is outside the pool (the plan had none left), or the request has more than max_new rows: nothing is moved and
+ * d_n_past_out[i] = n_past[i]. With pages->status also where the plan refused the request, or an accepted row has no slot: its K
+ * and V are not in the pages, whatever these hold. Without it a path over rows that the plan refused for their lengths or parents
+ * (status 2 or 3) is taken at its word. That a path follows the tree is not checked. Pages past the new length stay with the request. */
 navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, const int32_t *d_path, int32_t max_path,
                            const int32_t *d_accept, int32_t *d_n_past_out, int32_t *d_status, void *stream, char *err,
                            size_t errlen);

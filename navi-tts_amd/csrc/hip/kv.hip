@@ -397,9 +397,9 @@ void launch_append_types(const AppendArgs &a, bool xf, bool qf, int D, hipStream
 constexpr int CL = 32;                 // layers a launch
 struct CommitArgs {
     void *k[CL], *v[CL];
-    const int32_t *table, *n_past, *cu, *path, *accept;
+    const int32_t *table, *n_past, *cu, *path, *accept, *planned, *slot;   // planned: the plan's status, or null
     int32_t *past_out, *status;
-    int max_path, blocks, n_pages, ld, write;   // write: this launch stores the results
+    int max_path, max_new, blocks, n_pages, n_rows, ld, write;   // write: this launch stores the results
     Div page;
 };
 
@@ -412,7 +412,8 @@ __global__ void __launch_bounds__(CT) k_commit(CommitArgs a) {
     __shared__ int src[WAVE], dst[WAVE];
     __shared__ int s_n;
     const int i = blockIdx.y, l = threadIdx.x;
-    const int past = gld(a.n_past + i), count = gld(a.cu + i + 1) - gld(a.cu + i), n = gld(a.accept + i);
+    const int past = gld(a.n_past + i), c0 = gld(a.cu + i), count = gld(a.cu + i + 1) - c0, n = gld(a.accept + i);
+    const int refused = a.planned ? gld(a.planned + i) : 0;
     if (l < WAVE) {
         bool bad = n < 0 || n > a.max_path || past < 0;
         int p = -1;
@@ -425,8 +426,11 @@ __global__ void __launch_bounds__(CT) k_commit(CommitArgs a) {
             return static_cast<unsigned>(g) < static_cast<unsigned>(a.n_pages)
                        ? g * static_cast<int>(a.page.d) + static_cast<int>(at) - b * static_cast<int>(a.page.d) : -1;
         };
+        // rows that a plan refused were never appended: the request's last row has no page, or its status says so
+        const int last = past >= 0 && count > 0 ? slot_of(count - 1) : -1;
         if (!bad && l < n) {
-            bad = p < 0 || p >= count || (l > 0 && p <= prev);
+            bad = p < 0 || p >= count || (l > 0 && p <= prev) || count > a.max_new || last < 0 || refused != 0;
+            if (!bad && a.planned) bad = c0 < 0 || p >= a.n_rows - c0 || gld(a.slot + c0 + p) < 0;
             if (!bad) {
                 src[l] = slot_of(p);
                 dst[l] = slot_of(l);
@@ -559,7 +563,8 @@ navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, c
             set_err(err, errlen, "kv_commit: layer %d's cache is null or not 16-byte aligned", l);
             return NAVI_ERR_INVALID;
         }
-    for (const int32_t *in : {pages->n_past, static_cast<const int32_t *>(pages->cu_rows), static_cast<const int32_t *>(pages->block_table), d_path, d_accept})
+    for (const int32_t *in : {pages->n_past, static_cast<const int32_t *>(pages->cu_rows), static_cast<const int32_t *>(pages->block_table),
+                              static_cast<const int32_t *>(pages->row_slot), pages->status, d_path, d_accept})
         if (d_n_past_out == in || d_status == in || d_status == d_n_past_out) {
             set_err(err, errlen, "kv_commit: d_n_past_out and d_status are one array, or one of the inputs, which other blocks still read");
             return NAVI_ERR_INVALID;
@@ -578,6 +583,10 @@ navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, c
         a.cu = pages->cu_rows;
         a.path = d_path;
         a.accept = d_accept;
+        a.planned = pages->status;
+        a.slot = pages->row_slot;
+        a.max_new = pages->max_new;
+        a.n_rows = pages->n_rows;
         a.past_out = d_n_past_out;
         a.status = d_status;
         a.max_path = max_path;

@@ -92,7 +92,8 @@ class KvPages(C.Structure):
     """navi_kv_pages: a step's requests and rows on a pool of cache pages (device addresses)."""
     _fields_ = [("n_requests", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32), ("max_blocks", C.c_int32),
                 ("n_rows", C.c_int32), ("max_new", C.c_int32), ("block_table", C.c_void_p), ("n_past", C.c_void_p),
-                ("cu_rows", C.c_void_p), ("row_slot", C.c_void_p), ("row_pos", C.c_void_p), ("row_mask", C.c_void_p)]
+                ("cu_rows", C.c_void_p), ("row_slot", C.c_void_p), ("row_pos", C.c_void_p), ("row_mask", C.c_void_p),
+                ("status", C.c_void_p)]                       # the plan's, for kv_commit (None: not given)
 
 
 class KvHeads(C.Structure):

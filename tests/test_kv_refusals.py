@@ -155,3 +155,12 @@ def test_struct_layouts_match_the_header(tmp_path):
     got = subprocess.run([str(tmp_path / "l")], capture_output=True, text=True, check=True).stdout.splitlines()
     for line, py in zip(got, (abi.KvPages, abi.KvHeads)):
         assert [int(x) for x in line.split()] == [C.sizeof(py)] + [getattr(py, f[0]).offset for f in py._fields_]
+
+
+@pytest.mark.parametrize("name", ["n_past", "status"])
+@pytest.mark.parametrize("field", ["status", "row_slot"])
+def test_commit_refuses_results_over_the_plans(name, field):
+    at = dict(n_past=P + 320, status=P + 384)
+    p = pages(block_table=P + 64, n_past=P + 128, cu_rows=P + 192, row_slot=P + 256, status=P + 448)
+    setattr(p, field, at[name])
+    assert "inputs" in refused(4, abi.kv_commit, p, [P], [P + (1 << 20)], 1024, P, 4, P + 16, at["n_past"], at["status"])
