@@ -348,7 +348,8 @@ navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads 
 /* Workspace bytes of navi_tree_attention (host only; 0 when the work is not split, or the arguments are not valid). */
 size_t navi_tree_workspace(const navi_kv_pages *pages, const navi_kv_heads *heads, int32_t max_keys);
 /* The accepted rows of each request moved into place in every layer of `kv` (n_layer, max_pos >= the pool's rows, kv_dim the
- * row stride, a multiple of 8): with path = d_path[i][0 .. d_accept[i] - 1] (stride max_path <= 64), the indexes of accepted rows within
+ * row stride, a multiple of 8; whole strides are moved, so that the layers' K and V must not overlap as n_pages * page_size rows of kv_dim: K
+ * and V interleaved in one allocation are refused; an array named more than once is moved once): with path = d_path[i][0 .. d_accept[i] - 1] (stride max_path <= 64), the indexes of accepted rows within
  * the request's step in ascending order, position n_past[i] + j takes the K and V of position n_past[i] + path[j].
  * d_n_past_out[i] = n_past[i] + d_accept[i]. d_n_past_out and d_status are none of the call's inputs. d_status[i]: 0, or 2 where
  * d_accept[i] is outside 0 .. max_path, the path does not ascend or leaves the request's rows, a page of these, or of the request's

@@ -5,6 +5,8 @@
 #include "kv.h"
 
 #include <algorithm>
+#include <memory>
+#include <new>
 
 namespace navi_amd {
 namespace kv {
@@ -394,16 +396,16 @@ void launch_append_types(const AppendArgs &a, bool xf, bool qf, int D, hipStream
 
 // ---- commit ----------------------------------------------------------------------------------
 
-constexpr int CL = 32;                 // layers a launch
+constexpr int CL = 64;                 // arrays (a layer's K or V) a launch
 struct CommitArgs {
-    void *k[CL], *v[CL];
+    void *base[CL];
     const int32_t *table, *n_past, *cu, *path, *accept, *planned, *slot;   // planned: the plan's status, or null
     int32_t *past_out, *status;
     int max_path, max_new, blocks, n_pages, n_rows, ld, write;   // write: this launch stores the results
     Div page;
 };
 
-// Block (columns, request, layer and K or V): each thread moves 16 bytes of a row for the whole path, in order. A
+// Block (columns, request, array): each thread moves 16 bytes of a row for the whole path, in order. A
 // path ascends, so its j-th source lies at or above position j: a row is read before, or when, it
 // is written, and batches of eight that read before they write keep that. 32 requests' paths of 8 rows in 28 layers (44 MB)
 // take 10.4 us, 4.25 TB/s; one request's 3.7 us, three rounds of memory latency.
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(CT) k_commit(CommitArgs a) {
     __syncthreads();
     const int m = s_n, col = (blockIdx.x * CT + l) * 8;
     if (col >= a.ld) return;
-    uint16_t *base = static_cast<uint16_t *>(blockIdx.z & 1 ? a.v[blockIdx.z >> 1] : a.k[blockIdx.z >> 1]) + col;
+    uint16_t *base = static_cast<uint16_t *>(a.base[blockIdx.z]) + col;
     for (int j0 = 0; j0 < m; j0 += 8) {
         u32x4_t t[8];
 #pragma unroll
@@ -569,15 +571,30 @@ navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, c
             set_err(err, errlen, "kv_commit: d_n_past_out and d_status are one array, or one of the inputs, which other blocks still read");
             return NAVI_ERR_INVALID;
         }
+    // the arrays by address, each once; none may begin inside the one before
+    const std::unique_ptr<uintptr_t[]> at(new (std::nothrow) uintptr_t[2 * static_cast<size_t>(kv->n_layer)]);
+    if (!at) {
+        set_err(err, errlen, "kv_commit: out of host memory");
+        return NAVI_ERR_INVALID;
+    }
+    for (int l = 0; l < kv->n_layer; ++l) {
+        at[2 * l] = reinterpret_cast<uintptr_t>(kv->k[l]);
+        at[2 * l + 1] = reinterpret_cast<uintptr_t>(kv->v[l]);
+    }
+    std::sort(at.get(), at.get() + 2 * static_cast<size_t>(kv->n_layer));
+    const int arrays = static_cast<int>(std::unique(at.get(), at.get() + 2 * static_cast<size_t>(kv->n_layer)) - at.get());
+    const uint64_t bytes = static_cast<uint64_t>(pages->n_pages) * pages->page_size * 2 * kv->kv_dim;
+    for (int i = 0; i + 1 < arrays; ++i)
+        if (at[i + 1] - at[i] < bytes) {
+            set_err(err, errlen, "kv_commit: the cache's arrays overlap (%d rows of %d elements)", pages->n_pages * pages->page_size, kv->kv_dim);
+            return NAVI_ERR_INVALID;
+        }
     OnDevice dev;
     if ((st = dev.enter(stream, "kv_commit", err, errlen)) != NAVI_OK) return st;
-    for (int l0 = 0; l0 < kv->n_layer; l0 += CL) {
-        const int n = std::min(CL, kv->n_layer - l0);
+    for (int l0 = 0; l0 < arrays; l0 += CL) {
+        const int n = std::min(CL, arrays - l0);
         CommitArgs a{};
-        for (int l = 0; l < n; ++l) {
-            a.k[l] = kv->k[l0 + l];
-            a.v[l] = kv->v[l0 + l];
-        }
+        for (int l = 0; l < n; ++l) a.base[l] = reinterpret_cast<void *>(at[l0 + l]);
         a.table = pages->block_table;
         a.n_past = pages->n_past;
         a.cu = pages->cu_rows;
@@ -595,7 +612,7 @@ navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, c
         a.ld = kv->kv_dim;
         a.write = l0 == 0;
         a.page = make_div(static_cast<uint32_t>(pages->page_size));
-        hipLaunchKernelGGL(k_commit, dim3((kv->kv_dim / 8 + CT - 1) / CT, pages->n_requests, 2 * n), dim3(CT), 0,
+        hipLaunchKernelGGL(k_commit, dim3((kv->kv_dim / 8 + CT - 1) / CT, pages->n_requests, n), dim3(CT), 0,
                            static_cast<hipStream_t>(stream), a);
     }
     NAVI_TRY_HIP(hipGetLastError(), err, errlen);

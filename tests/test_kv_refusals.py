@@ -164,3 +164,13 @@ def test_commit_refuses_results_over_the_plans(name, field):
     p = pages(block_table=P + 64, n_past=P + 128, cu_rows=P + 192, row_slot=P + 256, status=P + 448)
     setattr(p, field, at[name])
     assert "inputs" in refused(4, abi.kv_commit, p, [P], [P + (1 << 20)], 1024, P, 4, P + 16, at["n_past"], at["status"])
+
+
+ROWS = 8 * 16 * 1024 * 2                        # bytes of a layer's K or V in the pool of pages()
+
+
+@pytest.mark.parametrize("k,v", [([P], [P + 256]), ([P], [P + ROWS - 16]), ([P + ROWS // 2], [P]), ([P, P + 512], [P + 2 * ROWS, P + 3 * ROWS]),
+                                 ([P, P + 3 * ROWS], [P + ROWS, P + 2 * ROWS + 16])], ids=str)
+def test_commit_refuses_rows_of_one_array_inside_another(k, v):
+    """Rows are moved whole: K and V interleaved in one allocation (V's base inside K's row) would move into each other, and past its end."""
+    assert "overlap" in refused(4, abi.kv_commit, pages(), k, v, 1024, P, 4, P, P + 64, P + 128)

@@ -101,3 +101,17 @@ def test_a_row_without_a_slot_is_not_committed():
     check(s, [[0, 1], [0, 4]], [True, False], True)
     check(s, [[0, 1], [0, 5]], [True, True], True)
     check(s, [[0, 1], [0, 4]], [True, True], False)
+
+
+def test_an_array_named_more_than_once_is_moved_once():
+    """K and V one array, and layers that share theirs: a second move would start from rows that the first has moved."""
+    s = Planned([(3, [j - 1 for j in range(12)]), (20, [-1])])
+    size, want = s.pool[0, 0].numel() * 2, s.pool.cpu()
+    a, b = (s.pool.data_ptr() + i * size for i in (0, 3))
+    path, acc, past, done = i32([list(range(1, 12)) + [0] * 5, [0] * 16]), i32([11, 0]), i32([0, 0]), i32([-9, -9])
+    abi.kv_commit(s.pages, [a, b, a], [a, b, b], WIDTH, path.data_ptr(), 16, acc.data_ptr(), past.data_ptr(), done.data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    at = s.slots(0, 12)
+    for i in ((0, 0), (1, 1)):
+        want[i][at[:11]] = want[i][at[1:]].clone()
+    assert torch.equal(s.pool.cpu(), want) and past.tolist() == [14, 20] and done.tolist() == [0, 0]
