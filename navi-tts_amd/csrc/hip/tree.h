@@ -16,7 +16,7 @@ struct Call {
     int q_dtype, ldq, ldkv, ldo, max_keys;
     float scale;
     bool tiled;                        // f32 out in the tile layout of rows.h (ldo unused)
-    bool slots;                        // rows without a slot (a request that the plan refused) see no row of the step
+    bool slots;                        // rows without a slot (a request that the plan refused) see nothing; their output is zeros, or left as it was
 };
 size_t workspace(const navi_kv_pages &pages, const navi_kv_heads &heads, int max_keys);
 void launch(const Call &c, hipStream_t s);   // arguments already checked

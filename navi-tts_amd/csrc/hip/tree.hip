@@ -59,7 +59,7 @@ struct Args {
     void *out;
     float *po, *pm;                    // the parts of requests that are cut (part_of)
     uint32_t *first;                   // and each group's chunks before every request [groups][n + 1]
-    const int32_t *table, *n_past, *cu, *slot;   // slot: null, or rows with slot < 0 see no row of the step
+    const int32_t *table, *n_past, *cu, *slot;   // slot: null, or rows with slot < 0 see nothing
     const uint64_t *mask;
     int n, hkv, g, blocks, n_pages, n_rows, max_new, ldq, ldkv, ldo, workers, groups, step, parts;
     int tiled;                         // f32 out: in the tile layout of rows.h, heads * D wide
@@ -135,10 +135,12 @@ __device__ __forceinline__ Where where_is(const Args &a, int req) {
     const int64_t room = min(static_cast<int64_t>(a.blocks) * a.page.d, static_cast<int64_t>(INT32_MAX - 4 * KT * NW));
     Where w;
     w.c0 = max(gld(a.cu + req), 0);
-    const int count = max(min(gld(a.cu + req + 1), a.n_rows) - w.c0, 0);
+    const int count = max(min(gld(a.cu + req + 1), a.n_rows) - w.c0, 0), past = gld(a.n_past + req);
     w.rows = min(count, a.max_new);
-    w.past = static_cast<int>(min<int64_t>(max(gld(a.n_past + req), 0), room));
+    w.past = static_cast<int>(min<int64_t>(max(past, 0), room));
     w.len = static_cast<int>(min<int64_t>(static_cast<int64_t>(w.past) + count, room));
+    // lengths that a plan refuses: no row of it has a slot
+    if (a.slot && (past < 0 || count > a.max_new || static_cast<int64_t>(past) + count > room)) w.rows = w.len = 0;
     return w;
 }
 
@@ -285,6 +287,7 @@ struct Rows {
     f32x4_t acc[NT][DT];
     float ref[NT], sub[NT], sum[NT], fac[NT];
     uint64_t seen[NT];
+    uint32_t off[NT];                  // bit r: row r of the tile has no slot (the same in all lanes)
 
     // Query row m of the request's as it stands in memory (past its rows: zeros), loaded; then its operands, a pair's hi
     // before its lo, and the factor of its scores.
@@ -340,7 +343,8 @@ struct Rows {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int j = div_by(a.heads_per, qrow0 + nt * 16 + lr);
-            seen[nt] = j < s.at.rows && (!a.slot || gld(a.slot + s.at.c0 + j) >= 0) ? gld(a.mask + s.at.c0 + j) : 0;
+            seen[nt] = j < s.at.rows ? gld(a.mask + s.at.c0 + j) : 0;
+            off[nt] = a.slot ? static_cast<uint32_t>(__ballot(j < s.at.rows && gld(a.slot + s.at.c0 + j) < 0)) & 0xFFFFu : 0u;
             ref[nt] = NONE;
             sub[nt] = sum[nt] = 0.f;
 #pragma unroll
@@ -454,6 +458,22 @@ struct Rows {
                 }
             }
         }
+    }
+
+    // Rows without a slot, whatever the cache held for them (infinities and NaN included): as rows that see nothing.
+    __device__ __forceinline__ void drop() {
+        const int lr = threadIdx.x & 15;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            if (off[nt]) {
+                const bool no = off[nt] >> lr & 1u;
+                ref[nt] = no ? NONE : ref[nt];
+                sum[nt] = no ? 0.f : sum[nt];
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[nt][d][e] = no ? 0.f : acc[nt][d][e];
+            }
     }
 
     // Row r of the group, columns col ..: stored, or kept as the chunk's part.
@@ -617,6 +637,7 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
         if (special) rows.add_special(sc, special, t, s, pg);
     }
 
+    rows.drop();
     // join the waves: reference = the greatest, sums and rows scaled to it
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -796,6 +817,7 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
         if (special) rows.add_special(sc, special, t, s, pg);
     }
 
+    rows.drop();
     // join the teams' results through LDS: reference = the greatest, sums and rows scaled to it; the first team adds and stores
     float *js = reinterpret_cast<float *>(sm);
 #pragma unroll

@@ -222,3 +222,30 @@ def test_verify_after_a_long_prefill_and_refusals(side):
     with pytest.raises(abi.NaviError) as e:
         pool.step([[-1]], [x])
     assert e.value.status == 4 and "f16 range" in str(e.value)
+
+
+def nan_pool(abi, L, rows, kept=()):
+    """A caller's pool whose rows are NaN but `kept` (rows of K and V that are 0.25), and its view."""
+    pool = torch.full((2, L, rows, 1024), float("nan"), dtype=torch.float16, device="cuda")
+    for r in kept:
+        pool[:, :, r] = 0.25
+    return pool, SimpleNamespace(view=abi.KvView(L, rows, 1024, *((C.c_void_p * L)(*(pool[i, l].data_ptr() for l in range(L))) for i in range(2))))
+
+
+@pytest.mark.parametrize("past,tree,status", [(10000, [-1, 0, 1], 2), (2 ** 31 - 5, [-1, 0, 1], 2), (-5, [-1, 0], 2), (190, [-1, 0, 1], 2), (3, [-1, 0, 2, 1], 3),
+                                              (3, [j - 1 for j in range(20)], 1)])
+def test_no_refused_request_can_fail_the_call(side, past, tree, status):
+    """Whatever a request holds that the plan refused (lengths out of range, bad parents, no pages): NaN in its held pages, cached
+    positions included, stays its own, and another request's results are those it has alone."""
+    abi, _, talker, _ = side
+    L, rng = talker.kv.n_layer, np.random.default_rng(12)
+    _, kv = nan_pool(abi, L, 512)
+    x = [rng.standard_normal((n, 1024)).astype(np.float32) for n in (5, len(tree))]
+    trees = [[-1, 0, 1, 1, 2], tree]
+    p = Pool(abi, talker, 2, {1: [1]})
+    p.past.copy_(i32([0, past]))
+    p.free.copy_(i32([1]))
+    h, l = p.step(trees, x, kv=kv, status=[0, status])
+    alone_h, alone_l = Pool(abi, talker, 1, {}).step(trees[:1], x[:1], kv=abi.KvCache(L, 512, 1024))
+    assert np.abs(h[:5] - alone_h).max() < 1e-3 and np.abs(l[:5] - alone_l).max() < 1e-3
+    assert np.isfinite(h).all() and np.isfinite(l).all()
