@@ -366,9 +366,10 @@ navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, c
  * every row's post-norm hidden in d_hidden f32 [n_rows][hidden] and its logits in d_logits f32 [n_rows][vocab]
  * (NULL: not computed). kv: the pool (n_layer, kv_dim and at least n_pages * page_size rows as navi_talker_kv's), or NULL: the
  * talker's own cache, whose max_positions rows are then the pages. n_rows <= max_prompt_tokens, max_new <= 64.
- * max_keys as in navi_tree_attention, at most max_positions; rows at positions past max_positions get no K and V. Rows of no
- * request, or of one that the plan refused, are taken as zeros, so that they do not fail the call; their results hold
- * nothing of use. Errors as navi_talker_prefill.
+ * max_keys as in navi_tree_attention, at most max_positions. A row at a position past max_positions gets no K and V, and its
+ * row_slot becomes -1, so that navi_kv_commit (with pages->status) takes no path over it. Rows without a slot (of a request that the
+ * plan refused too) and rows of no request are taken as zeros that see nothing, so that they do not fail the call; their
+ * results hold nothing of use. Errors as navi_talker_prefill.
  * Runs on the library stream (plan on it too) and is synchronous; navi_talker_last_ms is its device time. */
 navi_status navi_talker_verify(navi_talker *t, const navi_kv_view *kv, const navi_kv_pages *pages, int32_t max_keys, const float *d_rows,
                                float *d_hidden, float *d_logits, char *err, size_t errlen);

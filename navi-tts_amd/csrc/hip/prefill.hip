@@ -503,11 +503,17 @@ __global__ void __launch_bounds__(BT) k_tiled_rows_norm(const float *x, const fl
 }
 
 // Rows of a planned step that are no request's (past cu[n], or without a slot): zeros in the residual stream, and in the
-// attention's output, which is not written for all of them, so that nothing they hold reaches the f16-range check. Row = block,
-// of att up to the last tile's 16.
-__global__ void __launch_bounds__(BT) k_unowned(float *x, int T, int H, float *att, int QD, const int32_t *cu, int n, const int32_t *slot) {
+// attention's output, which is not written for all of them, so that nothing they hold reaches the f16-range check. A row at a
+// position outside 0 .. max_pos - 1, for which there is no rotation, loses its slot: its K and V are not stored, and the row itself
+// would read them. Row = block, of att up to the last tile's 16.
+__global__ void __launch_bounds__(BT) k_unowned(float *x, int T, int H, float *att, int QD, const int32_t *cu, int n, int32_t *slot, const int32_t *pos,
+                                                int max_pos) {
     const int r = blockIdx.x;
-    if (r < min(gld(cu + n), T) && gld(slot + r) >= 0) return;
+    if (r < min(gld(cu + n), T)) {
+        const bool in = static_cast<unsigned>(gld(pos + r)) < static_cast<unsigned>(max_pos);
+        if (in && gld(slot + r) >= 0) return;
+        if (!in && threadIdx.x == 0) gst(slot + r, -1);
+    }
     const f32x4_t zero{0.f, 0.f, 0.f, 0.f};
     if (r < T)
         for (int i = threadIdx.x * 4; i < H; i += BT * 4) st4(x + rows::pk_a(r, i, H), zero);
@@ -1103,7 +1109,7 @@ navi_status navi_talker_verify(navi_talker *t, const navi_kv_view *kv, const nav
     rows::tile_rows(d_rows, T, H, t->x, s, t->flag);
     t->flag_set = true;
     hipLaunchKernelGGL(k_unowned, dim3((T + 15) / 16 * 16), dim3(BT), 0, s, t->x, T, H, t->att, t->QD, pages->cu_rows, pages->n_requests,
-                       pages->row_slot);
+                       pages->row_slot, pages->row_pos, t->max_pos);
     for (int l = 0; l < t->L; ++l) {
         const LayerW &w = t->layers[l];
         bool ok = rows::launch_rows_pk(rows::EPI_PLAIN, true, t->x, T, H, w.ln1, t->eps, w.qkv_t, QKVW, t->part, QKVW, t->flag, s);

@@ -249,3 +249,45 @@ def test_no_refused_request_can_fail_the_call(side, past, tree, status):
     alone_h, alone_l = Pool(abi, talker, 1, {}).step(trees[:1], x[:1], kv=abi.KvCache(L, 512, 1024))
     assert np.abs(h[:5] - alone_h).max() < 1e-3 and np.abs(l[:5] - alone_l).max() < 1e-3
     assert np.isfinite(h).all() and np.isfinite(l).all()
+
+
+@pytest.mark.parametrize("past,inside", [(509, 3), (512, 0), (600, 0)])
+def test_a_request_that_runs_past_the_last_position(side, past, inside):
+    """Over a pool with more rows than the talker has positions (512), unwritten ones NaN: the rows past them get no K and V and no slot,
+    a commit takes no path over them, and the rows before them and the other request are what they are alone."""
+    abi, _, talker, _ = side
+    L, rng, rows = talker.kv.n_layer, np.random.default_rng(past), 1024
+    x = [rng.standard_normal((n, 1024)).astype(np.float32) for n in (5, 6)]
+    trees = [[-1, 0, 1, 1, 2], [j - 1 for j in range(6)]]
+    held = list(range(8, 8 + -(-past // PAGE)))
+
+    def step(trees, x):
+        pool, kv = nan_pool(abi, L, rows, [8 * PAGE + t for t in range(past)])
+        p = Pool(abi, talker, 2, {})
+        p.t = SimpleNamespace(params=talker.params, verify=lambda pages, keys, *a, **k: talker.verify(pages, 512, *a, **k))
+        p.n_pages, p.blocks = rows // PAGE, 48
+        p.table, p.held = i32([[-1] * 48, held + [-1] * (48 - len(held))]), i32([0, len(held)])
+        p.free, p.stack = i32([6]), i32(list(range(6)) + [0] * (p.n_pages - 6))
+        p.past.copy_(i32([0, past]))
+        h, l = p.step(trees, x, kv=kv)
+        return p, pool, kv, h, l
+
+    p, pool, kv, h, l = step(trees, x)
+    assert np.isfinite(h).all() and np.isfinite(l).all()
+    slot = p.slot.tolist()
+    assert all(s >= 0 for s in slot[:5 + inside]) and slot[5 + inside:] == [-1] * (6 - inside)
+    alone_h, alone_l = Pool(abi, talker, 1, {}).step(trees[:1], x[:1], kv=abi.KvCache(L, 512, 1024))
+    assert np.abs(h[:5] - alone_h).max() < 1e-3 and np.abs(l[:5] - alone_l).max() < 1e-3
+    if inside:
+        _, _, _, h1, l1 = step([[-1], trees[1][:inside]], [x[0][:1], x[1][:inside]])
+        assert np.abs(h[5:5 + inside] - h1[1:]).max() < 1e-3 and np.abs(l[5:5 + inside] - l1[1:]).max() < 1e-3
+    written = int(torch.isfinite(pool[0, 0, :, 0]).sum())
+    assert written == past + 5 + inside
+    p.pages.status = p.status.data_ptr()
+    for accept, done in ((inside, 0), (inside + 1, 2)):
+        path, acc, now, out = i32([list(range(8))] * 2), i32([1, accept]), i32([0, 0]), i32([9, 9])
+        torch.cuda.synchronize()
+        abi.kv_commit(p.pages, list(kv.view.k[:L]), list(kv.view.v[:L]), 1024, path.data_ptr(), 8, acc.data_ptr(), now.data_ptr(), out.data_ptr(),
+                      stream=abi.lib().navi_device_stream())
+        torch.cuda.synchronize()
+        assert out.tolist() == [0, done] and now.tolist() == [1, past + (accept if done == 0 else 0)]
