@@ -325,7 +325,8 @@ navi_status navi_kv_plan(const navi_kv_pages *pages, const int32_t *d_n_new, con
  * element i with element i + head_dim / 2; NULL: not turned). k and v are rounded to the pool's type and stored in
  * row row_slot[r] of d_k and d_v (stride ld_kv); q goes to row r of d_q (f32, or the pool's type; stride ldq). Rows
  * past cu_rows[n_requests] are left alone; a slot outside the pool stores no k and v; a position
- * outside 0 .. n_rot - 1 stores no k and v and a q of zeros. Strides in elements; strides and
+ * outside 0 .. n_rot - 1 stores no k and v and a q of zeros, and the row's row_slot becomes -1 (navi_kv_commit with pages->status
+ * takes no path over it). Strides in elements; strides and
  * pointers keep every row 16-byte aligned. d_q may be d_x with the same type and stride. */
 navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *heads, const void *d_x, int32_t x_dtype, int32_t ldx,
                            const float *d_q_norm, const float *d_k_norm, float eps, const float *d_rot, int32_t n_rot, void *d_k,

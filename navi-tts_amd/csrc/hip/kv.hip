@@ -296,7 +296,8 @@ struct AppendArgs {
     const void *x;
     const float *qn, *kn, *rot;
     void *k, *v, *q;
-    const int32_t *cu, *slot, *pos;
+    const int32_t *cu, *pos;
+    int32_t *slot;
     float eps;
     int n, n_rows, n_rot, slots, hq, hk, ldx, ldkv, ldq;
     Div heads;                         // by hq + 2 hk
@@ -336,6 +337,8 @@ __global__ void __launch_bounds__(256) k_append(AppendArgs a) {
     const int slot = gld(a.slot + r), pos = gld(a.pos + r);
     const bool in = !a.rot || static_cast<unsigned>(pos) < static_cast<unsigned>(a.n_rot);
     const bool isq = h < a.hq;
+    // a row that is not stored has no slot (the row's other tasks do not use it either)
+    if (!in && h == 0 && c == 0) gst(a.slot + r, -1);
     if (h < a.hq + a.hk) {
         const float *w = isq ? a.qn : a.kn;
         if (w) {
@@ -535,7 +538,7 @@ navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *head
     OnDevice dev;
     if ((st = dev.enter(stream, "kv_append", err, errlen)) != NAVI_OK) return st;
     if (pages->n_rows == 0) return NAVI_OK;
-    const AppendArgs a{d_x, d_q_norm, d_k_norm, d_rot, d_k, d_v, d_q, pages->cu_rows, pages->row_slot, pages->row_pos, eps, pages->n_requests,
+    const AppendArgs a{d_x, d_q_norm, d_k_norm, d_rot, d_k, d_v, d_q, pages->cu_rows, pages->row_pos, pages->row_slot, eps, pages->n_requests,
                        pages->n_rows, n_rot, pages->n_pages * pages->page_size, heads->n_head, heads->n_kv_head, ldx, ld_kv, ldq,
                        make_div(static_cast<uint32_t>(nh))};
     hipStream_t s = static_cast<hipStream_t>(stream);

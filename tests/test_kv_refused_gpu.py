@@ -115,3 +115,25 @@ def test_an_array_named_more_than_once_is_moved_once():
     for i in ((0, 0), (1, 1)):
         want[i][at[:11]] = want[i][at[1:]].clone()
     assert torch.equal(s.pool.cpu(), want) and past.tolist() == [14, 20] and done.tolist() == [0, 0]
+
+
+def test_append_takes_the_slot_of_a_row_without_a_rotation():
+    """Its K and V are not stored, so a commit over it is refused; the rows before it commit."""
+    s = Planned([(3, [-1, 0, 1]), (28, [-1, 0, 0, 1, 3, 4])])
+    slots = s.t["slot"].tolist()
+    heads, width = abi.KvHeads(2, 1, 64, abi.DT_F16), 64
+    x, q = torch.ones(9, 256, device="cuda").half(), torch.ones(9, 128, device="cuda").half()
+    k, v = torch.zeros(s.n_pages * PAGE, width, device="cuda").half(), torch.zeros(s.n_pages * PAGE, width, device="cuda").half()
+    turn = torch.cat([torch.ones(31, 32), torch.zeros(31, 32)], 1).cuda()                  # positions 0 .. 30
+    abi.kv_append(s.pages, heads, x.data_ptr(), abi.DT_F16, 256, k.data_ptr(), v.data_ptr(), width, q.data_ptr(), abi.DT_F16, 128, rot=turn.data_ptr(),
+                  n_rot=31, stream=stream())
+    torch.cuda.synchronize()
+    pos, want = s.t["pos"].tolist(), list(slots)
+    assert pos == [3, 4, 5, 28, 29, 29, 30, 31, 32]
+    want[7] = want[8] = -1
+    assert s.t["slot"].tolist() == want and q[7:].abs().max() == 0 and bool((q[:7] == 1).all())
+    stored = torch.zeros(s.n_pages * PAGE, dtype=torch.bool)
+    stored[slots[:7]] = True
+    assert torch.equal((k[:, 0] == 1).cpu(), stored) and torch.equal((v[:, 5] == 1).cpu(), stored)
+    check(s, [[0, 1], [0, 1, 3, 4]], [True, False], True)
+    check(s, [[0, 1], [0, 1, 3]], [True, True], True)
