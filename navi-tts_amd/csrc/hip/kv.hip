@@ -535,6 +535,10 @@ navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *head
         set_err(err, errlen, "kv_append: %d rows of %d heads are too many for one call", pages->n_rows, nh);
         return NAVI_ERR_INVALID;
     }
+    if (d_q && d_q == d_x && (x_dtype != q_dtype || ldx != ldq)) {
+        set_err(err, errlen, "kv_append: d_q over d_x of another type or stride (x %d, %d; q %d, %d)", x_dtype, ldx, q_dtype, ldq);
+        return NAVI_ERR_INVALID;
+    }
     OnDevice dev;
     if ((st = dev.enter(stream, "kv_append", err, errlen)) != NAVI_OK) return st;
     if (pages->n_rows == 0) return NAVI_OK;

@@ -1074,6 +1074,10 @@ navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads 
         set_err(err, errlen, "tree_attention: %d requests of %d heads are too many for one call", pages->n_requests, heads->n_head);
         return NAVI_ERR_INVALID;
     }
+    if (d_out && d_out == d_q && ldo != ldq) {
+        set_err(err, errlen, "tree_attention: d_out over d_q of another stride (%d, %d)", ldo, ldq);
+        return NAVI_ERR_INVALID;
+    }
     const size_t need = tree::workspace(*pages, *heads, max_keys);
     if (need > 0 && (!d_ws || !kv::aligned16(d_ws) || ws_bytes < need)) {
         set_err(err, errlen, "tree_attention: the workspace is null, misaligned or smaller than %zu bytes (%zu)", need, ws_bytes);

@@ -174,3 +174,15 @@ ROWS = 8 * 16 * 1024 * 2                        # bytes of a layer's K or V in t
 def test_commit_refuses_rows_of_one_array_inside_another(k, v):
     """Rows are moved whole: K and V interleaved in one allocation (V's base inside K's row) would move into each other, and past its end."""
     assert "overlap" in refused(4, abi.kv_commit, pages(), k, v, 1024, P, 4, P, P + 64, P + 128)
+
+
+def test_append_refuses_queries_over_rows_of_another_layout():
+    """In place a head overwrites itself only with the same type and stride."""
+    for kw in (dict(ldx=4096, ldq=2048), dict(ldx=4096, ldq=4096, xt=1), dict(ldx=4096, ldq=4096, qt=1)):
+        a, k = _append(x=P, q=P, **kw)
+        assert "over d_x" in refused(4, *a, **k)
+
+
+def test_attention_refuses_results_over_queries_of_another_stride():
+    assert "over d_q" in refused(4, *_attend(q=P, out=P, ldq=2048, ldo=4096))
+    assert "over d_q" in refused(4, *_attend(q=P, out=P, ldq=4096, ldo=2048, keys=4096))
