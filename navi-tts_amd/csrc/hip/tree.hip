@@ -1074,6 +1074,10 @@ navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads 
         set_err(err, errlen, "tree_attention: %d requests of %d heads are too many for one call", pages->n_requests, heads->n_head);
         return NAVI_ERR_INVALID;
     }
+    if (!std::isfinite(scale)) {
+        set_err(err, errlen, "tree_attention: scale %g", static_cast<double>(scale));
+        return NAVI_ERR_INVALID;
+    }
     if (d_out && d_out == d_q && ldo != ldq) {
         set_err(err, errlen, "tree_attention: d_out over d_q of another stride (%d, %d)", ldo, ldq);
         return NAVI_ERR_INVALID;

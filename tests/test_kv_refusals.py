@@ -186,3 +186,8 @@ def test_append_refuses_queries_over_rows_of_another_layout():
 def test_attention_refuses_results_over_queries_of_another_stride():
     assert "over d_q" in refused(4, *_attend(q=P, out=P, ldq=2048, ldo=4096))
     assert "over d_q" in refused(4, *_attend(q=P, out=P, ldq=4096, ldo=2048, keys=4096))
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf")])
+def test_attention_refuses_a_scale_that_is_no_number(scale):
+    assert "scale" in refused(4, abi.tree_attention, pages(), heads(), P, 0, 2048, P, P, 1024, scale, 64, P, 2048, P, 1 << 30)
