@@ -291,3 +291,16 @@ def test_a_request_that_runs_past_the_last_position(side, past, inside):
                       stream=abi.lib().navi_device_stream())
         torch.cuda.synchronize()
         assert out.tolist() == [0, done] and now.tolist() == [1, past + (accept if done == 0 else 0)]
+
+
+def test_verify_of_512_rows(side):
+    """Eight requests' chains of 64, each against the chain one request at a time."""
+    abi, _, _, W = side
+    talker, rng = abi.Talker(W, max_prompt_tokens=512, max_positions=512), np.random.default_rng(10)
+    x = [rng.standard_normal((64, 1024)).astype(np.float32) for _ in range(8)]
+    kv, chain = abi.KvCache(talker.kv.n_layer, 512, 1024), [j - 1 for j in range(64)]
+    h, l = Pool(abi, talker, 8, {}).step([chain] * 8, x, kv=kv)
+    assert np.isfinite(h).all() and np.isfinite(l).all()
+    for i in (0, 3, 7):
+        h1, l1 = Pool(abi, talker, 1, {}).step([chain], [x[i]], kv=kv)
+        assert np.abs(h[64 * i:64 * i + 64] - h1).max() < TOL_ABS and np.abs(l[64 * i:64 * i + 64] - l1).max() < TOL_ABS
