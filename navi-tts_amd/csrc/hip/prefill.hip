@@ -1116,7 +1116,7 @@ navi_status navi_talker_verify(navi_talker *t, const navi_kv_view *kv, const nav
         st = navi_kv_append(pages, &heads, t->part, NAVI_DT_F32, QKVW, w.qn, w.kn, t->eps, t->rot_all, t->max_pos, kv->k[l], kv->v[l], t->KVD,
                             t->q, NAVI_DT_F32, t->QD, s, err, errlen);
         if (st != NAVI_OK) return st;
-        tree::launch({pages, &heads, t->q, kv->k[l], kv->v[l], t->att, t->tree_ws, t->tree_bytes, NAVI_DT_F32, t->QD, t->KVD, t->QD, max_keys,
+        tree::launch({pages, &heads, t->q, kv->k[l], kv->v[l], t->att, t->tree_ws, NAVI_DT_F32, t->QD, t->KVD, t->QD, max_keys,
                       1.f / std::sqrt(static_cast<float>(HD)), true, true}, s);
         ok = ok && rows::launch_rows_pk(rows::EPI_RESID, false, t->att, T, t->QD, nullptr, 0.f, w.o_t, H, t->x, 0, t->flag, s) &&
              rows::launch_rows_pk(rows::EPI_SWIGLU, true, t->x, T, H, w.ln2, t->eps, w.gu_t, t->F, t->h, 0, t->flag, s) &&

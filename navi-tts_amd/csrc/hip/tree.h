@@ -12,7 +12,6 @@ struct Call {
     const navi_kv_heads *heads;
     const void *q, *k, *v;
     void *out, *ws;
-    size_t ws_bytes;
     int q_dtype, ldq, ldkv, ldo, max_keys;
     float scale;
     bool tiled;                        // f32 out in the tile layout of rows.h (ldo unused)

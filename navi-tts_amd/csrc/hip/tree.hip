@@ -1090,7 +1090,7 @@ navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads 
     kv::OnDevice dev;
     if ((st = dev.enter(stream, "tree_attention", err, errlen)) != NAVI_OK) return st;
     if (pages->n_rows == 0) return NAVI_OK;
-    tree::launch({pages, heads, d_q, d_k, d_v, d_out, d_ws, ws_bytes, q_dtype, ldq, ld_kv, ldo, max_keys, scale, false, false},
+    tree::launch({pages, heads, d_q, d_k, d_v, d_out, d_ws, q_dtype, ldq, ld_kv, ldo, max_keys, scale, false, false},
                  static_cast<hipStream_t>(stream));
     NAVI_TRY_HIP(hipGetLastError(), err, errlen);
     return NAVI_OK;
