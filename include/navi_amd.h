@@ -341,7 +341,9 @@ navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *head
  * infinities and NaN included; a position whose page is outside the pool is not seen; a row that sees
  * nothing gets zeros. Rows past cu_rows[n_requests] and past max_new of a request are left as they were.
  * max_keys: the most positions a request may reach (n_past + rows), by which the work is split; longer
- * requests are still right, but slow. n_requests * n_head < 2^23. d_ws: navi_tree_workspace(...) bytes, 16-byte aligned, for this call
+ * requests are still right, but slow. Above 256 requests none is split: a call takes as long as its longest request on one
+ * block a kv head. An infinity or NaN in V of a position that a row sees leaves the row's column infinite or NaN.
+ * scale is finite. n_requests * n_head < 2^23. d_ws: navi_tree_workspace(...) bytes, 16-byte aligned, for this call
  * alone until it is done: calls that may overlap need a workspace each. d_out may be d_q with the same stride. Alignment as navi_kv_append. */
 navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads *heads, const void *d_q, int32_t q_dtype, int32_t ldq,
                                 const void *d_k, const void *d_v, int32_t ld_kv, float scale, int32_t max_keys, void *d_out,

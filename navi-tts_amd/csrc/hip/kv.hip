@@ -324,7 +324,7 @@ __device__ __forceinline__ void store4(T *p, f32x4_t v) {
 
 // One head of one row takes D / 8 lanes: lane c holds elements 4c .. 4c + 3 of each half, the pairs that
 // the rotation mixes, so a head is read, normed, turned and written from registers. Its bytes bound it: 9009 bf16 rows
-// of 16 + 2 x 8 heads of 128 (148 MB read and written) take 33.8 us, 4.4 TB/s, a large copy 4.6; one row 2.9 us.
+// of 16 + 2 x 8 heads of 128 (148 MB read and written) take 35.4 us, 4.2 TB/s, a large copy 4.6; one row 2.9 us.
 template <class X, class Q, class E, int D>
 __global__ void __launch_bounds__(256) k_append(AppendArgs a) {
     constexpr int LN = D / 8, HB = 256 / LN;
@@ -411,7 +411,7 @@ struct CommitArgs {
 // Block (columns, request, array): each thread moves 16 bytes of a row for the whole path, in order. A
 // path ascends, so its j-th source lies at or above position j: a row is read before, or when, it
 // is written, and batches of eight that read before they write keep that. 32 requests' paths of 8 rows in 28 layers (44 MB)
-// take 10.4 us, 4.25 TB/s; one request's 3.7 us, three rounds of memory latency.
+// take 10.6 us, 4.1 TB/s; one request's 3.9 us, four rounds of memory latency (lengths; path; tables and slots; rows).
 constexpr int CT = 128;
 __global__ void __launch_bounds__(CT) k_commit(CommitArgs a) {
     __shared__ int src[WAVE], dst[WAVE];

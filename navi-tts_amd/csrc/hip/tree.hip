@@ -9,23 +9,23 @@
 //  * Scores are computed transposed, S^T = K Q^T (v_mfma_f32_16x16x32: 16 keys x 16 query rows): a lane then
 //    holds 4 keys of one query row per tile, and two such tiles are, register for register, the B operand
 //    of O^T += V^T P^T over 32 keys if V^T's operand takes its keys in that order too. P never leaves
-//    its registers, and a row's maximum, sum and mask are a lane's own values.
+//    its registers (as a hi + lo pair of the cache's type, two products), and a row's maximum, sum and mask are a lane's own values.
 //  * V^T's operand is V read from LDS through the transposing load (ds_read_b64_tr_b16: in a
 //    16-lane group lane 4r + c fetches columns 4c.. of key r and gets column `lane`, keys 0..3). V rows sit
 //    in LDS with their 32-byte chunks XORed by the key, so that the 16 rows such a load touches
 //    spread over all banks.
 //  * Up to 32 query rows (k_tree) a wave works alone on its own 32-key tiles, every W-th of the block's range, with K from
 //    memory in operand form, its own V buffer and no barrier until its range ends; then the waves' results are joined in
-//    LDS. 32 requests with one row each over 1024 keys take 25.7 us, 5.24 TB/s: the cache's bytes at the rate of a large
+//    LDS. 32 requests with one row each over 1024 keys take 25.9 us, 5.20 TB/s: the cache's bytes at the rate of a large
 //    read (5.6 TB/s here) are 24.
 //  * Above (k_tree_rows) two or four waves with 32 rows each share the K and V tiles, which go through LDS in two buffers with
-//    one barrier a tile. 64 requests x 24 rows (48 query rows) over 8192 keys 415 us, 5.2 TB/s; without the products 385.
-//    64 f32 rows (128 query rows) over 32768 keys 59 us: 39 us for every further 32768 keys, which with the pairs' doubled
+//    one barrier a tile. 64 requests x 24 rows (48 query rows) over 8192 keys 414 us (412 to 417 in three runs), 5.2 TB/s; without the products 385.
+//    64 f32 rows (128 query rows) over 32768 keys 58 us: 39 us for every further 32768 keys, which with the pairs' doubled
 //    products are 880 TFLOP/s, and 20 us for the start, the parts' 17 MB and the join.
 //  * Softmax against a reference value that moves only when a score passes it by more than SLACK: the
 //    rescaling, and the maximum over lanes that it needs, are off the common path. exp2 with the scale folded in.
 //  * Requests are cut into even chunks over the blocks, however uneven their lengths (lay_out): 64 requests of lengths spread from
-//    1 to 8000 70 us, uncut 143. A second kernel joins the chunks' results (unnormalised sums, reference, sum) in their order.
+//    1 to 8000 71 us, uncut 145. A second kernel joins the chunks' results (unnormalised sums, reference, sum) in their order.
 #include "dev_common.h"
 #include "tile_layout.h"
 #include "tree.h"
@@ -41,12 +41,15 @@ using kv::Div;
 using kv::div_by;
 
 constexpr int NW = 4, BT = NW * WAVE;  // waves of a block of k_tree_join
-// Of k_tree: eight, more loads on their way, where a block has a whole request (32 requests of 1024 keys: 25.7 us, with four
-// 27.0); four, and twice as many blocks, where requests are cut (64 ragged ones of up to 8000 keys: 70 us, with eight 86).
+// Of k_tree: eight, more loads on their way, where a block has a whole request; four, and twice as many blocks, where requests are
+// cut (64 ragged ones of up to 8000 keys: 71 us, with eight 84). Eight waves fill a CU, so their gain ends where the blocks are
+// more than the CUs: 8 kv heads over 1000 keys, us with eight / four: 24 requests 29.1 / 29.2, 32 25.7 / 27.1, 33 42.6 / 38.4,
+// 40 46.6 / 45.0, 48 51.0 / 49.4, 64 56.3 / 55.1.
 constexpr int alone_of(bool cut) { return cut ? 4 : 8; }
 // Of k_tree_rows, RW waves of which share their query rows' tiles: eight, one block a CU, so that half as many parts of
-// a cut request are stored and joined (64 drafted rows over 32768 keys: 57 us, with four 64); four where two waves share and
-// the registers allow two blocks a CU (64 requests x 24 rows over 8192 keys: 401 us, with eight 417).
+// a cut request are stored and joined (64 drafted f32 rows over 32768 keys: 59 us, with four 64; 16 x 80 query rows over 4000 78 and
+// 80); four where two waves share and the registers allow two blocks a CU (64 requests x 24 rows over 8192 keys: 415 us in each of
+// two runs, with eight 432 and 435).
 constexpr int waves_of(bool pair, int rw) { return rw == 2 && !pair ? 4 : 8; }
 constexpr int KT = 32;                 // keys of a wave's tile
 // p = 2^(s - reference + LIFT): at most 2^(SLACK + LIFT) = 2^14, inside f16, and f16's full precision down to
@@ -930,11 +933,17 @@ Cut cut_of(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys, bool pa
     const int waves = c.waves == 1 ? alone_of(true) : waves_of(pair, c.waves);
     c.step = waves / c.waves;                           // tiles of a block's turn
     const int steps = (max_keys + KT * c.step - 1) / (KT * c.step);
-    // A block a request where no request can be long enough to share (one row of 16 heads over 256 keys: 8.3 us, cut 10.5; over
-    // 512: 11.6 and 10.4); where there are blocks for all CUs and no request is so long that an uneven one would cost more than
-    // the chunks and the join (one row of 32 requests, all alike and of lengths spread down to one: of 1000 keys 25.7 and 19.5 us,
-    // cut 30.5 and 14.5; of 1400 38.6 and 24.7, cut 45.4 and 19.4; of 2000 54.2 and 33.9, cut 59.2 and 22.6); and for more
-    // requests than a block lays out. Else enough blocks for all waves of the CUs.
+    // A block a request where no request can be long enough to share (one row of 16 heads over 256 keys: 8.6 us, cut 10.6; over
+    // 512: 11.9 and 10.5); where there are blocks for all CUs and no request is long; and for more requests than a block lays out,
+    // whatever their lengths (of 1 to 1000 keys: 256 requests 70 us, 300 81; of 1 to 32768: 950 and 1000). Else enough blocks for
+    // all waves of the CUs. The second rule is a choice, since the host knows the most keys and not the lengths: cutting costs a
+    // batch of even lengths the layout and the join, and gains where they are uneven, the more the longer the longest. 32 requests,
+    // us uncut / cut, all alike and of lengths spread down to one:
+    //   one row, up to 1000 keys 25.6 / 30.2 and 19.6 / 14.4, 1400 38.2 / 44.5 and 24.9 / 19.3, 2000 53.6 / 59.0 and 34.3 / 22.6;
+    //   24 rows (48 query rows), up to 600 keys 26.0 / 33.8 and 22.8 / 22.4, 1000 37.3 / 42.8 and 31.3 / 27.6, 1400 54.8 / 59.7 and
+    //   42.4 / 30.9.
+    // Below 1280 keys even batches are favoured, above uneven ones. Just past a block a CU an uncut call pays a second round: 33
+    // requests of one row, up to 1000 keys, 42.7 / 37.2 and 19.7 / 16.7; 48 requests 49.6 / 47.2 and 20.0 / 20.0.
     if (p.n_requests > MAXB || steps == 1 || (c.waves == 1 && max_keys <= 384) || (max_keys <= 1280 && p.n_requests * heads >= 256)) {
         c.workers = c.parts = 0;
         return c;
