@@ -94,7 +94,7 @@ typedef struct {                       /* the fields of params.h:29-73 the path 
     int32_t codec_bos_id, codec_pad_id, codec_think_id, codec_nothink_id, codec_think_bos_id, codec_think_eos_id;
 } navi_model_params;
 
-typedef enum { NAVI_DT_F32 = 0, NAVI_DT_F16 = 1, NAVI_DT_BF16 = 2, NAVI_DT_I32 = 3, NAVI_DT_U8 = 4 } navi_dtype;
+typedef enum { NAVI_DT_F32 = 0, NAVI_DT_F16 = 1, NAVI_DT_BF16 = 2, NAVI_DT_I32 = 3, NAVI_DT_U8 = 4, NAVI_DT_F8E4M3 = 5 } navi_dtype;
 
 /* One device-resident weight (DeviceTensor, device_weights.h:17-21): the C
  * stand-in for DeviceWeights::get(name). Shapes are checked by each create(). */
@@ -263,7 +263,8 @@ navi_status navi_linear_noalloc(const float *d_x, int32_t ldx, int32_t M, const 
  * cache. For servers whose requests share one pool of cache rows and check several drafted tokens a
  * step. A pool holds, per layer, K and V rows [n_pages * page_size][kv_dim] of two-byte elements: the
  * layout of navi_kv_view, whose max_pos rows become pages of page_size rows (a single request's
- * cache is a pool of one page). Request i keeps position t in row
+ * cache is a pool of one page). Or, with kv_dtype NAVI_DT_F8E4M3, of one-byte elements: e4m3 (3 bits of fraction, 2^-9 .. 448,
+ * no infinities), which stand for code * factor of their kv head: half the bytes to hold and to read. Request i keeps position t in row
  * block_table[i][t / page_size] * page_size + t % page_size, its slot. One step:
  *   navi_kv_plan         pages, slots, positions and ancestors of the step's rows
  *   navi_kv_append       a layer's q|k|v rows: K and V into the pages, q for the attention
@@ -292,7 +293,10 @@ typedef struct {                       /* a step's requests and rows on a pool o
 
 typedef struct {
     int32_t n_head, n_kv_head, head_dim;   /* n_head a multiple of n_kv_head; head_dim 64 or 128 */
-    int32_t kv_dtype;                      /* of the pool: NAVI_DT_F16 or NAVI_DT_BF16 */
+    int32_t kv_dtype;                      /* of the pool: NAVI_DT_F16, NAVI_DT_BF16 or NAVI_DT_F8E4M3 */
+    /* of an e4m3 pool (else not looked at): device arrays [n_kv_head], above 0 and finite; a stored code stands for code * factor.
+     * NULL: 1. One pair a layer as its calibration gave them. */
+    const float *k_scale, *v_scale;
 } navi_kv_heads;
 
 /* The step's block tables and slot maps from its lengths. Per request: d_n_new[i] rows are added to
@@ -327,7 +331,9 @@ navi_status navi_kv_plan(const navi_kv_pages *pages, const int32_t *d_n_new, con
  * past cu_rows[n_requests] are left alone; a slot outside the pool stores no k and v; a position
  * outside 0 .. n_rot - 1 stores no k and v and a q of zeros, and the row's row_slot becomes -1 (navi_kv_commit with pages->status
  * takes no path over it). Strides in elements; strides and
- * pointers keep every row 16-byte aligned. d_q may be d_x with the same type and stride. */
+ * pointers keep every row 16-byte aligned. d_q may be d_x with the same type and stride.
+ * An e4m3 pool: rows and q are f32, f16 or bf16 each; k and v are divided by their head's factor (heads->k_scale, v_scale) in
+ * f32 and rounded to the nearest code, ties to even; past 448 factors, infinities too, to 448 of their sign; NaN stays NaN. */
 navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *heads, const void *d_x, int32_t x_dtype, int32_t ldx,
                            const float *d_q_norm, const float *d_k_norm, float eps, const float *d_rot, int32_t n_rot, void *d_k,
                            void *d_v, int32_t ld_kv, void *d_q, int32_t q_dtype, int32_t ldq, void *stream, char *err,
@@ -343,6 +349,8 @@ navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *head
  * max_keys: the most positions a request may reach (n_past + rows), by which the work is split; longer
  * requests are still right, but slow. Above 256 requests none is split: a call takes as long as its longest request on one
  * block a kv head. An infinity or NaN in V of a position that a row sees leaves the row's column infinite or NaN.
+ * An e4m3 pool: d_q and d_out are f32, f16 or bf16; out = v_scale softmax(scale k_scale q . K) V with the head's factors on the codes; the
+ * probabilities travel as pairs of f16, or of bf16 for bf16 q.
  * scale is finite. n_requests * n_head < 2^23. d_ws: navi_tree_workspace(...) bytes, 16-byte aligned, for this call
  * alone until it is done: calls that may overlap need a workspace each. d_out may be d_q with the same stride. Alignment as navi_kv_append. */
 navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads *heads, const void *d_q, int32_t q_dtype, int32_t ldq,
@@ -352,7 +360,8 @@ navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads 
 size_t navi_tree_workspace(const navi_kv_pages *pages, const navi_kv_heads *heads, int32_t max_keys);
 /* The accepted rows of each request moved into place in every layer of `kv` (n_layer, max_pos >= the pool's rows, kv_dim the
  * row stride, a multiple of 8; whole strides are moved, so that the layers' K and V must not overlap as n_pages * page_size rows of kv_dim: K
- * and V interleaved in one allocation are refused; an array named more than once is moved once): with path = d_path[i][0 .. d_accept[i] - 1] (stride max_path <= 64), the indexes of accepted rows within
+ * and V interleaved in one allocation are refused; an array named more than once is moved once; kv_dim counts two-byte elements, so that an
+ * e4m3 pool's rows of ld_kv bytes have a kv_dim of ld_kv / 2): with path = d_path[i][0 .. d_accept[i] - 1] (stride max_path <= 64), the indexes of accepted rows within
  * the request's step in ascending order, position n_past[i] + j takes the K and V of position n_past[i] + path[j].
  * d_n_past_out[i] = n_past[i] + d_accept[i]. d_n_past_out and d_status are none of the call's inputs. d_status[i]: 0, or 2 where
  * d_accept[i] is outside 0 .. max_path, the path does not ascend or leaves the request's rows, a page of these, or of the request's

@@ -2,6 +2,7 @@
 // tables and slots from the requests' lengths, its K and V rows into the pages, and the accepted
 // drafts' rows moved into place. The attention that reads the pages is in tree.hip.
 #include "dev_common.h"
+#include "f8.h"
 #include "kv.h"
 
 #include <algorithm>
@@ -34,12 +35,17 @@ navi_status check_heads(const char *who, const navi_kv_heads *h, int ld_kv, char
         set_err(err, errlen, "%s: %d heads over %d kv heads", who, h->n_head, h->n_kv_head);
         return NAVI_ERR_INVALID;
     }
-    if ((h->head_dim != 64 && h->head_dim != 128) || (h->kv_dtype != NAVI_DT_F16 && h->kv_dtype != NAVI_DT_BF16)) {
-        set_err(err, errlen, "%s: unsupported head_dim %d or cache type %d (64 or 128; f16 or bf16)", who, h->head_dim, h->kv_dtype);
+    const bool f8 = h->kv_dtype == NAVI_DT_F8E4M3;
+    if ((h->head_dim != 64 && h->head_dim != 128) || (h->kv_dtype != NAVI_DT_F16 && h->kv_dtype != NAVI_DT_BF16 && !f8)) {
+        set_err(err, errlen, "%s: unsupported head_dim %d or cache type %d (64 or 128; f16, bf16 or e4m3)", who, h->head_dim, h->kv_dtype);
         return NAVI_ERR_UNSUPPORTED;
     }
-    if (ld_kv < h->n_kv_head * h->head_dim || ld_kv % 8 != 0) {
+    if (ld_kv < h->n_kv_head * h->head_dim || ld_kv % (f8 ? 16 : 8) != 0) {
         set_err(err, errlen, "%s: cache row stride %d for %d kv heads of %d", who, ld_kv, h->n_kv_head, h->head_dim);
+        return NAVI_ERR_INVALID;
+    }
+    if (f8 && ((reinterpret_cast<uintptr_t>(h->k_scale) | reinterpret_cast<uintptr_t>(h->v_scale)) & 3u)) {
+        set_err(err, errlen, "%s: the kv heads' factors are not 4-byte aligned", who);
         return NAVI_ERR_INVALID;
     }
     return NAVI_OK;
@@ -294,7 +300,7 @@ __global__ void __launch_bounds__(FT) k_plan_fill(PlanArgs a) {
 
 struct AppendArgs {
     const void *x;
-    const float *qn, *kn, *rot;
+    const float *qn, *kn, *rot, *ks, *vs;      // ks, vs: an e4m3 pool's factors, or null
     void *k, *v, *q;
     const int32_t *cu, *pos;
     int32_t *slot;
@@ -316,6 +322,7 @@ __device__ __forceinline__ f32x4_t load4(const T *p) {
 template <class T>
 __device__ __forceinline__ void store4(T *p, f32x4_t v) {
     if constexpr (sizeof(T) == 4) st4(reinterpret_cast<float *>(p), v);
+    else if constexpr (sizeof(T) == 1) gst(reinterpret_cast<uint32_t *>(p), f8_pack4(v));
     else {
         typedef T T4 __attribute__((ext_vector_type(4)));
         *(NAVI_GLOBAL T4 *) p = T4{static_cast<T>(v[0]), static_cast<T>(v[1]), static_cast<T>(v[2]), static_cast<T>(v[3])};
@@ -375,7 +382,16 @@ __global__ void __launch_bounds__(256) k_append(AppendArgs a) {
         store4(q + D / 2, x1);
     } else if (in && static_cast<unsigned>(slot) < static_cast<unsigned>(a.slots)) {
         const bool isk = h < a.hq + a.hk;
-        E *d = static_cast<E *>(isk ? a.k : a.v) + static_cast<size_t>(slot) * a.ldkv + (h - a.hq - (isk ? 0 : a.hk)) * D + 4 * c;
+        const int kvh = h - a.hq - (isk ? 0 : a.hk);
+        if constexpr (sizeof(E) == 1) {
+            const float *f = isk ? a.ks : a.vs;
+            if (f) {
+                const float s = gld(f + kvh);
+                x0 /= s;
+                x1 /= s;
+            }
+        }
+        E *d = static_cast<E *>(isk ? a.k : a.v) + static_cast<size_t>(slot) * a.ldkv + kvh * D + 4 * c;
         store4(d, x0);
         store4(d + D / 2, x1);
     }
@@ -395,6 +411,14 @@ void launch_append_types(const AppendArgs &a, bool xf, bool qf, int D, hipStream
     else if (xf) launch_append<float, E, E>(a, D, s);
     else if (qf) launch_append<E, float, E>(a, D, s);
     else launch_append<E, E, E>(a, D, s);
+}
+
+// An e4m3 pool's rows and queries have any of the three types each.
+template <class X>
+void launch_append_f8(const AppendArgs &a, int q_dtype, int D, hipStream_t s) {
+    if (q_dtype == NAVI_DT_F32) launch_append<X, float, f8_t>(a, D, s);
+    else if (q_dtype == NAVI_DT_F16) launch_append<X, _Float16, f8_t>(a, D, s);
+    else launch_append<X, __bf16, f8_t>(a, D, s);
 }
 
 // ---- commit ----------------------------------------------------------------------------------
@@ -520,7 +544,9 @@ navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *head
     if (st == NAVI_OK) st = check_heads("kv_append", heads, ld_kv, err, errlen);
     if (st != NAVI_OK) return st;
     const int D = heads->head_dim, nh = heads->n_head + 2 * heads->n_kv_head;
-    if ((x_dtype != NAVI_DT_F32 && x_dtype != heads->kv_dtype) || (q_dtype != NAVI_DT_F32 && q_dtype != heads->kv_dtype)) {
+    const bool f8 = heads->kv_dtype == NAVI_DT_F8E4M3;
+    auto known = [&](int t) { return t == NAVI_DT_F32 || (f8 ? t == NAVI_DT_F16 || t == NAVI_DT_BF16 : t == heads->kv_dtype); };
+    if (!known(x_dtype) || !known(q_dtype)) {
         set_err(err, errlen, "kv_append: unsupported types (x %d, q %d, cache %d)", x_dtype, q_dtype, heads->kv_dtype);
         return NAVI_ERR_UNSUPPORTED;
     }
@@ -542,11 +568,15 @@ navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *head
     OnDevice dev;
     if ((st = dev.enter(stream, "kv_append", err, errlen)) != NAVI_OK) return st;
     if (pages->n_rows == 0) return NAVI_OK;
-    const AppendArgs a{d_x, d_q_norm, d_k_norm, d_rot, d_k, d_v, d_q, pages->cu_rows, pages->row_pos, pages->row_slot, eps, pages->n_requests,
+    const AppendArgs a{d_x, d_q_norm, d_k_norm, d_rot, f8 ? heads->k_scale : nullptr, f8 ? heads->v_scale : nullptr, d_k, d_v, d_q, pages->cu_rows, pages->row_pos, pages->row_slot, eps, pages->n_requests,
                        pages->n_rows, n_rot, pages->n_pages * pages->page_size, heads->n_head, heads->n_kv_head, ldx, ld_kv, ldq,
                        make_div(static_cast<uint32_t>(nh))};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (heads->kv_dtype == NAVI_DT_F16) launch_append_types<_Float16>(a, x_dtype == NAVI_DT_F32, q_dtype == NAVI_DT_F32, D, s);
+    if (f8) {
+        if (x_dtype == NAVI_DT_F32) launch_append_f8<float>(a, q_dtype, D, s);
+        else if (x_dtype == NAVI_DT_F16) launch_append_f8<_Float16>(a, q_dtype, D, s);
+        else launch_append_f8<__bf16>(a, q_dtype, D, s);
+    } else if (heads->kv_dtype == NAVI_DT_F16) launch_append_types<_Float16>(a, x_dtype == NAVI_DT_F32, q_dtype == NAVI_DT_F32, D, s);
     else launch_append_types<__bf16>(a, x_dtype == NAVI_DT_F32, q_dtype == NAVI_DT_F32, D, s);
     NAVI_TRY_HIP(hipGetLastError(), err, errlen);
     return NAVI_OK;

@@ -27,6 +27,7 @@
 //  * Requests are cut into even chunks over the blocks, however uneven their lengths (lay_out): 64 requests of lengths spread from
 //    1 to 8000 71 us, uncut 145. A second kernel joins the chunks' results (unnormalised sums, reference, sum) in their order.
 #include "dev_common.h"
+#include "f8.h"
 #include "tile_layout.h"
 #include "tree.h"
 
@@ -59,6 +60,7 @@ constexpr float NONE = -INFINITY;
 
 struct Args {
     const void *q, *k, *v;
+    const float *ks, *vs;              // an e4m3 pool's factors of K and V a kv head, or null
     void *out;
     float *po, *pm;                    // the parts of requests that are cut (part_of)
     uint32_t *first;                   // and each group's chunks before every request [groups][n + 1]
@@ -99,6 +101,10 @@ __device__ __forceinline__ bool any_special(u32x4_t x) {
     for (int i = 0; i < 4; ++i) b |= (x[i] & LO) == LO || (x[i] & HI) == HI;
     return b;
 }
+
+// What the scores of a kv head's keys are multiplied with, and what its sums of V are.
+__device__ __forceinline__ float score_factor(const Args &a, int kvh) { return a.ks ? a.scale * gld(a.ks + kvh) : a.scale; }
+__device__ __forceinline__ float value_factor(const Args &a, int kvh) { return a.vs ? gld(a.vs + kvh) : 1.f; }
 
 // Four consecutive columns of an output row.
 template <class E, bool PAIR>
@@ -297,17 +303,23 @@ struct Rows {
     struct Raw {
         u32x4_t x[QP * KS];
     };
+    // Step k of the operands has columns 32 k + 8 (l / 16) .. of the head; WIDE: 64 (k / 2) + 16 (l / 16) + 8 (k % 2) .., as K in 8 bits comes
+    // into registers.
+    template <bool WIDE>
     static __device__ __forceinline__ void fetch(const Args &a, const Share &s, int m, Raw &r) {
         const int lg = (threadIdx.x & 63) >> 4, j = div_by(a.heads_per, m);
         const bool on = j < s.at.rows;
-        const size_t at = static_cast<size_t>(s.at.c0 + (on ? j : 0)) * a.ldq + static_cast<size_t>(s.kvh * a.g + (on ? m - j * a.g : 0)) * D + 8 * lg;
+        const size_t at = static_cast<size_t>(s.at.c0 + (on ? j : 0)) * a.ldq + static_cast<size_t>(s.kvh * a.g + (on ? m - j * a.g : 0)) * D +
+                          (WIDE ? 16 : 8) * lg;
         const unsigned char *p = static_cast<const unsigned char *>(a.q) + at * 2 * QP;
 #pragma unroll
-        for (int i = 0; i < QP * KS; ++i)
-            r.x[i] = on ? *(const NAVI_GLOBAL u32x4_t *) (p + 64 * QP * (i / QP) + 16 * (i % QP)) : u32x4_t{0u, 0u, 0u, 0u};
+        for (int i = 0; i < QP * KS; ++i) {
+            const int k = i / QP, col = WIDE ? 64 * (k / 2) + 8 * (k % 2) : 32 * k;
+            r.x[i] = on ? *(const NAVI_GLOBAL u32x4_t *) (p + 2 * QP * col + 16 * (i % QP)) : u32x4_t{0u, 0u, 0u, 0u};
+        }
     }
-    static __device__ __forceinline__ float operands(const Args &a, const Raw &r, v8 (&q)[QP * KS]) {
-        float f = a.scale;
+    static __device__ __forceinline__ float operands(const Args &a, float scale, const Raw &r, v8 (&q)[QP * KS]) {
+        float f = scale;
         if constexpr (PAIR) {
             // q times a power of two that puts the row's largest value into [1, 2): pairs keep 22 bits of it
             // whatever its range; the scores get the inverse
@@ -323,7 +335,7 @@ struct Rows {
                 }
             top = row_max(top);
             const int ex = top > 0.f && top < INFINITY ? ilogbf(top) : 0;
-            f = ldexpf(a.scale, ex);
+            f = ldexpf(scale, ex);
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -440,12 +452,13 @@ struct Rows {
 
     // Drafted keys with an infinity or NaN in V (rare; bits `special` of the tile): zeros in the products of add, since 0
     // times one would reach the rows that do not see them. Here the rows that do see them add theirs; sc: p.
+    template <class P>
     __device__ __forceinline__ void add_special(const f32x4_t (&sc)[NT][2], uint32_t special, int tile, const Share &s, const Pages &pg) {
         const int l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
         for (; special; special &= special - 1) {
             const int kin = __builtin_ctz(special), key = tile * KT + kin, ahead = key - s.at.past;
             const int slot = pg.slot_of(key, pg.page_of(key));
-            const E *vp = static_cast<const E *>(pg.a.v) + static_cast<size_t>(max(slot, 0)) * pg.a.ldkv + s.kvh * D + 4 * lg;
+            const P *vp = static_cast<const P *>(pg.a.v) + static_cast<size_t>(max(slot, 0)) * pg.a.ldkv + s.kvh * D + 4 * lg;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float p = 0.f;
@@ -455,7 +468,14 @@ struct Rows {
                 const bool vis = ahead >= 0 && ahead < 64 && (seen[nt] >> (ahead & 63) & 1);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    const v4 x = bits<v4>(*(const NAVI_GLOBAL u32x2_t *) (vp + 16 * d));
+                    v4 x;
+                    if constexpr (sizeof(P) == 1) {
+                        uint32_t w[2];
+                        f8_unpack4<E>(gld(reinterpret_cast<const uint32_t *>(vp + 16 * d)), w);
+                        x = bits<v4>(w);
+                    } else {
+                        x = bits<v4>(*(const NAVI_GLOBAL u32x2_t *) (vp + 16 * d));
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[nt][d][e] = vis ? fmaf(p, static_cast<float>(x[e]), acc[nt][d][e]) : acc[nt][d][e];
                 }
@@ -491,17 +511,32 @@ struct Rows {
                 gst(a.pm + 2 * at + 1, total);
             }
         } else {
-            store_out<E, PAIR>(a, s.at.c0 + j, (s.kvh * a.g + q - j * a.g) * D + col, a.hkv * a.g * D, o * (m == NONE ? 0.f : 1.f / total));
+            store_out<E, PAIR>(a, s.at.c0 + j, (s.kvh * a.g + q - j * a.g) * D + col, a.hkv * a.g * D, o * (m == NONE ? 0.f : value_factor(a, s.kvh) / total));
         }
     }
 };
 
+// Step k's 16 bytes of E from a lane's loads of a pool's row: as they are, or half a load's codes.
+template <class E, bool F8, int LD>
+__device__ __forceinline__ u32x4_t operand_of(const u32x4_t (&r)[LD], int k) {
+    if constexpr (F8) {
+        uint32_t lo[2], hi[2];
+        f8_unpack4<E>(r[k / 2][2 * (k % 2)], lo);
+        f8_unpack4<E>(r[k / 2][2 * (k % 2) + 1], hi);
+        return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+    } else {
+        return r[k];
+    }
+}
+
 // Up to 32 query rows: every wave has all of them and works alone on its own tiles, every W-th of the block's, with K from
 // memory in operand form and its own V buffer, no barrier until the end; then the W results are joined in LDS.
 // CUT: a block takes a chunk of a request's keys, else all of them.
-template <class E, bool PAIR, int D, int NT, bool CUT>
+// P: the pool's elements, E or e4m3; these come in 16-byte loads of twice as many columns and become E in registers.
+template <class E, bool PAIR, class P, int D, int NT, bool CUT>
 __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) k_tree(Args a) {
     constexpr int W = alone_of(CUT);
+    constexpr bool F8 = sizeof(P) == 1;
     typedef Rows<E, PAIR, D, NT> R;
     typedef typename R::v8 v8;
     constexpr int KS = R::KS, DT = R::DT, QP = R::QP, VB = KT * D * 2, DP = D + 4;
@@ -524,9 +559,10 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
     const int qrow0 = s.group * NT * 16;
     const Pages pg{a.table + static_cast<size_t>(s.req) * a.blocks, s.at.len, a};
 
-    u32x4_t kr[2][KS], vr[2][KS];
+    constexpr int LD = F8 ? KS / 2 : KS, LC = D / LD;             // loads a key and lane, columns of one over the four lanes
+    u32x4_t kr[2][LD], vr[2][LD];
     int slot[2], page[2];
-    const E *kb = static_cast<const E *>(a.k) + s.kvh * D + 8 * lg, *vb = static_cast<const E *>(a.v) + s.kvh * D + 8 * lg;
+    const P *kb = static_cast<const P *>(a.k) + s.kvh * D + LC / 4 * lg, *vb = static_cast<const P *>(a.v) + s.kvh * D + LC / 4 * lg;
     auto look_up = [&](int t) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) page[kt] = pg.page_of(t * KT + kt * 16 + lr);
@@ -537,12 +573,12 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
             slot[kt] = pg.slot_of(t * KT + kt * 16 + lr, page[kt]);
             const size_t at = static_cast<size_t>(max(slot[kt], 0)) * a.ldkv;
 #pragma unroll
-            for (int k = 0; k < KS; ++k) kr[kt][k] = *(const NAVI_GLOBAL u32x4_t *) (kb + at + 32 * k);
+            for (int k = 0; k < LD; ++k) kr[kt][k] = *(const NAVI_GLOBAL u32x4_t *) (kb + at + LC * k);
         }
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int k = 0; k < KS; ++k) vr[kt][k] = *(const NAVI_GLOBAL u32x4_t *) (vb + static_cast<size_t>(max(slot[kt], 0)) * a.ldkv + 32 * k);
+            for (int k = 0; k < LD; ++k) vr[kt][k] = *(const NAVI_GLOBAL u32x4_t *) (vb + static_cast<size_t>(max(slot[kt], 0)) * a.ldkv + LC * k);
     };
     int t = s.t0 + wv;
     if constexpr (CUT) {
@@ -553,7 +589,7 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
     }
     // q before K and V, which a wait for it would otherwise include (one row over 256 keys: 8.7 us, after them 10.2)
     typename R::Raw raw;
-    if (wv < NT) R::fetch(a, s, qrow0 + wv * 16 + lr, raw);
+    if (wv < NT) R::template fetch<F8>(a, s, qrow0 + wv * 16 + lr, raw);
     R rows;
     rows.start(a, s, qrow0);
     if (t < s.t_end) {
@@ -564,7 +600,7 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
     u32x4_t *s_q = reinterpret_cast<u32x4_t *>(sm + W * VB);
     if (wv < NT) {
         v8 q[QP * KS];
-        const float f = R::operands(a, raw, q);
+        const float f = R::operands(a, score_factor(a, s.kvh), raw, q);
 #pragma unroll
         for (int i = 0; i < QP * KS; ++i) s_q[((i / KS * NT + wv) * KS + i % KS) * WAVE + l] = bits<u32x4_t>(q[i]);
         if (lg == 0) s_fac[wv * 16 + lr] = f;
@@ -593,10 +629,13 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             if (k + 1 < KS) load_q(k + 1);
+            v8 kf[2];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) kf[kt] = bits<v8>(operand_of<E, F8>(kr[kt], k));
 #pragma unroll
             for (int i = 0; i < QP * NT; ++i)
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) sc[i % NT][kt] = Types<E>::mfma(bits<v8>(kr[kt][k]), qb[k & 1][i], sc[i % NT][kt]);
+                for (int kt = 0; kt < 2; ++kt) sc[i % NT][kt] = Types<E>::mfma(kf[kt], qb[k & 1][i], sc[i % NT][kt]);
         }
         __builtin_amdgcn_sched_group_barrier(0x100, QP * NT, 0);          // LDS reads
 #pragma unroll
@@ -611,9 +650,9 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int k = 0; k < KS; ++k) {
+                for (int k = 0; k < LD; ++k) {
                     if (slot[kt] < 0) vr[kt][k] = u32x4_t{0u, 0u, 0u, 0u};
-                    if (t * KT + kt * 16 + lr >= s.at.past) sp[kt] |= any_special<E>(vr[kt][k]);
+                    if (t * KT + kt * 16 + lr >= s.at.past) sp[kt] |= F8 ? f8_any_nan(vr[kt][k]) : any_special<E>(vr[kt][k]);
                 }
             uint64_t b0 = __ballot(sp[0]), b1 = __ballot(sp[1]);
             if (b0 | b1) {
@@ -623,13 +662,15 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                    for (int k = 0; k < KS; ++k) vr[kt][k] = special >> (kt * 16 + lr) & 1 ? u32x4_t{0u, 0u, 0u, 0u} : vr[kt][k];
+                    for (int k = 0; k < LD; ++k) vr[kt][k] = special >> (kt * 16 + lr) & 1 ? u32x4_t{0u, 0u, 0u, 0u} : vr[kt][k];
             }
         }
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int k = 0; k < KS; ++k) *reinterpret_cast<u32x4_t *>(v_at<D>(buf, kt * 16 + lr, 2 * k + (lg >> 1), lg & 1)) = vr[kt][k];
+            for (int k = 0; k < KS; ++k)
+                if constexpr (F8) *reinterpret_cast<u32x4_t *>(v_at<D>(buf, kt * 16 + lr, 4 * (k / 2) + lg, k % 2)) = operand_of<E, F8>(vr[kt], k);
+                else *reinterpret_cast<u32x4_t *>(v_at<D>(buf, kt * 16 + lr, 2 * k + (lg >> 1), lg & 1)) = vr[kt][k];
         // the next tile's rows, in flight from here
         if (t + W < s.t_end) {
             load(t + W);
@@ -637,7 +678,7 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
         }
         if (masked) rows.hide(sc, there, t * KT - s.at.past);
         rows.add(sc, buf);
-        if (special) rows.add_special(sc, special, t, s, pg);
+        if (special) rows.template add_special<P>(sc, special, t, s, pg);
     }
 
     rows.drop();
@@ -681,8 +722,10 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
 // More than 32 query rows: a wave has 32 of them (RW waves the block's 32 RW), and the RW waves share the K and V tiles, which
 // they bring into LDS together: the cache is read once for 64 or 128 rows. KW such teams take every KW-th tile. Two
 // buffers: a tile is written while the one before is multiplied and the one after is on its way from memory; one barrier a tile.
-template <class E, bool PAIR, int D, int RW, bool CUT>
+template <class E, bool PAIR, class P, int D, int RW, bool CUT>
 __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args a) {
+    constexpr bool F8 = sizeof(P) == 1;
+    typedef std::conditional_t<F8, u32x2_t, u32x4_t> Got;        // 8 elements of the pool; E in LDS
     constexpr int NT = 2, RWV = waves_of(PAIR, RW), KW = RWV / RW;
     typedef Rows<E, PAIR, D, NT> R;
     typedef typename R::v8 v8;
@@ -703,9 +746,9 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
 
     // staging: this lane's 16 bytes of rows rw KPW + i RPI + l / LPR of the tile
     const int c = l % LPR, r0 = rw * KPW + l / LPR;
-    u32x4_t kr[SI], vr[SI];
+    Got kr[SI], vr[SI];
     int slot[SI], page[SI];
-    const E *kb = static_cast<const E *>(a.k) + s.kvh * D + 8 * c, *vb = static_cast<const E *>(a.v) + s.kvh * D + 8 * c;
+    const P *kb = static_cast<const P *>(a.k) + s.kvh * D + 8 * c, *vb = static_cast<const P *>(a.v) + s.kvh * D + 8 * c;
     auto look_up = [&](int t) {
 #pragma unroll
         for (int i = 0; i < SI; ++i) page[i] = pg.page_of(t * KT + r0 + i * RPI);
@@ -715,8 +758,8 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
         for (int i = 0; i < SI; ++i) {
             slot[i] = pg.slot_of(t * KT + r0 + i * RPI, page[i]);
             const size_t at = static_cast<size_t>(max(slot[i], 0)) * a.ldkv;
-            kr[i] = *(const NAVI_GLOBAL u32x4_t *) (kb + at);
-            vr[i] = *(const NAVI_GLOBAL u32x4_t *) (vb + at);
+            kr[i] = *(const NAVI_GLOBAL Got *) (kb + at);
+            vr[i] = *(const NAVI_GLOBAL Got *) (vb + at);
         }
     };
     auto bits_of = [&](uint64_t b, int i) {                       // a ballot over load i's rows as bits of the tile's keys
@@ -724,6 +767,14 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
 #pragma unroll
         for (int r = 0; r < RPI; ++r) x |= static_cast<uint32_t>((b >> (r * LPR) & ((uint64_t(1) << LPR) - 1)) != 0) << r;
         return x << (rw * KPW + i * RPI);
+    };
+    auto as_e = [](const Got &g) {
+        if constexpr (F8) {
+            const u32x4_t one[1] = {u32x4_t{g[0], g[1], 0u, 0u}};
+            return operand_of<E, true>(one, 0);
+        } else {
+            return g;
+        }
     };
     auto put = [&](int b, int t) {
         unsigned char *kd = sm + (b * KW + kw) * 2 * TB, *vd = kd + TB;
@@ -737,17 +788,20 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
 #pragma unroll
             for (int i = 0; i < SI; ++i) {
                 there |= bits_of(__ballot(slot[i] >= 0), i);
-                vr[i] = slot[i] < 0 ? u32x4_t{0u, 0u, 0u, 0u} : vr[i];
-                const uint32_t x = bits_of(__ballot(t * KT + r0 + i * RPI >= s.at.past && any_special<E>(vr[i])), i);
+                vr[i] = slot[i] < 0 ? Got(0u) : vr[i];
+                bool odd;
+                if constexpr (F8) odd = f8_any_nan(u32x4_t{vr[i][0], vr[i][1], 0u, 0u});
+                else odd = any_special<E>(vr[i]);
+                const uint32_t x = bits_of(__ballot(t * KT + r0 + i * RPI >= s.at.past && odd), i);
                 special |= x;
-                vr[i] = x >> (r0 + i * RPI) & 1 ? u32x4_t{0u, 0u, 0u, 0u} : vr[i];
+                vr[i] = x >> (r0 + i * RPI) & 1 ? Got(0u) : vr[i];
             }
         }
 #pragma unroll
         for (int i = 0; i < SI; ++i) {
             const int r = r0 + i * RPI;
-            *reinterpret_cast<u32x4_t *>(kd + r * RB + ((c ^ (r & (LPR - 1))) << 4)) = kr[i];
-            *reinterpret_cast<u32x4_t *>(v_at<D>(vd, r, c >> 1, c & 1)) = vr[i];
+            *reinterpret_cast<u32x4_t *>(kd + r * RB + ((c ^ (r & (LPR - 1))) << 4)) = as_e(kr[i]);
+            *reinterpret_cast<u32x4_t *>(v_at<D>(vd, r, c >> 1, c & 1)) = as_e(vr[i]);
         }
         if (l == 0) {
             s_there[b][kw][rw] = there;
@@ -767,8 +821,8 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
     for (int nt = 0; nt < NT; ++nt) {
         v8 x[QP * KS];
         typename R::Raw raw;
-        R::fetch(a, s, qrow0 + nt * 16 + lr, raw);
-        rows.fac[nt] = R::operands(a, raw, x);
+        R::template fetch<false>(a, s, qrow0 + nt * 16 + lr, raw);
+        rows.fac[nt] = R::operands(a, score_factor(a, s.kvh), raw, x);
 #pragma unroll
         for (int i = 0; i < QP * KS; ++i)
             if (i < KS) q[nt][i] = x[i];
@@ -817,7 +871,7 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
         }
         if ((t + 1) * KT > s.at.past || there != 0xFFFFFFFFu) rows.hide(sc, there, t * KT - s.at.past);
         rows.add(sc, kd + TB);
-        if (special) rows.add_special(sc, special, t, s, pg);
+        if (special) rows.template add_special<P>(sc, special, t, s, pg);
     }
 
     rows.drop();
@@ -910,7 +964,7 @@ __global__ void __launch_bounds__(BT) k_tree_join(Args a, int group_rows) {
         }
         if (pl == 0) {
             const int mrow = qrow0 + r, j = div_by(a.heads_per, mrow), head = kvh * a.g + mrow - j * a.g;
-            const float inv = top == NONE ? 0.f : 1.f / sum;
+            const float inv = top == NONE ? 0.f : value_factor(a, kvh) / sum;
             store_out<E, PAIR>(a, wh.c0 + j, head * D + 8 * c, a.hkv * a.g * D, o[0] * inv);
             store_out<E, PAIR>(a, wh.c0 + j, head * D + 8 * c + 4, a.hkv * a.g * D, o[1] * inv);
         }
@@ -970,35 +1024,53 @@ size_t workspace(const navi_kv_pages &p, const navi_kv_heads &h, int max_keys) {
     return need;
 }
 
-template <class E, bool PAIR, int D, bool CUT>
+template <class E, bool PAIR, class P, int D, bool CUT>
 void launch_cut(const Args &a, const Cut &c, hipStream_t s) {
     const dim3 rbt(static_cast<unsigned>(waves_of(PAIR, c.waves) * WAVE));
     const dim3 grid(static_cast<unsigned>(CUT ? c.workers + a.n : a.n) * a.groups * a.hkv);
     const dim3 abt(alone_of(CUT) * WAVE);
-    if (c.tiles == 1) hipLaunchKernelGGL((k_tree<E, PAIR, D, 1, CUT>), grid, abt, 0, s, a);
-    else if (c.waves == 1) hipLaunchKernelGGL((k_tree<E, PAIR, D, 2, CUT>), grid, abt, 0, s, a);
-    else if (c.waves == 2) hipLaunchKernelGGL((k_tree_rows<E, PAIR, D, 2, CUT>), grid, rbt, 0, s, a);
-    else hipLaunchKernelGGL((k_tree_rows<E, PAIR, D, 4, CUT>), grid, rbt, 0, s, a);
+    if (c.tiles == 1) hipLaunchKernelGGL((k_tree<E, PAIR, P, D, 1, CUT>), grid, abt, 0, s, a);
+    else if (c.waves == 1) hipLaunchKernelGGL((k_tree<E, PAIR, P, D, 2, CUT>), grid, abt, 0, s, a);
+    else if (c.waves == 2) hipLaunchKernelGGL((k_tree_rows<E, PAIR, P, D, 2, CUT>), grid, rbt, 0, s, a);
+    else hipLaunchKernelGGL((k_tree_rows<E, PAIR, P, D, 4, CUT>), grid, rbt, 0, s, a);
 }
 
-template <class E, bool PAIR, int D>
+template <class E, bool PAIR, class P, int D>
 void launch_as(const Args &a, const Cut &c, hipStream_t s) {
-    if (c.workers == 0) return launch_cut<E, PAIR, D, false>(a, c, s);
-    launch_cut<E, PAIR, D, true>(a, c, s);
+    if (c.workers == 0) return launch_cut<E, PAIR, P, D, false>(a, c, s);
+    launch_cut<E, PAIR, P, D, true>(a, c, s);
     const unsigned units = static_cast<unsigned>(a.n) * a.groups * a.hkv;
     hipLaunchKernelGGL((k_tree_join<E, PAIR, D>), dim3(units, std::max(1u, std::min(static_cast<unsigned>(c.rows / NW), 1024u / units))), dim3(BT), 0, s,
                        a, c.rows);
 }
 
+template <int D>
+void launch_dim(const Args &a, const Cut &c, int q_dtype, int kv_dtype, hipStream_t s) {
+    const bool pair = q_dtype == NAVI_DT_F32, bf = q_dtype == NAVI_DT_BF16;
+    if (kv_dtype == NAVI_DT_F8E4M3) {
+        if (pair) launch_as<_Float16, true, f8_t, D>(a, c, s);
+        else if (bf) launch_as<__bf16, false, f8_t, D>(a, c, s);
+        else launch_as<_Float16, false, f8_t, D>(a, c, s);
+    } else {
+        if (pair) launch_as<_Float16, true, _Float16, D>(a, c, s);
+        else if (bf) launch_as<__bf16, false, __bf16, D>(a, c, s);
+        else launch_as<_Float16, false, _Float16, D>(a, c, s);
+    }
+}
+
 void launch(const Call &x, hipStream_t s) {
     const navi_kv_pages &p = *x.pages;
     const navi_kv_heads &h = *x.heads;
-    const bool pair = x.q_dtype == NAVI_DT_F32, bf = h.kv_dtype == NAVI_DT_BF16;
+    const bool pair = x.q_dtype == NAVI_DT_F32;
     const Cut c = cut_of(p, h, x.max_keys, pair);
     Args a{};
     a.q = x.q;
     a.k = x.k;
     a.v = x.v;
+    if (h.kv_dtype == NAVI_DT_F8E4M3) {
+        a.ks = h.k_scale;
+        a.vs = h.v_scale;
+    }
     a.out = x.out;
     a.po = static_cast<float *>(x.ws);
     if (a.po) {
@@ -1029,15 +1101,8 @@ void launch(const Call &x, hipStream_t s) {
     a.heads_per = kv::make_div(static_cast<uint32_t>(a.g));
     a.flip = x.scale < 0.f;
     a.scale = std::fabs(x.scale) * 1.44269504088896340736f;
-    if (h.head_dim == 128) {
-        if (pair) launch_as<_Float16, true, 128>(a, c, s);
-        else if (bf) launch_as<__bf16, false, 128>(a, c, s);
-        else launch_as<_Float16, false, 128>(a, c, s);
-    } else {
-        if (pair) launch_as<_Float16, true, 64>(a, c, s);
-        else if (bf) launch_as<__bf16, false, 64>(a, c, s);
-        else launch_as<_Float16, false, 64>(a, c, s);
-    }
+    if (h.head_dim == 128) launch_dim<128>(a, c, x.q_dtype, h.kv_dtype, s);
+    else launch_dim<64>(a, c, x.q_dtype, h.kv_dtype, s);
 }
 
 } // namespace tree
@@ -1061,8 +1126,10 @@ navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads 
     if (st == NAVI_OK) st = kv::check_heads("tree_attention", heads, ld_kv, err, errlen);
     if (st != NAVI_OK) return st;
     const long width = static_cast<long>(heads->n_head) * heads->head_dim;
-    if (q_dtype != heads->kv_dtype && !(q_dtype == NAVI_DT_F32 && heads->kv_dtype == NAVI_DT_F16)) {
-        set_err(err, errlen, "tree_attention: unsupported types (q %d, cache %d): the cache's type, or f32 over f16", q_dtype, heads->kv_dtype);
+    const bool known = heads->kv_dtype == NAVI_DT_F8E4M3 ? q_dtype == NAVI_DT_F32 || q_dtype == NAVI_DT_F16 || q_dtype == NAVI_DT_BF16
+                                                         : q_dtype == heads->kv_dtype || (q_dtype == NAVI_DT_F32 && heads->kv_dtype == NAVI_DT_F16);
+    if (!known) {
+        set_err(err, errlen, "tree_attention: unsupported types (q %d, cache %d): the cache's type, or f32 over f16, or any over e4m3", q_dtype, heads->kv_dtype);
         return NAVI_ERR_UNSUPPORTED;
     }
     if (pages->max_new > 64) {

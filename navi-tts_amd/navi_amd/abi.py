@@ -85,7 +85,7 @@ class KvView(C.Structure):
                 ("k", C.POINTER(C.c_void_p)), ("v", C.POINTER(C.c_void_p))]
 
 
-DT_F32, DT_F16, DT_BF16 = 0, 1, 2            # navi_dtype
+DT_F32, DT_F16, DT_BF16, DT_F8E4M3 = 0, 1, 2, 5            # navi_dtype
 
 
 class KvPages(C.Structure):
@@ -97,7 +97,9 @@ class KvPages(C.Structure):
 
 
 class KvHeads(C.Structure):
-    _fields_ = [("n_head", C.c_int32), ("n_kv_head", C.c_int32), ("head_dim", C.c_int32), ("kv_dtype", C.c_int32)]
+    """navi_kv_heads; k_scale, v_scale: device addresses of an e4m3 pool's factors a kv head (None: 1)."""
+    _fields_ = [("n_head", C.c_int32), ("n_kv_head", C.c_int32), ("head_dim", C.c_int32), ("kv_dtype", C.c_int32),
+                ("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
 
 
 class Sampling(C.Structure):
