@@ -372,6 +372,47 @@ size_t navi_tree_workspace(const navi_kv_pages *pages, const navi_kv_heads *head
 navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, const int32_t *d_path, int32_t max_path,
                            const int32_t *d_accept, int32_t *d_n_past_out, int32_t *d_status, void *stream, char *err,
                            size_t errlen);
+/* ---- a step's logits to its next codes: no counterpart in the reference, whose sampler is part of the frame -----------------
+ * Both enqueue on `stream` and return, as the four above; pointers named d_* are device memory of the library's device. */
+
+typedef struct {                       /* how a row's token is taken */
+    float   temperature;               /* not above 0, or NaN: the largest logit */
+    int32_t top_k;                     /* the first top_k tokens; below 1: all */
+    float   top_p;                     /* of these the fewest, from the first, whose probabilities reach top_p (one at least); not below 1: all */
+    float   min_p;                     /* of these the ones with at least min_p times the first one's probability; not above 0: all */
+    float   repetition_penalty;        /* seen tokens' logits are divided by it above 0, multiplied below (in f32); not above 0: off */
+} navi_sample_rule;
+
+/* A token for every row of logits (f32, f16 or bf16 [n_rows][vocab], stride ld >= vocab; any alignment of their type; vocab <= 2^20). Tokens stand in the
+ * order of their logits, the lowest index first among equals; a row's rule keeps a part of that order, with probabilities
+ * softmax(logit / temperature) over the tokens that top_k leaves for top_p, and over those that are left at the end for the draw: the token
+ * is the first, in the order of the indexes, at which the sum of the kept ones passes d_u[row] (0 <= u < 1; what is outside counts as the end of
+ * that range). Weights are computed and summed in 64 bits: rows give the same token whatever is sampled beside them. Tokens below 2^-63 of
+ * the first one's probability have none.
+ * d_rules: device [n_rules], n_rules 1 (for all rows) or n_rows. d_allowed: bits [n_rows][ld_allowed words], token i bit i % 32 of word i / 32; a token
+ * without its bit is left out, as are NaN and -infinity; +infinity counts as the largest finite number. d_seen: bits of the tokens that the repetition penalty
+ * applies to. Either may be NULL; a stride of 0: one set for all rows. A row without a token gets -1, and log probability -infinity.
+ * d_token[row * ld_token]; d_logprob [n_rows] (NULL: not wanted): log of the token's probability among those kept (0 without
+ * temperature). Results are none of the inputs. d_ws: navi_sample_workspace(n_rows, vocab) bytes, 16-byte aligned, for this call alone until it is
+ * done; none up to 16384 tokens. */
+navi_status navi_sample_rows(const void *d_logits, int32_t dtype, int32_t ld, int32_t n_rows, int32_t vocab, const navi_sample_rule *d_rules,
+                             int32_t n_rules, const float *d_u, const uint32_t *d_allowed, int32_t ld_allowed, const uint32_t *d_seen,
+                             int32_t ld_seen, int32_t *d_token, int32_t ld_token, float *d_logprob, void *d_ws, size_t ws_bytes, void *stream,
+                             char *err, size_t errlen);
+/* Workspace bytes of navi_sample_rows (host only; 0 where none is needed, or the arguments are not valid). */
+size_t navi_sample_workspace(int32_t n_rows, int32_t vocab);
+/* Which drafted rows the sampled codes confirm, for navi_kv_commit. Row r of a planned step was drafted to follow its parent (d_parent as
+ * navi_kv_plan's; NULL: the row before) with the n_codes codes of d_drafted row r (stride ld_drafted); the model has given the codes of d_sampled
+ * row r (stride ld_sampled) to follow it. From the last cached row on, whose sampled codes are d_last [n_requests][n_codes], the row of the lowest index that
+ * follows the one reached and was drafted with the codes sampled there is taken, until none is, or max_path (<= 64) are. d_last NULL: the first row that
+ * follows the cached ones is taken whatever its codes (it is what the request goes on with). A code below 0 equals none. Rows without a
+ * slot are not taken, nor any of a request with more than max_new (<= 64) rows or, with pages->status, one that the plan refused.
+ * d_path [n_requests][max_path]: the rows' indexes in the step, ascending, 0 past them; d_accept [n_requests]: how many; d_next [n_requests]
+ * [n_codes]: the codes sampled at the last one taken (none taken: d_last's, or -1): the next step's first row. d_next may be d_last; else the
+ * results are none of the inputs. */
+navi_status navi_draft_accept(const navi_kv_pages *pages, const int32_t *d_parent, const int32_t *d_drafted, int32_t ld_drafted, const int32_t *d_sampled,
+                              int32_t ld_sampled, int32_t n_codes, const int32_t *d_last, int32_t *d_path, int32_t max_path, int32_t *d_accept,
+                              int32_t *d_next, void *stream, char *err, size_t errlen);
 /* The talker over a planned step: the layers of navi_talker_prefill on the step's rows d_rows f32 [n_rows][hidden]
  * (drafted step inputs; one row a request is a decode step, a chain of 64 a piece of a prompt), each row seeing its
  * request's cached positions and its ancestors in the step. Stores the rows' K and V in the pages of every layer, and

@@ -42,7 +42,7 @@ EXPORTS = [
     "navi_streams_tap_hidden",
     "navi_streams_tap_logits", "navi_streams_tap_cp_logits",
     "navi_kv_plan", "navi_kv_append", "navi_kv_commit", "navi_tree_attention", "navi_tree_workspace",
-    "navi_talker_verify",
+    "navi_talker_verify", "navi_sample_rows", "navi_sample_workspace", "navi_draft_accept",
 ]
 
 
@@ -100,6 +100,12 @@ class KvHeads(C.Structure):
     """navi_kv_heads; k_scale, v_scale: device addresses of an e4m3 pool's factors a kv head (None: 1)."""
     _fields_ = [("n_head", C.c_int32), ("n_kv_head", C.c_int32), ("head_dim", C.c_int32), ("kv_dtype", C.c_int32),
                 ("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+
+
+class SampleRule(C.Structure):
+    """navi_sample_rule: how sample_rows takes a row's token (arrays of them live on the device)."""
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float),
+                ("repetition_penalty", C.c_float)]
 
 
 class Sampling(C.Structure):
@@ -279,6 +285,13 @@ def lib() -> C.CDLL:
                                       C.c_void_p, E, C.c_size_t]
     L.navi_tree_workspace.argtypes = [C.POINTER(KvPages), C.POINTER(KvHeads), C.c_int32]
     L.navi_tree_workspace.restype = C.c_size_t
+    L.navi_sample_rows.argtypes = [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p,
+                                   C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_size_t,
+                                   C.c_void_p, E, C.c_size_t]
+    L.navi_sample_workspace.argtypes = [C.c_int32, C.c_int32]
+    L.navi_sample_workspace.restype = C.c_size_t
+    L.navi_draft_accept.argtypes = [C.POINTER(KvPages), C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p,
+                                    C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, E, C.c_size_t]
     _lib = L
     return L
 
@@ -805,6 +818,28 @@ def kv_commit(pages: KvPages, k, v, ld_kv: int, path: int, max_path: int, accept
     view = KvView(n, pages.n_pages * pages.page_size, ld_kv, (C.c_void_p * n)(*k), (C.c_void_p * n)(*v))
     err = C.create_string_buffer(256)
     _check(lib().navi_kv_commit(pages, view, path, max_path, accept, n_past, status, stream, err, 256), err)
+
+
+def sample_workspace(n_rows: int, vocab: int) -> int:
+    """navi_sample_workspace: the bytes of workspace that sample_rows needs."""
+    return lib().navi_sample_workspace(n_rows, vocab)
+
+
+def sample_rows(logits: int, dtype: int, ld: int, n_rows: int, vocab: int, rules: int, n_rules: int, u: int, token: int, *, ld_token: int = 1,
+                logprob: int | None = None, allowed: int | None = None, ld_allowed: int = 0, seen: int | None = None, ld_seen: int = 0,
+                ws: int | None = None, ws_bytes: int = 0, stream: int | None = None):
+    """navi_sample_rows: a token for every row of logits, under the row's SampleRule and its number of u."""
+    err = C.create_string_buffer(256)
+    _check(lib().navi_sample_rows(logits, dtype, ld, n_rows, vocab, rules, n_rules, u, allowed, ld_allowed, seen, ld_seen, token, ld_token,
+                                  logprob, ws, ws_bytes, stream, err, 256), err)
+
+
+def draft_accept(pages: KvPages, drafted: int, ld_drafted: int, sampled: int, ld_sampled: int, n_codes: int, path: int, max_path: int,
+                 accept: int, next: int, *, parent: int | None = None, last: int | None = None, stream: int | None = None):
+    """navi_draft_accept: the drafted rows of each request that the sampled codes confirm, as kv_commit takes them."""
+    err = C.create_string_buffer(256)
+    _check(lib().navi_draft_accept(pages, parent, drafted, ld_drafted, sampled, ld_sampled, n_codes, last, path, max_path, accept, next, stream,
+                                   err, 256), err)
 
 
 # ---- vocoder ---------------------------------------------------------------------------
