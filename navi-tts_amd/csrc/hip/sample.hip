@@ -14,8 +14,8 @@
 //  * Then the kept weights are summed in the order of the indexes, and the wave that holds the border names the token.
 //
 // Up to 16384 tokens a block has its row in registers and does all of this in one launch. Longer rows are cut into chunks: a launch makes
-// the chunks' bins, a second copies the tokens of the bins in question, a third does the rest, reading again only the chunk that
-// the number falls into.
+// the chunks' bins, a second the rows', a third copies the tokens of the bins in question, a fourth does the rest, reading again only
+// the chunk that the number falls into.
 #include "host_util.h"
 #include "kv.h"
 #include "sampler.h"
@@ -35,7 +35,10 @@ constexpr int CAP = 8192;              // tokens of the bins in question that ar
 constexpr int ROW_MOST = 16384;        // tokens of a row that a block has in registers
 constexpr int MAXC = 64;               // most chunks of a row
 constexpr int PER = 16;                // tokens of a thread of a chunk
+constexpr int COPIES = 4;
+constexpr unsigned long long ONE = 1ull << 48;   // a token in a sum of weights
 
+struct Record;
 struct Args {
     const void *x;
     const navi_sample_rule *rules;
@@ -43,8 +46,11 @@ struct Args {
     const uint32_t *allowed, *seen;
     int32_t *token;
     float *logprob;
-    uint64_t *bins, *best, *list;      // the workspace (ws_of): [row][chunk][BINS], [row][chunk], [row][CAP]
-    int32_t *listed;                   // [row]
+    // the workspace (ws_of): the chunks' bins and largest keys, the rows' bins, and the keys to look at again
+    uint64_t *bins, *best, *sums, *list;
+    double *upto;
+    float *most;
+    Record *record;
     int rows, vocab, ld, n_rules, ld_allowed, ld_seen, ld_token, chunks;
 };
 
@@ -55,56 +61,60 @@ __device__ __forceinline__ int index_of(uint64_t key) { return static_cast<int>(
 
 struct Rule {
     double c4;                         // 4 log2 e / temperature
+    double inv;                        // 1 / c4
     double p, m;                       // top_p; log2 min_p
-    float penalty;
+    double over, times;                // what a seen token's logit is multiplied with above 0 and below
     int k;                             // 0: off, as p of 1 and m of -inf are
-    bool greedy;
+    bool greedy, penal;
     __device__ __forceinline__ bool cuts() const { return k > 0 || p < 1.0 || m != -INFINITY; }
+    // In 64 bits and rounded once: the product as it is, and the quotient too, since a quotient of two f32 lies at least 2^-49 of itself
+    // from the middle between two others (below 2^-126, where they are further apart than that, the last bit may differ).
+    __device__ __forceinline__ float seen(float v) const { return static_cast<float>(static_cast<double>(v) * (v > 0.f ? over : times)); }
 };
 __device__ __forceinline__ Rule rule_of(const Args &a, int row) {
     const navi_sample_rule *s = a.rules + (a.n_rules == 1 ? 0 : row);
     Rule r;
     const float t = gld(&s->temperature), p = gld(&s->top_p), m = gld(&s->min_p), pen = gld(&s->repetition_penalty);
     r.greedy = !(t > 0.f);
-    r.c4 = r.greedy ? 0.0 : 4.0 * 1.44269504088896340736 / static_cast<double>(t);
+    // above 0 even for an infinite temperature, so that it times -inf is no NaN, and times the least number not 0
+    r.c4 = r.greedy ? 1.0 : fmax(4.0 * 1.44269504088896340736 / static_cast<double>(t), 1e-60);
     r.k = max(gld(&s->top_k), 0);
+    r.inv = 1.0 / r.c4;
     r.p = p < 1.f ? fmax(static_cast<double>(p), 0.0) : 1.0;
-    r.m = m > 0.f ? log2(fmin(static_cast<double>(m), 1.0)) : -INFINITY;
-    r.penalty = pen > 0.f ? pen : 1.f;
+    r.m = -INFINITY;
+    if (m > 0.f) r.m = log2(fmin(static_cast<double>(m), 1.0));
+    r.penal = pen > 0.f && pen != 1.f;
+    r.times = static_cast<double>(pen);
+    r.over = 1.0 / r.times;
     return r;
 }
 
-// A row's logits as its rule sees them: -inf for what is not allowed, NaN and -inf; no -0; at most the largest finite number.
+// A row's logits: as they stand in memory, and as its rule sees them: -inf for what is not allowed, NaN and -inf; no -0; at most the
+// largest finite number.
 template <class T>
 struct Row {
     const T *x;
     const uint32_t *allowed, *seen;
-    float penalty;
     int vocab;
     bool vec;                          // four at a time are aligned
-    __device__ __forceinline__ Row(const Args &a, int row, float pen) {
+    __device__ __forceinline__ Row(const Args &a, int row) {
         x = static_cast<const T *>(a.x) + static_cast<size_t>(row) * a.ld;
         allowed = a.allowed ? a.allowed + static_cast<size_t>(row) * a.ld_allowed : nullptr;
-        seen = a.seen && pen != 1.f ? a.seen + static_cast<size_t>(row) * a.ld_seen : nullptr;
-        penalty = pen;
+        seen = a.seen ? a.seen + static_cast<size_t>(row) * a.ld_seen : nullptr;
         vocab = a.vocab;
         vec = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0;
     }
-    __device__ __forceinline__ float as_seen(float v, int i, uint32_t allow, uint32_t see) const {
-        if (see >> (i & 31) & 1u) v = v > 0.f ? v / penalty : v * penalty;
-        v = v != v ? -INFINITY : fminf(v, FLT_MAX) + 0.f;
-        return allow >> (i & 31) & 1u ? v : -INFINITY;
+    static __device__ __forceinline__ float number(float v) {
+        v = v > FLT_MAX ? FLT_MAX : v;
+        return (v == v ? v : -INFINITY) + 0.f;
     }
-    __device__ __forceinline__ float at(int i) const {
-        return as_seen(static_cast<float>(gld(x + i)), i, allowed ? gld(allowed + (i >> 5)) : ~0u, seen ? gld(seen + (i >> 5)) : 0u);
+    __device__ __forceinline__ float at(int i, const Rule &r) const {
+        float v = static_cast<float>(gld(x + i));
+        if (seen && r.penal && gld(seen + (i >> 5)) >> (i & 31) & 1u) v = r.seen(v);
+        return allowed && !(gld(allowed + (i >> 5)) >> (i & 31) & 1u) ? -INFINITY : number(v);
     }
     // tokens i .. i + 3, i a multiple of 4; -inf past the last
-    __device__ __forceinline__ void four(int i, float *v) const {
-        if (i >= vocab) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = -INFINITY;
-            return;
-        }
+    __device__ __forceinline__ void load(int i, float *v) const {
         if (vec && i + 4 <= vocab) {
             typedef T T4 __attribute__((ext_vector_type(4)));
             const T4 t = *(const NAVI_GLOBAL T4 *) (x + i);
@@ -114,25 +124,110 @@ struct Row {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = i + e < vocab ? static_cast<float>(gld(x + i + e)) : -INFINITY;
         }
-        const uint32_t allow = allowed ? gld(allowed + (i >> 5)) : ~0u, see = seen ? gld(seen + (i >> 5)) : 0u;
+    }
+    __device__ __forceinline__ void see(int i, float *v, const Rule &r) const {
+        if (seen && r.penal) {
+            const uint32_t w = i < vocab ? gld(seen + (i >> 5)) >> (i & 31) : 0u;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = as_seen(v[e], i + e, allow, see);
+            for (int e = 0; e < 4; ++e) v[e] = w >> e & 1u ? r.seen(v[e]) : v[e];
+        }
+        const uint32_t w = allowed && i < vocab ? gld(allowed + (i >> 5)) >> (i & 31) : 15u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = w >> e & 1u ? number(v[e]) : -INFINITY;
     }
 };
-
-// 2^(f / 4) for 0 <= f < 1: e^g about the middle, g = (f / 4 - 1 / 8) ln 2; the eighth power that is left out is 2^-43.
-__device__ __forceinline__ double quarter(double f) {
-    const double g = fma(f, 0.25 * 0.693147180559945309417, -0.125 * 0.693147180559945309417);
-    double s = 1.0 / 5040;
-    s = fma(s, g, 1.0 / 720);
-    s = fma(s, g, 1.0 / 120);
-    s = fma(s, g, 1.0 / 24);
-    s = fma(s, g, 1.0 / 6);
-    s = fma(s, g, 0.5);
-    s = fma(s, g, 1.0);
-    s = fma(s, g, 1.0);
-    return s * 1.09050773266525765921;                            // 2^(1 / 8)
+// Thread t's N tokens of a block's: 4 from i0 + 4 (k BT + t).
+template <int BT>
+__device__ __forceinline__ int token_at(int i0, int i) { return i0 + (i / 4 * BT + static_cast<int>(threadIdx.x)) * 4 + i % 4; }
+template <int BT, int N, class T>
+__device__ __forceinline__ void load_all(const Row<T> &x, int i0, float (&v)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; k += 4) x.load(token_at<BT>(i0, k), v + k);
 }
+template <int BT, int N, class T>
+__device__ __forceinline__ void see_all(const Row<T> &x, int i0, float (&v)[N], const Rule &r) {
+#pragma unroll
+    for (int k = 0; k < N; k += 4) x.see(token_at<BT>(i0, k), v + k, r);
+}
+
+// The largest key of a block's tokens, 0 without one, and for each part of a wave's (256 tokens) its largest logit. `index`: whether the key's
+// index is wanted (else that of some token).
+template <int BT, int PARTS>
+__device__ __forceinline__ uint64_t block_best(const float (&v)[4 * PARTS], int i0, float (&most)[PARTS], bool index, float *red, int *red_at) {
+    const int l = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) {
+        most[k] = wave_max(fmaxf(fmaxf(v[4 * k], v[4 * k + 1]), fmaxf(v[4 * k + 2], v[4 * k + 3])));
+        m = fmaxf(m, most[k]);
+    }
+    if (l == 0) red[wv] = m;
+    __syncthreads();
+    m = red[0];
+#pragma unroll
+    for (int i = 1; i < BT / WAVE; ++i) m = fmaxf(m, red[i]);
+    if (m == -INFINITY) return 0;
+    if (!index) return key_of(m, i0);
+    int at = INT32_MAX;
+#pragma unroll
+    for (int i = 4 * PARTS - 1; i >= 0; --i) at = v[i] == m ? token_at<BT>(i0, i) : at;
+    at = wave_min_int(at);
+    if (l == 0) red_at[wv] = at;
+    __syncthreads();
+    at = red_at[0];
+#pragma unroll
+    for (int i = 1; i < BT / WAVE; ++i) at = min(at, red_at[i]);
+    return key_of(m, at);
+}
+// The block's 4 BT PARTS tokens from i0 on into LDS as the rule sees them. A thread uses only those that it has put there (token_at) until the
+// next barrier.
+template <int BT, int PARTS, class T>
+__device__ __forceinline__ void keep(const float (&v)[4 * PARTS], float *xs) {
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) *reinterpret_cast<f32x4_t *>(xs + token_at<BT>(0, 4 * k)) = f32x4_t{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
+}
+
+// A weight over its bin's edge, 2^(f / 4) for 0 <= f < 1, in units of 2^-31 of the edge: a polynomial in f (Taylor's about the
+// middle, its seventh power 2^-37), rounded.
+constexpr double UNIT = 2147483648.0;
+constexpr double LN = 0.25 * 0.693147180559945309417;
+__device__ __forceinline__ double quarter(double f) {
+    const double g = f - 0.5;
+    constexpr double M = 1.09050773266525765921;                  // 2^(1 / 8)
+    constexpr double C1 = LN, C2 = C1 * LN / 2, C3 = C2 * LN / 3, C4 = C3 * LN / 4, C5 = C4 * LN / 5, C6 = C5 * LN / 6, C7 = C6 * LN / 7;
+    double s = C7 * M;
+    s = fma(s, g, C6 * M);
+    s = fma(s, g, C5 * M);
+    s = fma(s, g, C4 * M);
+    s = fma(s, g, C3 * M);
+    s = fma(s, g, C2 * M);
+    s = fma(s, g, C1 * M);
+    return fma(s, g, M);
+}
+// The constants in scalar registers: written as such, the compiler moves each into the sum's register first, three instructions a step.
+struct Units {
+    double c[7];
+    __device__ __forceinline__ Units() {
+        constexpr double M = 1.09050773266525765921 * UNIT;
+        constexpr double C1 = LN, C2 = C1 * LN / 2, C3 = C2 * LN / 3, C4 = C3 * LN / 4, C5 = C4 * LN / 5, C6 = C5 * LN / 6;
+        const double k[7] = {M + 0.5, C1 * M, C2 * M, C3 * M, C4 * M, C5 * M, C6 * M};
+#pragma unroll
+        for (int i = 0; i < 7; ++i) {
+            c[i] = k[i];
+            asm("" : "+s"(c[i]));
+        }
+    }
+    __device__ __forceinline__ uint32_t of(double f) const {
+        const double g = f - 0.5;
+        double s = fma(c[6], g, c[5]);
+        s = fma(s, g, c[4]);
+        s = fma(s, g, c[3]);
+        s = fma(s, g, c[2]);
+        s = fma(s, g, c[1]);
+        return static_cast<uint32_t>(fma(s, g, c[0]));
+    }
+};
+__device__ __forceinline__ uint32_t units(double f) { return Units().of(f); }
 // 2^(-j / 4)
 __device__ __forceinline__ double bin_edge(int j) {
     const double q[4] = {1.0, 0.840896415253714543031, 0.707106781186547524401, 0.594603557501360533359};
@@ -140,52 +235,102 @@ __device__ __forceinline__ double bin_edge(int j) {
     return ldexp(f, -(j >> 2));
 }
 
-constexpr double UNIT = 2147483648.0;  // 2^31: a weight at its bin's edge
-
-// A token's bin below the row's (or chunk's) first, BINS or more: none, and its weight over the bin's edge.
+// A token's bin below the row's (or chunk's) first, BINS: none of them, and its place in it.
 struct Place {
     int j;
-    double w;
+    double f;
 };
-__device__ __forceinline__ int bin_of(float x, double c4, double top) {
-    return x == -INFINITY ? BINS : static_cast<int>(fmin(top - floor(static_cast<double>(x) * c4), static_cast<double>(BINS)));
-}
 __device__ __forceinline__ Place place_of(float x, double c4, double top) {
-    const double q = static_cast<double>(x) * c4, b = floor(q);
-    Place p;
-    p.j = x == -INFINITY ? BINS : static_cast<int>(fmin(top - b, static_cast<double>(BINS)));
-    p.w = quarter(q - b);
-    return p;
+    const double q = static_cast<double>(x) * c4, b = floor(q);   // -inf: in no bin
+    return Place{static_cast<int>(fmin(top - b, static_cast<double>(BINS))), q - b};
 }
-__device__ __forceinline__ uint64_t units(double w) { return static_cast<uint64_t>(static_cast<uint32_t>(w * UNIT + 0.5)); }
+__device__ __forceinline__ int bin_of(float x, double c4, double top) { return place_of(x, c4, top).j; }
 
-__device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
-#pragma unroll
-    for (int o = 1; o < WAVE; o <<= 1) v = max(v, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(v), o)));
+// The least float key whose logit reaches a border: reaches(x) is true from some x on. One more than the largest's: none does. Halving from the
+// two keys beside the guess, which hold the border unless the guess is poor; 35 steps at most.
+constexpr uint32_t KEY_LEAST = 0x00800000u, KEY_MOST = 0xFF7FFFFFu;   // of -FLT_MAX and FLT_MAX
+template <class F>
+__device__ __forceinline__ uint32_t least_key(double guess, F reaches) {
+    const uint32_t k = float_key(static_cast<float>(fmin(fmax(guess, -static_cast<double>(FLT_MAX)), static_cast<double>(FLT_MAX))));
+    uint32_t lo = KEY_LEAST, hi = KEY_MOST + 1u;                  // the border lies within
+    auto probe = [&](uint32_t at) {
+        if (reaches(key_float(at))) hi = at;
+        else lo = at + 1u;
+    };
+    if (k - 2u > lo) probe(k - 2u);
+    if (k + 2u >= lo && k + 2u < hi) probe(k + 2u);
+    while (lo < hi) probe(lo + (hi - lo) / 2u);
+    return lo;
+}
+__device__ __forceinline__ uint32_t bin_start(int j, const Rule &r, double top) {
+    const double b = top - j;
+    return j < 0 ? KEY_MOST + 1u : least_key(b * r.inv, [&](float x) { return floor(static_cast<double>(x) * r.c4) >= b; });
+}
+// Keys from lo on, len of them.
+struct Keys {
+    uint64_t lo, len;
+    __device__ __forceinline__ bool have(uint64_t k) const { return k - lo < len; }
+};
+__device__ __forceinline__ Keys between(uint32_t lo, uint32_t hi) { return Keys{static_cast<uint64_t>(lo) << 32, static_cast<uint64_t>(hi - lo) << 32}; }
+// The least float key that min_p leaves (m > -inf).
+__device__ __forceinline__ uint32_t least_of(const Rule &r, double best4) {
+    return least_key((best4 + 4.0 * r.m) * r.inv, [&](float x) { return (static_cast<double>(x) * r.c4 - best4) * 0.25 >= r.m; });
+}
+
+// ---- 64 bits over a wave: DPP moves of both halves (dev_common.h has the patterns) --------------
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xF, false);
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+__device__ __forceinline__ uint64_t lane64(uint64_t v, int l) {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), l), hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), l);
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+__device__ __forceinline__ double as_double(uint64_t v) { return __longlong_as_double(static_cast<long long>(v)); }
+__device__ __forceinline__ uint64_t as_bits(double v) { return static_cast<uint64_t>(__double_as_longlong(v)); }
+__device__ __forceinline__ double lane_double(double v, int l) { return as_double(lane64(as_bits(v), l)); }
+
+// Inclusive sums over the lanes; what a move does not reach adds 0.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ void scan_step(double &v) { v += as_double(dpp64<CTRL, ROWS>(as_bits(v))); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ void scan_step(uint64_t &v) { v += dpp64<CTRL, ROWS>(v); }
+template <class V>
+__device__ __forceinline__ V wave_scan(V v) {
+    scan_step<0x111, 0xF>(v);
+    scan_step<0x112, 0xF>(v);
+    scan_step<0x114, 0xF>(v);
+    scan_step<0x118, 0xF>(v);
+    scan_step<0x142, 0xA>(v);
+    scan_step<0x143, 0xC>(v);
     return v;
 }
-__device__ __forceinline__ double wave_scan(double v) {           // inclusive
-    const int l = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < WAVE; o <<= 1) {
-        const double x = __shfl_up(v, o);
-        if (l >= o) v += x;
-    }
-    return v;
+__device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
+    v = max(v, dpp64<0x111, 0xF>(v));
+    v = max(v, dpp64<0x112, 0xF>(v));
+    v = max(v, dpp64<0x114, 0xF>(v));
+    v = max(v, dpp64<0x118, 0xF>(v));
+    v = max(v, dpp64<0x142, 0xA>(v));
+    v = max(v, dpp64<0x143, 0xC>(v));
+    return lane64(v, 63);
 }
 
 template <int BT>
 struct Lds {
     static constexpr int NW = BT / WAVE;
-    unsigned long long w[BINS];        // sums of the weights of the bins, then of a radix digit's tokens
-    unsigned n[BINS];                  // and their counts
-    double upto[BINS];                 // weights and counts of the bins up to each, in units of the first bin's edge
-    int count[BINS];
+    unsigned long long w[COPIES][BINS];    // sums of the bins' weights, counts above bit 48, by lane: fewer of an instruction meet; then of a digit's tokens
+    unsigned n[BINS];                  // counts that may pass 16 bits
     unsigned long long red[2][NW];
-    double seg[64], part[4];
-    int partn[4];
-    unsigned long long key;
-    int listed, kb, pb;
+    int count[NW];
+    float most[NW];
+    double seg[64];
+    unsigned long long few[WAVE];      // the tokens that are left to rank
+    uint32_t unit[WAVE];
+    unsigned long long key, sum;
+    int listed;
 };
 
 // The block's largest; `slot` 0 or 1 of red, free until the call after the next with the same one.
@@ -200,302 +345,366 @@ __device__ __forceinline__ uint64_t block_max(uint64_t v, Lds<BT> &q, int slot) 
     return m;
 }
 
-// upto and count from w and n.
-template <int BT>
-__device__ __forceinline__ void sum_bins(Lds<BT> &q) {
-    const int t = threadIdx.x, wv = t >> 6;
-    double w = 0.0;
-    int n = 0;
-    if (t < BINS) {
-        w = wave_scan(static_cast<double>(q.w[t]) * (bin_edge(t) / UNIT));
-        n = wave_incl_scan(static_cast<int>(q.n[t]));
-        if ((t & 63) == 63) {
-            q.part[wv] = w;
-            q.partn[wv] = n;
-        }
-    }
-    __syncthreads();
-    if (t < BINS) {
-        double before = 0.0;
-        int first = 0;
+// A row's bins in a wave's registers, lane l with bins 4 l .. 4 l + 3, and their sums: every wave looks for itself, without barriers.
+struct Edge {
+    int bin, count, own;               // BINS: none; the tokens before it, and in it
+    double before, upto;               // weights before it, and with it, in units of the first bin's edge
+};
+struct Bins {
+    int n[4], first;
+    double w[4], before, all;
+    int tokens;
+    __device__ __forceinline__ Bins(const int (&count)[4], const uint64_t (&mass)[4]) {
+        const int l = threadIdx.x & 63;
+        int c = 0;
+        double s = 0.0;
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            before += i < wv ? q.part[i] : 0.0;
-            first += i < wv ? q.partn[i] : 0;
+        for (int i = 0; i < 4; ++i) {
+            n[i] = count[i];
+            w[i] = static_cast<double>(mass[i]) * ldexp(bin_edge(i) / UNIT, -l);
+            c += n[i];
+            s += w[i];
         }
-        q.upto[t] = before + w;
-        q.count[t] = first + n;
+        first = wave_incl_scan(c) - c;
+        const double upto = wave_scan(s);
+        all = lane_double(upto, 63);
+        before = __shfl_up(upto, 1);
+        if (l == 0) before = 0.0;
+        tokens = __builtin_amdgcn_readlane(first + c, 63);
     }
-    __syncthreads();
-}
-
-// The bin in which a rule's top_k ends (BINS: it keeps all), and the one in which the weights up to it reach `mass`. All threads.
-template <int BT>
-__device__ __forceinline__ int bin_of_count(Lds<BT> &q, int k) {
-    const int t = threadIdx.x;
-    if (k < 1 || k >= q.count[BINS - 1]) return BINS;             // the same for all
-    if (t < BINS && q.count[t] >= k && (t == 0 || q.count[t - 1] < k)) q.kb = t;
-    __syncthreads();
-    return q.kb;
-}
-template <int BT>
-__device__ __forceinline__ int bin_of_mass(Lds<BT> &q, double mass) {
-    const int t = threadIdx.x;
-    __syncthreads();                                              // the readers of the call before are done
-    if (t < BINS) {
-        const int here = q.count[t], before = t ? q.count[t - 1] : 0;
-        if (here > before && (q.upto[t] >= mass || here == q.count[BINS - 1]) && (before == 0 || q.upto[t - 1] < mass)) q.pb = t;
+    // the bin in which the first k tokens end
+    __device__ __forceinline__ Edge of_count(int k) const {
+        Edge e{BINS, 0, 0, 0.0, all};
+        if (k < 1 || k >= tokens) return e;
+        int c = first, bin = -1, cb = 0, own = 0;
+        double s = before, sb = 0.0, su = 0.0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (c < k && c + n[i] >= k) { bin = 4 * static_cast<int>(threadIdx.x & 63) + i; cb = c; own = n[i]; sb = s; su = s + w[i]; }
+            c += n[i];
+            s += w[i];
+        }
+        return take(__builtin_ctzll(__ballot(bin >= 0)), bin, cb, own, sb, su);
     }
-    __syncthreads();
-    return q.pb;
-}
+    // the one in which the weights reach `mass`; where rounding keeps their sum below it, the last that has a token
+    __device__ __forceinline__ Edge of_mass(double mass) const {
+        int bin = -1, cb = 0, own = 0, last = -1, lc = 0, ln = 0, c = first;
+        double sb = 0.0, su = 0.0, lb = 0.0, lu = 0.0, s = before;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const double u = s + w[i];
+            if (n[i] > 0) {
+                last = 4 * static_cast<int>(threadIdx.x & 63) + i; lc = c; ln = n[i]; lb = s; lu = u;
+                if (bin < 0 && u >= mass) { bin = last; cb = c; own = n[i]; sb = s; su = u; }
+            }
+            c += n[i];
+            s = u;
+        }
+        const uint64_t hit = __ballot(bin >= 0);
+        if (hit) return take(__builtin_ctzll(hit), bin, cb, own, sb, su);
+        return take(63 - __builtin_clzll(__ballot(last >= 0)), last, lc, ln, lb, lu);
+    }
+    static __device__ __forceinline__ Edge take(int lane, int bin, int c, int own, double b, double u) {
+        return Edge{__builtin_amdgcn_readlane(bin, lane), __builtin_amdgcn_readlane(c, lane), __builtin_amdgcn_readlane(own, lane), lane_double(b, lane),
+                    lane_double(u, lane)};
+    }
+};
 
-// The bins whose tokens are looked at again: those in which top_k and min_p end, and p0 .. p1, in one of which top_p does.
+// The bins whose tokens are looked at again: the one in which top_k ends, and p0 .. p1, in one of which top_p does.
 struct Marks {
-    int kb, mb, p0, p1;
-    __device__ __forceinline__ bool any() const { return kb < BINS || mb < BINS || p0 <= p1; }
-    __device__ __forceinline__ bool has(int j) const { return j < BINS && (j == kb || j == mb || (j >= p0 && j <= p1)); }
+    Edge k;
+    int p0, p1, own;                   // own: the tokens in p0
+    __device__ __forceinline__ Marks(const Bins &b, const Rule &r) {
+        k = b.of_count(r.k);
+        p0 = BINS;
+        p1 = -1;
+        own = 0;
+        if (r.p < 1.0) {
+            const Edge e = b.of_mass(r.p * (k.bin < BINS ? k.before : b.all));
+            p0 = e.bin;
+            own = e.own;
+            p1 = k.bin < BINS ? b.of_mass(r.p * k.upto).bin : p0;
+        }
+    }
+    // whether the parts' sums are made of top_k's bin, and of top_p's if that is one: where the tokens are too many to rank at once
+    __device__ __forceinline__ bool fine_k() const { return k.bin < BINS && k.own > WAVE; }
+    __device__ __forceinline__ bool fine_p() const { return p0 == p1 && own > WAVE; }
+    __device__ __forceinline__ bool has(int j) const { return j < BINS && (j == k.bin || (j >= p0 && j <= p1)); }
 };
 
 // Tokens to look at again: keys in LDS, or, where they are too many, the row.
-struct List {
+template <class T, int BATCH>
+struct Tokens {
+    typedef uint64_t Batch[BATCH];
     const unsigned long long *key;
     int n;
-    template <int BT, class F>
-    __device__ __forceinline__ void each(F f) const {
-        for (int i = threadIdx.x; i < n; i += BT) f(static_cast<uint64_t>(key[i]));
-    }
-};
-template <class T>
-struct Whole {
+    bool held;
     const Row<T> &row;
+    const Rule &r;
+    double top;
+    // f(keys) of the thread's tokens, BATCH at a time (0: none), so that their loads and sums overlap
     template <int BT, class F>
     __device__ __forceinline__ void each(F f) const {
-        for (int i = threadIdx.x; i < row.vocab; i += BT) {
-            const float x = row.at(i);
-            if (x != -INFINITY) f(key_of(x, i));
-        }
-    }
-};
-
-// Of the tokens in bin `bin`, largest key first: the key at which their count reaches `need`, or (need 0) their weights' sum `mass` in
-// units. `sum`: the weights up to it and with it. A digit of 8 bits at a time, from the highest in which the keys differ, until one token is left.
-// q.w and q.n are used. All threads.
-template <int BT, class S>
-__device__ uint64_t select(const S &s, Lds<BT> &q, double c4, double top, int bin, int need, double mass, uint64_t &sum) {
-    const int t = threadIdx.x, l = t & 63;
-    uint64_t hi = 0, lo = 0;                                      // lo: of the complements
-    s.template each<BT>([&](uint64_t k) {
-        if (bin_of(logit_of(k), c4, top) == bin) {
-            hi = max(hi, k);
-            lo = max(lo, ~k);
-        }
-    });
-    __syncthreads();
-    hi = block_max(hi, q, 0);
-    lo = ~block_max(lo, q, 1);
-    sum = 0;
-    if (hi == 0) return 0;                                        // no token
-    int h = hi == lo ? 0 : 64 - __builtin_clzll(hi ^ lo);         // bits from h on are settled
-    uint64_t prefix = h < 64 ? hi >> h : 0;
-    if (h == 0) {
-        sum = units(place_of(logit_of(hi), c4, top).w);
-        return hi;
-    }
-    while (true) {
-        const int width = min(h, 8), at = h - width;
-        __syncthreads();
-        if (t < BINS) {
-            q.w[t] = 0;
-            q.n[t] = 0;
-        }
-        __syncthreads();
-        s.template each<BT>([&](uint64_t k) {
-            const Place p = place_of(logit_of(k), c4, top);
-            if (p.j != bin || (h < 64 ? k >> h : 0) != prefix) return;
-            const unsigned d = static_cast<unsigned>(k >> at) & ((1u << width) - 1u);
-            atomicAdd(&q.n[d], 1u);
-            atomicAdd(&q.w[d], static_cast<unsigned long long>(units(p.w)));
-        });
-        __syncthreads();
-        // lane l has digits 255 - 4 l .. 252 - 4 l; every wave finds the digit itself
-        int c[4], cs = 0;
-        uint64_t w[4], ws = 0;
+        const int end = held ? n : row.vocab;
+#pragma unroll 1
+        for (int i0 = threadIdx.x & ~63; i0 < end; i0 += BATCH * BT) {
+            Batch k;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            c[i] = static_cast<int>(q.n[255 - 4 * l - i]);
-            w[i] = q.w[255 - 4 * l - i];
-            cs += c[i];
-            ws += w[i];
-        }
-        int cb = wave_incl_scan(cs) - cs;
-        uint64_t wb = ws;
-#pragma unroll
-        for (int o = 1; o < WAVE; o <<= 1) {
-            const uint64_t x = __shfl_up(static_cast<unsigned long long>(wb), o);
-            if (l >= o) wb += x;
-        }
-        wb -= ws;
-        int d = -1, dc = 0, dn = 0, last = -1, lc = 0, ln = 0;
-        uint64_t dw = 0, db = 0, lw = 0, lb = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool reached = need > 0 ? cb + c[i] >= need : static_cast<double>(wb + w[i]) >= mass;
-            if (c[i] > 0) {
-                if (d < 0 && reached) { d = 255 - 4 * l - i; dc = cb; dn = c[i]; dw = w[i]; db = wb; }
-                last = 255 - 4 * l - i; lc = cb; ln = c[i]; lw = w[i]; lb = wb;
-            }
-            cb += c[i];
-            wb += w[i];
-        }
-        uint64_t hit = __ballot(d >= 0);
-        int src;
-        if (hit) {
-            src = __builtin_ctzll(hit);
-        } else {                                                  // the sum falls short of the mass by its rounding: the last one
-            src = 63 - __builtin_clzll(__ballot(last >= 0));
-            d = last; dc = lc; dn = ln; dw = lw; db = lb;
-        }
-        d = __shfl(d, src);
-        dn = __shfl(dn, src);
-        dc = __shfl(dc, src);
-        dw = __shfl(static_cast<unsigned long long>(dw), src);
-        db = __shfl(static_cast<unsigned long long>(db), src);
-        need -= need > 0 ? dc : 0;
-        mass -= static_cast<double>(db);
-        sum += db;
-        prefix = prefix << width | static_cast<uint64_t>(d);
-        h = at;
-        if (dn == 1 || h == 0) {
-            sum += dw;
-            if (h == 0) return prefix;
-            s.template each<BT>([&](uint64_t k) {
-                if (k >> h == prefix && bin_of(logit_of(k), c4, top) == bin) q.key = k;
-            });
-            __syncthreads();
-            return q.key;
-        }
-    }
-}
-
-// The last of the order that is kept: all bins before `bin`, and of it the keys from `key` on. bin BINS: all.
-struct Cut {
-    int bin;
-    uint64_t key;
-    __device__ __forceinline__ void narrow(int b, uint64_t k) {
-        if (b < bin || (b == bin && k > key)) {
-            bin = b;
-            key = k;
-        }
-    }
-    __device__ __forceinline__ bool keeps(int j, uint64_t k) const { return j < bin || (j == bin && k >= key); }
-};
-
-// From the bins' sums (sum_bins). best4: 4 c times the row's largest logit. All threads.
-template <int BT>
-__device__ __forceinline__ Marks marks_of(Lds<BT> &q, const Rule &r, double best4, double top) {
-    Marks k{bin_of_count(q, r.k), BINS, BINS, -1};
-    if (r.m != -INFINITY) k.mb = static_cast<int>(fmin(top - floor(best4 + 4.0 * r.m), static_cast<double>(BINS)));
-    if (r.p < 1.0) {
-        const double least = k.kb == BINS ? q.upto[BINS - 1] : k.kb ? q.upto[k.kb - 1] : 0.0, most = q.upto[min(k.kb, BINS - 1)];
-        k.p0 = bin_of_mass(q, r.p * least);
-        k.p1 = bin_of_mass(q, r.p * most);
-    }
-    return k;
-}
-
-// What a rule keeps, from the bins' sums and the tokens of the bins in question.
-template <int BT, class S>
-__device__ Cut cut_of(const S &s, Lds<BT> &q, const Rule &r, double best4, double top, const Marks &marks) {
-    const int kb = marks.kb, mb = marks.mb;
-    Cut cut{BINS, 0};
-    double all = q.upto[BINS - 1];
-    uint64_t sum;
-    if (kb < BINS) {
-        const double before = kb ? q.upto[kb - 1] : 0.0;
-        cut.narrow(kb, select(s, q, r.c4, top, kb, r.k - (kb ? q.count[kb - 1] : 0), 0.0, sum));
-        all = before + static_cast<double>(sum) * (bin_edge(kb) / UNIT);
-    }
-    if (r.p < 1.0) {
-        const double mass = r.p * all;
-        const int pb = min(max(bin_of_mass(q, mass), marks.p0), marks.p1);
-        const double before = pb ? q.upto[pb - 1] : 0.0;
-        cut.narrow(pb, select(s, q, r.c4, top, pb, 0, (mass - before) * (UNIT / bin_edge(pb)), sum));
-    }
-    if (mb < BINS) {
-        // the least key that reaches min_p, or, where none of the bin does, one more than all of them
-        uint64_t least = 0, most = 0;                             // least: of the complements
-        s.template each<BT>([&](uint64_t k) {
-            const float x = logit_of(k);
-            if (bin_of(x, r.c4, top) != mb) return;
-            most = max(most, k);
-            if ((static_cast<double>(x) * r.c4 - best4) * 0.25 >= r.m) least = max(least, ~k);
-        });
-        __syncthreads();
-        least = block_max(least, q, 0);
-        most = block_max(most, q, 1);
-        cut.narrow(mb, least ? ~least : most + 1);
-    }
-    return cut;
-}
-
-// The first token of the block's BT x N (from i0 on, in registers: thread t has 4 from i0 + 4 (k BT + t)) at which the kept weights'
-// sum passes `number` (FROM_U: that part of the sum); none passes it: the last kept one. `total`: the sum of all kept weights of the row, for the
-// log probability (FROM_U: the block's).
-template <int BT, int N, bool FROM_U>
-__device__ __forceinline__ void draw(const Args &a, int row, const float (&v)[N], int i0, Lds<BT> &q, const Rule &r, double top, const Cut &cut, double number,
-                                     double total) {
-    constexpr int K = N / 4, NW = BT / WAVE;
-    static_assert(K * NW <= 64, "a segment a lane");
-    const int t = threadIdx.x, l = t & 63, wv = t >> 6;
-    double own[K];
-    __syncthreads();
-    if (K * NW < 64 && t < 64) q.seg[t] = 0.0;
-    if (K * NW < 64) __syncthreads();
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        own[k] = 0.0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const Place p = place_of(v[4 * k + e], r.c4, top);
-            if (p.j < BINS && cut.keeps(p.j, key_of(v[4 * k + e], i0 + (k * BT + t) * 4 + e))) own[k] += p.w * bin_edge(p.j);
-        }
-        const double sum = wave_scan(own[k]);
-        if (l == 63) q.seg[k * NW + wv] = sum;
-    }
-    __syncthreads();
-    const double mine = q.seg[l], upto = wave_scan(mine);
-    if (FROM_U) {
-        total = __shfl(upto, 63);
-        number *= total;
-    }
-    const uint64_t past = __ballot(upto > number), some = __ballot(mine > 0.0);
-    if (!some) return;                                            // nothing is kept here
-    const int seg = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
-    if (seg % NW != wv) return;
-    const double before = seg ? __shfl(upto, seg - 1) : 0.0;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        if (seg / NW != k) continue;
-        const double sum = before + wave_scan(own[k]);
-        const uint64_t over = __ballot(own[k] > 0.0 && sum > number), any = __ballot(own[k] > 0.0);
-        const int lane = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
-        if (l == lane) {
-            double run = sum - own[k], weight = 0.0;
-            int pick = -1;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = i0 + (k * BT + t) * 4 + e;
-                const Place p = place_of(v[4 * k + e], r.c4, top);
-                if (p.j < BINS && cut.keeps(p.j, key_of(v[4 * k + e], i)) && (pick < 0 || run <= number)) {
-                    pick = i;
-                    weight = p.w * bin_edge(p.j);
-                    run += weight;
+            for (int j = 0; j < BATCH; ++j) {
+                const int i = i0 + j * BT + (threadIdx.x & 63);
+                k[j] = 0;
+                if (held) {
+                    if (i < end) k[j] = key[i];
+                } else if (i < end) {
+                    const float x = row.at(i, r);
+                    if (x != -INFINITY) k[j] = key_of(x, i);
                 }
             }
-            gst(a.token + static_cast<size_t>(row) * a.ld_token, pick);
-            if (a.logprob) gst(a.logprob + row, static_cast<float>(log(weight / total)));
+            f(k);
         }
+    }
+    __device__ __forceinline__ uint32_t units_of(uint64_t k) const { return units(place_of(logit_of(k), r.c4, top).f); }
+};
+
+// Of the n <= 64 keys q.few (weights q.unit), largest first: the one at which their count reaches `need`, or (need 0) their weights' sum `mass` in
+// units; none: the last. `sum`: plus the weights up to it and with it. Each key against all of them, BT / 64 lanes a key. All threads, after a barrier.
+template <int BT>
+__device__ __forceinline__ uint64_t rank(Lds<BT> &q, int n, int need, double mass, uint64_t &sum) {
+    constexpr int G = BT / WAVE;
+    static_assert(G == 4 || G == 8, "");
+    const int i = threadIdx.x / G;
+    const uint64_t key = i < n ? q.few[i] : 0;
+    int place = 0;
+    uint64_t before = 0;
+#pragma unroll 4
+    for (int j = threadIdx.x % G; j < n; j += G) {
+        const bool ahead = q.few[j] > key;
+        place += ahead;
+        before += ahead ? q.unit[j] : 0u;
+    }
+    auto all = [&](auto move) {                                   // the sum with the lanes that `move` takes from
+        place += static_cast<int>(move(static_cast<uint64_t>(place)));
+        before += move(before);
+    };
+    all([](uint64_t v) { return dpp64<0xB1, 0xF>(v); });          // quad_perm [1,0,3,2]
+    all([](uint64_t v) { return dpp64<0x4E, 0xF>(v); });          // quad_perm [2,3,0,1]
+    if (G == 8) all([](uint64_t v) { return dpp64<0x141, 0xF>(v); });   // row_half_mirror
+    const uint64_t upto = before + (key ? q.unit[i] : 0u);
+    const bool reached = need > 0 ? place == need - 1 : static_cast<double>(upto) >= mass && (place == 0 || static_cast<double>(before) < mass);
+    const bool last = place == n - 1 && (need > 0 ? need > n : static_cast<double>(upto) < mass);
+    if (threadIdx.x % G == 0 && key && (reached || last)) {
+        q.key = key;
+        q.sum = upto;
+    }
+    __syncthreads();
+    sum += n > 0 ? q.sum : 0;
+    return n > 0 ? q.key : 0;
+}
+
+// Sums of weights and counts of 256 parts of a marked bin's float keys, of 2^shift keys each; or null.
+struct Fine {
+    const uint64_t *sums;
+    int shift;
+};
+__device__ __forceinline__ int fine_shift(uint32_t len) { return len > 256u ? 24 - __builtin_clz(len - 1u) : 0; }
+
+// The digit in which the count reaches `need`, or (need 0) the weights `mass`; these and `sum` then without the digits above. Lane l has the counts and
+// weights of digits 255 - 4 l .. 252 - 4 l; every wave finds it for itself.
+__device__ __forceinline__ int digit_of(const int (&c)[4], const uint64_t (&w)[4], int &need, double &mass, uint64_t &sum) {
+    const int l = threadIdx.x & 63, cs = c[0] + c[1] + c[2] + c[3];
+    const uint64_t ws = w[0] + w[1] + w[2] + w[3];
+    int cb = wave_incl_scan(cs) - cs;
+    uint64_t wb = wave_scan(ws) - ws;
+    int d = -1, dc = 0, last = -1, lc = 0;
+    uint64_t db = 0, lb = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool reached = need > 0 ? cb + c[i] >= need : static_cast<double>(wb + w[i]) >= mass;
+        if (c[i] > 0) {
+            if (d < 0 && reached) { d = 255 - 4 * l - i; dc = cb; db = wb; }
+            last = 255 - 4 * l - i; lc = cb; lb = wb;
+        }
+        cb += c[i];
+        wb += w[i];
+    }
+    const uint64_t hit = __ballot(d >= 0);
+    int src;
+    if (hit) {
+        src = __builtin_ctzll(hit);
+    } else {                                                      // the sum falls short of the mass by its rounding: the last one
+        src = 63 - __builtin_clzll(__ballot(last >= 0));
+        d = last; dc = lc; db = lb;
+    }
+    need -= need > 0 ? __builtin_amdgcn_readlane(dc, src) : 0;
+    db = lane64(db, src);
+    mass -= static_cast<double>(db);
+    sum += db;
+    return __builtin_amdgcn_readlane(d, src);
+}
+
+// The same for the tokens of `in`; all threads. Up to 64 tokens every wave ranks for itself. More: the block narrows them by a digit of 8 bits, from
+// the highest in which their keys differ (f16 logits have few different values, and indexes few different bits), and looks
+// again. q.w, q.n and q.few are used.
+template <int BT, class S>
+__device__ __forceinline__ uint64_t select(const S &s, Lds<BT> &q, Keys in, const Fine &fine, int need, double mass, uint64_t &sum) {
+    const int t = threadIdx.x, l = t & 63;
+    sum = 0;
+    if (fine.sums) {
+        int c[4];
+        uint64_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = gld(fine.sums + 255 - 4 * l - i);
+            c[i] = static_cast<int>(gld(fine.sums + BINS + 255 - 4 * l - i));
+        }
+        const int d = digit_of(c, w, need, mass, sum);
+        in = Keys{in.lo + (static_cast<uint64_t>(d) << (32 + fine.shift)), uint64_t(1) << (32 + fine.shift)};
+    }
+    if (s.held && s.n <= WAVE) {
+        __syncthreads();                                          // the caller's readers of q are done
+        if (t < WAVE) {                                           // those of `in`, side by side
+            const uint64_t k = t < s.n ? static_cast<uint64_t>(s.key[t]) : 0;
+            const bool on = in.have(k);
+            const uint64_t m = __ballot(on);
+            if (on) {
+                const int at = __popcll(m & ((uint64_t(1) << t) - 1));
+                q.few[at] = k;
+                q.unit[at] = s.units_of(k);
+            }
+            if (t == 0) q.listed = __popcll(m);
+        }
+        __syncthreads();
+        return rank(q, q.listed, need, mass, sum);
+    }
+#pragma unroll 1
+    while (true) {
+        __syncthreads();                                          // what the round before, or the caller, has left here has been read
+        if (t == 0) q.listed = 0;
+        for (int i = t; i < COPIES * BINS; i += BT) q.w[0][i] = 0;
+        if (t < BINS) q.n[t] = 0;
+        uint64_t hi = 0, lo = 0;                                  // lo: of the complements
+        int n = 0;
+        s.template each<BT>([&](const typename S::Batch &k) {
+#pragma unroll
+            for (const uint64_t x : k) {
+                const bool on = in.have(x);
+                hi = max(hi, on ? x : 0);
+                lo = max(lo, on ? ~x : 0);
+                n += on;
+            }
+        });
+        hi = wave_max64(hi);
+        lo = wave_max64(lo);
+        n = wave_incl_scan(n);
+        if (l == 63) {
+            q.red[0][t >> 6] = hi;
+            q.red[1][t >> 6] = lo;
+            q.count[t >> 6] = n;
+        }
+        __syncthreads();
+        hi = lo = 0;
+        n = 0;
+#pragma unroll
+        for (int i = 0; i < Lds<BT>::NW; ++i) {
+            hi = max(hi, static_cast<uint64_t>(q.red[0][i]));
+            lo = max(lo, static_cast<uint64_t>(q.red[1][i]));
+            n += q.count[i];
+        }
+        lo = ~lo;
+        if (n <= WAVE) {
+            s.template each<BT>([&](const typename S::Batch &k) {
+#pragma unroll
+                for (const uint64_t x : k)
+                    if (in.have(x)) {
+                        const int at = atomicAdd(&q.listed, 1);
+                        q.few[at] = x;
+                        q.unit[at] = s.units_of(x);
+                    }
+            });
+            __syncthreads();
+            return rank(q, n, need, mass, sum);
+        }
+        const int h = 64 - __builtin_clzll(hi ^ lo), width = min(h, 8), at = h - width;   // bits from h on are alike
+        s.template each<BT>([&](const typename S::Batch &k) {
+#pragma unroll
+            for (const uint64_t x : k) {
+                if (!in.have(x)) continue;
+                const unsigned d = static_cast<unsigned>(x >> at) & ((1u << width) - 1u);
+                atomicAdd(&q.w[t & (COPIES - 1)][d], (s.held ? ONE : 0ull) + s.units_of(x));
+                if (!s.held) atomicAdd(&q.n[d], 1u);
+            }
+        });
+        __syncthreads();
+        int c[4];
+        uint64_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = 255 - 4 * l - i;
+            w[i] = 0;
+#pragma unroll
+            for (int j = 0; j < COPIES; ++j) w[i] += q.w[j][d];
+            c[i] = s.held ? static_cast<int>(w[i] >> 48) : static_cast<int>(q.n[d]);
+            if (s.held) w[i] &= ONE - 1;
+        }
+        const uint64_t above = h < 64 ? hi >> h << h : 0;
+        in = Keys{above | static_cast<uint64_t>(digit_of(c, w, need, mass, sum)) << at, uint64_t(1) << at};
+    }
+}
+
+// The last of the order that is kept: keys from `key` on, the last of them in `bin` (BINS: all are kept).
+struct Cut {
+    uint64_t key;
+    int bin;
+    __device__ __forceinline__ Cut() : key(static_cast<uint64_t>(KEY_LEAST) << 32), bin(BINS) {}
+    __device__ __forceinline__ void narrow(int b, uint64_t k) {
+        if (k > key) {
+            key = k;
+            bin = b;
+        }
+    }
+};
+
+// The float keys of the marked bins, a lane a border.
+struct Ranges {
+    uint32_t k0, k1, p0, p1;           // top_k's bin, top_p's bins: first key, one past the last
+    __device__ __forceinline__ Ranges(const Marks &m, const Rule &r, double top) {
+        const int l = threadIdx.x & 3, j = l == 0 ? m.k.bin : l == 1 ? m.k.bin - 1 : l == 2 ? m.p1 : m.p0 - 1;
+        const uint32_t start = bin_start(j, r, top);
+        k0 = __builtin_amdgcn_readlane(start, 0);
+        k1 = __builtin_amdgcn_readlane(start, 1);
+        p0 = __builtin_amdgcn_readlane(start, 2);
+        p1 = __builtin_amdgcn_readlane(start, 3);
+        if (m.k.bin >= BINS) k0 = k1 = 0u;
+        if (m.p0 > m.p1) p0 = p1 = 0u;
+    }
+    __device__ __forceinline__ bool has(uint32_t k) const { return k - k0 < k1 - k0 || k - p0 < p1 - p0; }
+};
+
+// What top_k and top_p keep, from the bins' sums and the tokens of the marked bins.
+template <int BT, class S>
+__device__ __forceinline__ void cut_tokens(Cut &cut, const S &s, Lds<BT> &q, const Rule &r, const Bins &bins, double top, const Marks &marks, const Ranges &ranges,
+                                           const uint64_t *fine) {
+    double all = bins.all;
+#pragma unroll 1
+    for (int by = 0; by < 2; ++by) {                              // top_k, then top_p of what it leaves: one copy of the code
+        if (by == 0 ? marks.k.bin >= BINS : r.p >= 1.0) continue;
+        Keys in = between(ranges.k0, ranges.k1);
+        int bin = marks.k.bin, need = r.k - marks.k.count;
+        double mass = 0.0;
+        if (by == 1) {
+            // between p0 and p1 whatever the rounding of the sums
+            mass = r.p * all;
+            Edge e = bins.of_mass(mass);
+            if (e.bin < marks.p0 || e.bin > marks.p1) e = bins.of_mass(r.p * (marks.k.bin < BINS ? marks.k.upto : bins.all));
+            bin = e.bin;
+            need = 0;
+            mass = (mass - e.before) * (UNIT / bin_edge(bin));
+            in = marks.p0 == marks.p1 ? between(ranges.p0, ranges.p1) : between(bin_start(bin, r, top), bin_start(bin - 1, r, top));
+        }
+        uint64_t sum;
+        const bool parts = fine && (by == 0 ? marks.fine_k() : marks.fine_p());
+        cut.narrow(bin, select(s, q, in, Fine{parts ? fine + by * 2 * BINS : nullptr, fine_shift(static_cast<uint32_t>(in.len >> 32))}, need, mass, sum));
+        if (by == 0) all = marks.k.before + static_cast<double>(sum) * (bin_edge(bin) / UNIT);
     }
 }
 
@@ -503,6 +712,75 @@ __device__ __forceinline__ void put(const Args &a, int row, int token, float log
     gst(a.token + static_cast<size_t>(row) * a.ld_token, token);
     if (a.logprob) gst(a.logprob + row, logprob);
 }
+
+// The first token of the 4 BT PARTS in LDS (from i0 on) at which the kept weights' sum passes `number` (FROM_U: that part of the sum); none
+// passes it: the last kept one. `total`: the sum of all kept weights of the row, for the log probability (FROM_U: of those here).
+template <int BT, int PARTS, bool FROM_U>
+__device__ __forceinline__ void draw(const Args &a, int row, const float *xs, int i0, Lds<BT> &q, const Rule &r, double top, const Cut &cut, double number,
+                                     double total) {
+    constexpr int NW = BT / WAVE;
+    static_assert(PARTS * NW <= 64, "a segment a lane");
+    const int t = threadIdx.x, l = t & 63, wv = t >> 6;
+    auto weight = [&](float x, int i) {                           // of token i, 0 where it is not kept
+        double w = 0.0;
+        if (key_of(x, i0 + i) >= cut.key) {
+            const Place p = place_of(x, r.c4, top);
+            if (p.j < BINS) w = quarter(p.f) * bin_edge(p.j);
+        }
+        return w;
+    };
+    auto four = [&](int k, f32x4_t &x) {                          // of the thread's four in part k
+        const int i = token_at<BT>(0, 4 * k);
+        x = *reinterpret_cast<const f32x4_t *>(xs + i);
+        double w = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w += weight(x[e], i + e);
+        return w;
+    };
+    f32x4_t x;
+    constexpr int AT_ONCE = PARTS < 4 ? PARTS : 4;                // that many parts' sums overlap
+#pragma unroll 1
+    for (int k = 0; k < PARTS; k += AT_ONCE) {
+        double sum[AT_ONCE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) sum[j] = four(k + j, x);
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            sum[j] = wave_scan(sum[j]);
+            if (l == 63) q.seg[(k + j) * NW + wv] = sum[j];
+        }
+    }
+    __syncthreads();
+    const double mine = l < PARTS * NW ? q.seg[l] : 0.0, upto = wave_scan(mine);
+    if (FROM_U) {
+        total = lane_double(upto, 63);
+        number *= total;
+    }
+    const uint64_t past = __ballot(upto > number), some = __ballot(mine > 0.0);
+    if (!some) return;                                            // nothing is kept here
+    const int seg = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+    if (seg % NW != wv) return;
+    const double before = seg ? lane_double(upto, seg - 1) : 0.0, log_total = a.logprob ? log(total) : 0.0;
+    const double own = four(seg / NW, x), sum = before + wave_scan(own);
+    const uint64_t over = __ballot(own > 0.0 && sum > number), any = __ballot(own > 0.0);
+    if (l != (over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any))) return;
+    double run = sum - own;
+    float y = 0.f;
+    int pick = -1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int i = token_at<BT>(0, 4 * (seg / NW)) + e;
+        const double w = weight(x[e], i);
+        if (w > 0.0 && (pick < 0 || run <= number)) {
+            pick = i0 + i;
+            y = x[e];
+            run += w;
+        }
+    }
+    // the logarithm of a weight is what it was made from
+    put(a, row, pick, static_cast<float>((static_cast<double>(y) * r.c4 - top) * LN - log_total));
+}
+
 __device__ __forceinline__ double number_of(const Args &a, int row) {
     const float u = gld(a.u + row);
     return u > 0.f ? static_cast<double>(fminf(u, 0x1.fffffep-1f)) : 0.0;
@@ -510,212 +788,380 @@ __device__ __forceinline__ double number_of(const Args &a, int row) {
 
 // ---- a row a block ---------------------------------------------------------------------------
 
-template <class T, int BT, int N>
+template <class T, int BT, int PARTS>
 __global__ void __launch_bounds__(BT) k_row(Args a) {
+    constexpr int MOST = 4 * BT * PARTS, HELD = MOST < CAP ? MOST : CAP;
     __shared__ Lds<BT> q;
-    constexpr int HELD = BT * N < CAP ? BT * N : CAP;
+    __shared__ __align__(16) float xs[MOST];
     __shared__ unsigned long long list[HELD];
-    const int row = blockIdx.x, t = threadIdx.x;
-    const Rule r = rule_of(a, row);
-    const Row<T> x(a, row, r.penalty);
-    float v[N];
-    uint64_t best = 0;
-    if (t < BINS) {
-        q.w[t] = 0;
-        q.n[t] = 0;
+    const int row = blockIdx.x, t = threadIdx.x, l = t & 63;
+    const Row<T> x(a, row);
+    uint64_t best;
+    Rule r;
+    double number;
+    {
+        float v[4 * PARTS];
+        load_all<BT>(x, 0, v);
+        number = number_of(a, row);
+        r = rule_of(a, row);
+        for (int i = t; i < COPIES * BINS; i += BT) q.w[0][i] = 0;
+        if (t == 0) q.listed = 0;
+        see_all<BT>(x, 0, v, r);
+        keep<BT, PARTS, T>(v, xs);
+        float most[PARTS];
+        best = block_best<BT, PARTS>(v, 0, most, r.greedy, q.most, q.count);
     }
-    if (t == 0) q.listed = 0;
-#pragma unroll
-    for (int k = 0; k < N / 4; ++k) x.four((k * BT + t) * 4, v + 4 * k);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (v[i] != -INFINITY) best = max(best, key_of(v[i], (i / 4 * BT + t) * 4 + i % 4));
-    best = block_max(best, q, 0);
     if (best == 0 || r.greedy) {
         if (t == 0) put(a, row, best ? index_of(best) : -1, best ? 0.f : -INFINITY);
         return;
     }
     const double best4 = static_cast<double>(logit_of(best)) * r.c4, top = floor(best4);
-    Cut cut{BINS, 0};
-    if (r.cuts()) {
+    Cut cut;
+    if (r.m != -INFINITY) cut.narrow(0, static_cast<uint64_t>(least_of(r, best4)) << 32);
+    if (r.k > 0 || r.p < 1.0) {
+        const Units un;
+#pragma unroll 2
+        for (int k = 0; k < PARTS; ++k) {
+            const f32x4_t v = *reinterpret_cast<const f32x4_t *>(xs + token_at<BT>(0, 4 * k));
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const Place p = place_of(v[i], r.c4, top);
-            if (p.j < BINS) atomicAdd(&q.w[p.j], 1ull << 48 | units(p.w));
-        }
-        __syncthreads();
-        if (t < BINS) {
-            q.n[t] = static_cast<unsigned>(q.w[t] >> 48);
-            q.w[t] &= (1ull << 48) - 1;
-        }
-        __syncthreads();
-        sum_bins(q);
-        const Marks marks = marks_of(q, r, best4, top);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (marks.has(bin_of(v[i], r.c4, top))) {
-                const int at = atomicAdd(&q.listed, 1);
-                if (at < HELD) list[at] = key_of(v[i], (i / 4 * BT + t) * 4 + i % 4);
+            for (int e = 0; e < 4; ++e) {
+                const Place p = place_of(v[e], r.c4, top);
+                if (p.j < BINS) atomicAdd(&q.w[t & (COPIES - 1)][p.j], ONE + un.of(p.f));
             }
         }
         __syncthreads();
-        if (q.listed <= HELD) cut = cut_of(List{list, q.listed}, q, r, best4, top, marks);
-        else cut = cut_of(Whole<T>{x}, q, r, best4, top, marks);
+        int n[4];
+        uint64_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = 0;
+#pragma unroll
+            for (int j = 0; j < COPIES; ++j) w[i] += q.w[j][4 * l + i];
+            n[i] = static_cast<int>(w[i] >> 48);
+            w[i] &= ONE - 1;
+        }
+        const Bins bins(n, w);
+        const Marks marks(bins, r);
+        const Ranges ranges(marks, r, top);
+#pragma unroll 2
+        for (int k = 0; k < PARTS; ++k) {
+            const int i = token_at<BT>(0, 4 * k);
+            const f32x4_t v = *reinterpret_cast<const f32x4_t *>(xs + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (ranges.has(float_key(v[e]))) {
+                    const int at = atomicAdd(&q.listed, 1);
+                    if (at < HELD) list[at] = key_of(v[e], i + e);
+                }
+        }
+        __syncthreads();
+        const int listed = q.listed;
+        cut_tokens(cut, Tokens<T, 2>{list, listed, listed <= HELD, x, r, top}, q, r, bins, top, marks, ranges, nullptr);
     }
-    draw<BT, N, true>(a, row, v, 0, q, r, top, cut, number_of(a, row), 0.0);
+    draw<BT, PARTS, true>(a, row, xs, 0, q, r, top, cut, number, 0.0);
 }
 
 // ---- a row in chunks -------------------------------------------------------------------------
 
+// What the launches tell each other about a row.
+struct Record {
+    uint64_t best;                     // its largest key
+    uint32_t lo[3], len[3];            // float keys of the marked bins (top_k's, top_p's, min_p's): lo .. lo + len - 1
+    int32_t listed, fine;              // keys copied; bit 0, 1: the sums of parts of top_k's bin, of top_p's, are wanted
+};
+
 // A chunk's bins below its own largest token's, and that token's key.
 template <class T, int BT>
 __global__ void __launch_bounds__(BT) k_bins(Args a) {
-    __shared__ unsigned long long w[4][BINS];
-    __shared__ Lds<BT> q;
+    constexpr int EIGHT = 8;           // copies of the bins
+    __shared__ unsigned long long w[EIGHT][BINS + 1];
     const int chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks, t = threadIdx.x, i0 = chunk * BT * PER;
-    const Rule r = rule_of(a, row);
-    const Row<T> x(a, row, r.penalty);
+    const Row<T> x(a, row);
     float v[PER];
-    for (int i = t; i < 4 * BINS; i += BT) w[i / BINS][i % BINS] = 0;
-    if (chunk == 0 && t == 0) gst(a.listed + row, 0);
-#pragma unroll
-    for (int k = 0; k < PER / 4; ++k) x.four(i0 + (k * BT + t) * 4, v + 4 * k);
-    uint64_t best = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-        if (v[i] != -INFINITY) best = max(best, key_of(v[i], i0 + (i / 4 * BT + t) * 4 + i % 4));
-    best = block_max(best, q, 0);
+    load_all<BT>(x, i0, v);
+    const Rule r = rule_of(a, row);
+    for (int i = t; i < EIGHT * (BINS + 1); i += BT) w[0][i] = 0;
+    see_all<BT>(x, i0, v, r);
+    __shared__ float red[BT / WAVE];
+    __shared__ int red_at[BT / WAVE];
+    float most[PER / 4];
+    const uint64_t best = block_best<BT, PER / 4>(v, i0, most, r.greedy, red, red_at);
     const size_t at = static_cast<size_t>(row) * a.chunks + chunk;
     if (t == 0) gst(a.best + at, best);
+    if ((t & 63) == 0) {
+#pragma unroll
+        for (int k = 0; k < PER / 4; ++k) gst(a.most + (at * (PER / 4) + k) * (BT / WAVE) + (t >> 6), most[k]);
+    }
     if (r.greedy) return;
     if (best) {
         const double top = floor(static_cast<double>(logit_of(best)) * r.c4);
+        const Units un;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const Place p = place_of(v[i], r.c4, top);
-            if (p.j < BINS) atomicAdd(&w[t & 3][p.j], 1ull << 48 | units(p.w));
+            if (p.j < BINS) atomicAdd(&w[t & (EIGHT - 1)][p.j], ONE + un.of(p.f));
         }
     }
     __syncthreads();
-    for (int i = t; i < BINS; i += BT) gst(a.bins + at * BINS + i, static_cast<uint64_t>(w[0][i] + w[1][i] + w[2][i] + w[3][i]));
+    for (int i = t; i < BINS; i += BT) {
+        unsigned long long sum = 0;
+#pragma unroll
+        for (int c = 0; c < EIGHT; ++c) sum += w[c][i];
+        gst(a.bins + at * BINS + i, static_cast<uint64_t>(sum));
+        // and the weights up to each bin, in units of the first one's edge
+        const double upto = wave_scan(static_cast<double>(sum & (ONE - 1)) * (bin_edge(i) / UNIT));
+        w[0][i] = as_bits(upto);
+    }
+    __syncthreads();
+    for (int i = t; i < BINS; i += BT) {
+        double before = 0.0;
+#pragma unroll
+        for (int j = 0; j < BINS / WAVE - 1; ++j) before += j < i / WAVE ? as_double(w[0][j * WAVE + WAVE - 1]) : 0.0;
+        gst(a.upto + at * BINS + i, before + as_double(w[0][i]));
+    }
 }
 
-// A row's largest token and its bins from its chunks'; q.w, q.n, upto and count are set where it is not greedy. false: no token.
-struct Merged {
-    uint64_t best;
-    double best4, top;
-};
-template <int BT>
-__device__ __forceinline__ Merged merge(const Args &a, int row, const Rule &r, Lds<BT> &q) {
-    const int t = threadIdx.x;
+// A row's bins from its chunks', in the wave's registers.
+__device__ __forceinline__ Bins bins_of(const Args &a, int row) {
+    const int l = threadIdx.x & 63;
+    const uint64_t *s = a.sums + static_cast<size_t>(row) * 6 * BINS;
+    int n[4];
+    uint64_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = gld(s + 4 * l + i);
+        n[i] = static_cast<int>(gld(s + BINS + 4 * l + i));
+    }
+    return Bins(n, w);
+}
+
+constexpr int MT = 1024;
+// The rows' bins and records.
+__global__ void __launch_bounds__(MT) k_rows(Args a) {
+    __shared__ Lds<MT> q;
+    const int row = blockIdx.x, t = threadIdx.x;
     const size_t at = static_cast<size_t>(row) * a.chunks;
+    // all chunks' bins on their way at once (of a greedy row: nothing of use); a chunk without a token has none
+    uint64_t got[MAXC * BINS / MT];
+#pragma unroll
+    for (int i = 0; i < MAXC * BINS / MT; ++i) got[i] = i * (MT / BINS) + t / BINS < a.chunks ? gld(a.bins + at * BINS + i * MT + t) : uint64_t(0);
+    const Rule r = rule_of(a, row);
     if (t < BINS) {
-        q.w[t] = 0;
+        q.w[0][t] = 0;
         q.n[t] = 0;
     }
-    Merged m;
-    m.best = block_max(t < a.chunks ? gld(a.best + at + t) : uint64_t(0), q, 0);
-    m.best4 = static_cast<double>(logit_of(m.best)) * r.c4;
-    m.top = floor(m.best4);
-    if (m.best == 0 || r.greedy) return m;
-    for (int i = t; i < a.chunks * BINS; i += BT) {
-        const uint64_t b = gld(a.best + at + i / BINS), x = gld(a.bins + at * BINS + i);
-        if (!b || !x) continue;
-        const double j = m.top - floor(static_cast<double>(logit_of(b)) * r.c4) + i % BINS;
+    const uint64_t best = block_max(t < a.chunks ? gld(a.best + at + t) : uint64_t(0), q, 0);
+    Record *rec = a.record + row;
+    if (t == 0) {
+        gst(&rec->best, best);
+        gst(&rec->listed, 0);
+    }
+    if (t < 3) gst(&rec->len[t], 0u);
+    if (t == 0) gst(&rec->fine, 0);
+    if (best == 0 || r.greedy) return;
+    const double best4 = static_cast<double>(logit_of(best)) * r.c4, top = floor(best4);
+#pragma unroll
+    for (int i = 0; i < MAXC * BINS / MT; ++i) {
+        if (i * (MT / BINS) >= a.chunks || !got[i]) continue;
+        const uint64_t b = gld(a.best + at + i * (MT / BINS) + t / BINS);
+        const double j = top - floor(static_cast<double>(logit_of(b)) * r.c4) + t % BINS;
         if (j < BINS) {
-            atomicAdd(&q.n[static_cast<int>(j)], static_cast<unsigned>(x >> 48));
-            atomicAdd(&q.w[static_cast<int>(j)], static_cast<unsigned long long>(x & ((1ull << 48) - 1)));
+            atomicAdd(&q.n[static_cast<int>(j)], static_cast<unsigned>(got[i] >> 48));
+            atomicAdd(&q.w[0][static_cast<int>(j)], static_cast<unsigned long long>(got[i] & (ONE - 1)));
         }
     }
     __syncthreads();
-    sum_bins(q);
-    return m;
+    uint64_t *s = a.sums + static_cast<size_t>(row) * 6 * BINS;   // weights, counts; the same of parts of top_k's bin; of top_p's
+    gst(s + 2 * BINS + t, uint64_t(0));
+    if (t < BINS) {
+        gst(s + t, static_cast<uint64_t>(q.w[0][t]));
+        gst(s + BINS + t, static_cast<uint64_t>(q.n[t]));
+    }
+    if (t >= WAVE || !r.cuts()) return;
+    int n[4];
+    uint64_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = q.w[0][4 * t + i];
+        n[i] = static_cast<int>(q.n[4 * t + i]);
+    }
+    const Bins bins(n, w);
+    const Marks m(bins, r);
+    if (t < 3) {
+        int first = t == 0 ? m.k.bin : m.p0, last = t == 0 ? m.k.bin : m.p1;
+        if (t == 2) first = last = r.m == -INFINITY ? BINS : bin_of(key_float(least_of(r, best4)), r.c4, top);
+        if (first < BINS && first <= last) {
+            const uint32_t lo = bin_start(last, r, top);
+            gst(&rec->lo[t], lo);
+            gst(&rec->len[t], bin_start(first - 1, r, top) - lo);
+        }
+        if (t == 0) gst(&rec->fine, (m.fine_k() ? 1 : 0) | (m.fine_p() ? 2 : 0));
+    }
 }
 
 // The tokens of the bins in question, in any order.
 template <class T, int BT>
 __global__ void __launch_bounds__(BT) k_list(Args a) {
-    __shared__ Lds<BT> q;
-    const int chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks, t = threadIdx.x, i0 = chunk * BT * PER;
-    const Rule r = rule_of(a, row);
-    if (r.greedy || !r.cuts()) return;
-    const Row<T> x(a, row, r.penalty);
-    const Merged m = merge(a, row, r, q);
-    if (m.best == 0) return;
-    const Marks marks = marks_of(q, r, m.best4, m.top);
-    if (!marks.any()) return;
+    constexpr int NW = BT / WAVE;
+    __shared__ int part[NW], s_at;
+    __shared__ unsigned long long w[2][BINS];                     // count above bit 48
+    const int chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks, t = threadIdx.x, l = t & 63, wv = t >> 6, i0 = chunk * BT * PER;
+    Record *rec = a.record + row;
+    uint32_t lo[3], len[3], least = ~0u;
+    const float *most = a.most + static_cast<size_t>(blockIdx.x) * (PER / 4) * NW + wv;
+    float top_of[PER / 4];
+#pragma unroll
+    for (int k = 0; k < PER / 4; ++k) top_of[k] = gld(most + k * NW);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        len[i] = gld(&rec->len[i]);
+        lo[i] = gld(&rec->lo[i]);
+        if (len[i]) least = min(least, lo[i]);
+    }
+    if (least == ~0u) return;
+    const Row<T> x(a, row);
     float v[PER];
+    // parts of a wave whose largest logit is below all marked bins are not read again
 #pragma unroll
-    for (int k = 0; k < PER / 4; ++k) x.four(i0 + (k * BT + t) * 4, v + 4 * k);
+    for (int k = 0; k < PER / 4; ++k) {
+        if (float_key(top_of[k]) >= least) {
+            x.load(token_at<BT>(i0, 4 * k), v + 4 * k);
+        } else {
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-        if (marks.has(bin_of(v[i], r.c4, m.top))) {
-            const int at = atomicAdd(a.listed + row, 1);
-            if (at < CAP) gst(a.list + static_cast<size_t>(row) * CAP + at, key_of(v[i], i0 + (i / 4 * BT + t) * 4 + i % 4));
+            for (int e = 0; e < 4; ++e) v[4 * k + e] = -INFINITY;
         }
+    }
+    const int fine = gld(&rec->fine);
+    const uint64_t best = gld(&rec->best);
+    const Rule r = rule_of(a, row);
+    for (int i = t; i < 2 * BINS; i += BT) w[0][i] = 0;
+    see_all<BT>(x, i0, v, r);
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const uint32_t k = float_key(v[i]);
+        mine |= static_cast<uint32_t>(k - lo[0] < len[0] || k - lo[1] < len[1] || k - lo[2] < len[2]) << i;
+    }
+    const int n = __popc(mine), upto = wave_incl_scan(n);
+    if (l == 63) part[wv] = upto;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        before += i < wv ? part[i] : 0;
+        all += part[i];
+    }
+    if (all == 0) return;
+    if (t == 0) s_at = atomicAdd(&rec->listed, all);
+    __syncthreads();
+    int at = s_at + before + upto - n;
+    const double top = floor(static_cast<double>(logit_of(best)) * r.c4);
+    const int s0 = fine_shift(len[0]), s1 = fine_shift(len[1]);
+    // few of a thread's tokens, read again: a loop over registers would be as long a piece of code as there are tokens
+#pragma unroll 1
+    for (; mine; mine &= mine - 1, ++at) {
+        const int i = token_at<BT>(i0, __builtin_ctz(mine));
+        const float y = x.at(i, r);
+        if (at < CAP) gst(a.list + static_cast<size_t>(row) * CAP + at, key_of(y, i));
+        if (!fine) continue;
+        const uint32_t k = float_key(y);
+        const unsigned long long one = ONE + units(place_of(y, r.c4, top).f);
+        if ((fine & 1) && k - lo[0] < len[0]) atomicAdd(&w[0][(k - lo[0]) >> s0], one);
+        if ((fine & 2) && k - lo[1] < len[1]) atomicAdd(&w[1][(k - lo[1]) >> s1], one);
+    }
+    if (!fine) return;
+    __syncthreads();
+    for (int i = t; i < 2 * BINS; i += BT) {
+        const unsigned long long y = w[0][i];
+        if (!y) continue;
+        unsigned long long *to = reinterpret_cast<unsigned long long *>(a.sums + (static_cast<size_t>(row) * 3 + 1 + i / BINS) * 2 * BINS + i % BINS);
+        atomicAdd(to, y & (ONE - 1));
+        atomicAdd(to + BINS, y >> 48);
+    }
 }
 
-constexpr int FT = 1024;
 // What is kept, the chunk into which the number falls, and the token. CHUNK: tokens of a chunk.
-template <class T, int CHUNK>
+template <class T, int CHUNK, int FT>
 __global__ void __launch_bounds__(FT) k_pick(Args a) {
+    constexpr int PARTS = CHUNK / (4 * FT);
     __shared__ Lds<FT> q;
-    __shared__ unsigned long long list[CAP];
+    __shared__ __align__(16) unsigned long long list[CAP];        // and then the chunk's logits
     __shared__ unsigned long long part[MAXC];                     // of the last kept bin, in units
-    __shared__ double mass[MAXC];
-    const int row = blockIdx.x, t = threadIdx.x, l = t & 63, wv = t >> 6;
+    static_assert(CAP * 8 >= CHUNK * 4, "");
+    float *xs = reinterpret_cast<float *>(list);
+    const int row = blockIdx.x, t = threadIdx.x, l = t & 63;
+    const uint64_t best = gld(&a.record[row].best);
+    const int n = gld(&a.record[row].listed);
+    const double u = number_of(a, row);
     const Rule r = rule_of(a, row);
-    const Merged m = merge(a, row, r, q);
-    if (m.best == 0 || r.greedy) {
-        if (t == 0) put(a, row, m.best ? index_of(m.best) : -1, m.best ? 0.f : -INFINITY);
+    if (best == 0 || r.greedy) {
+        if (t == 0) put(a, row, best ? index_of(best) : -1, best ? 0.f : -INFINITY);
         return;
     }
-    const Row<T> x(a, row, r.penalty);
-    const Marks marks = marks_of(q, r, m.best4, m.top);
-    const int n = marks.any() ? gld(a.listed + row) : 0;
+    const Row<T> x(a, row);
+    const double best4 = static_cast<double>(logit_of(best)) * r.c4, top = floor(best4);
+    const size_t at = static_cast<size_t>(row) * a.chunks;
+    const uint64_t own = l < a.chunks ? gld(a.best + at + l) : 0;   // a lane a chunk
     const bool held = n <= CAP;
     if (held)
         for (int i = t; i < n; i += FT) list[i] = gld(a.list + static_cast<size_t>(row) * CAP + i);
     if (t < MAXC) part[t] = 0;
+    Cut cut;
+    if (r.m != -INFINITY) {
+        const uint32_t k = least_of(r, best4);
+        cut.narrow(bin_of(key_float(k), r.c4, top), static_cast<uint64_t>(k) << 32);
+    }
     __syncthreads();
-    Cut cut{BINS, 0};
-    if (marks.any()) cut = held ? cut_of(List{list, n}, q, r, m.best4, m.top, marks) : cut_of(Whole<T>{x}, q, r, m.best4, m.top, marks);
+    if (r.k > 0 || r.p < 1.0) {
+        const Bins bins = bins_of(a, row);
+        const Marks marks(bins, r);
+        cut_tokens(cut, Tokens<T, 8>{list, n, held, x, r, top}, q, r, bins, top, marks, Ranges(marks, r, top), a.sums + (static_cast<size_t>(row) * 3 + 1) * 2 * BINS);
+    }
+    // the chunks' weights in the bins before the last kept one
+    const double first = top - floor(static_cast<double>(logit_of(own)) * r.c4);   // a chunk's first bin among the row's
+    const double upto_bin = static_cast<double>(cut.bin) - 1.0 - first;
+    double mine = own && upto_bin >= 0.0 ? gld(a.upto + (at + l) * BINS + min(static_cast<int>(upto_bin), BINS - 1)) : 0.0;
+    if (mine > 0.0) mine *= bin_edge(static_cast<int>(first));
     if (cut.bin < BINS) {
-        auto add = [&](uint64_t k) {
-            const Place p = place_of(logit_of(k), r.c4, m.top);
-            if (p.j == cut.bin && k >= cut.key) atomicAdd(&part[index_of(k) / CHUNK], static_cast<unsigned long long>(units(p.w)));
-        };
-        if (held) List{list, n}.each<FT>(add);
-        else Whole<T>{x}.template each<FT>(add);
-    }
-    __syncthreads();
-    // the chunks' kept weights, a wave a chunk
-    const size_t at = static_cast<size_t>(row) * a.chunks;
-    for (int c = wv; c < a.chunks; c += FT / WAVE) {
-        const uint64_t b = gld(a.best + at + c);
-        double sum = 0.0;
-        if (b) {
-            const double off = m.top - floor(static_cast<double>(logit_of(b)) * r.c4);
-#pragma unroll
-            for (int i = 0; i < BINS / WAVE; ++i) {
-                const double j = off + (i * WAVE + l);
-                if (j < cut.bin)
-                    sum += static_cast<double>(gld(a.bins + (at + c) * BINS + i * WAVE + l) & ((1ull << 48) - 1)) * (bin_edge(static_cast<int>(j)) / UNIT);
+        // and of that one's tokens those that are kept, chunk by chunk of a wave's: a chunk's lie side by side in the list
+        const Keys in = between(bin_start(cut.bin, r, top), bin_start(cut.bin - 1, r, top));
+        // tokens side by side to a thread, which adds up those of a chunk first
+        const int count = held ? n : a.vocab, share = (count + FT - 1) / FT, end = min(count, (t + 1) * share);
+        uint64_t run = 0;
+        int chunk = 0;
+        for (int i = t * share; i < end; ++i) {
+            uint64_t k;
+            if (held) {
+                k = list[i];
+            } else {
+                const float y = x.at(i, r);
+                k = y == -INFINITY ? 0 : key_of(y, i);
             }
+            if (!in.have(k) || k < cut.key) continue;
+            const int c = index_of(k) / CHUNK;
+            if (c != chunk) {
+                if (run) atomicAdd(&part[chunk], static_cast<unsigned long long>(run));
+                chunk = c;
+                run = 0;
+            }
+            run += units(place_of(logit_of(k), r.c4, top).f);
         }
-        sum = wave_scan(sum);
-        if (l == 63) mass[c] = sum + (cut.bin < BINS ? static_cast<double>(part[c]) * (bin_edge(cut.bin) / UNIT) : 0.0);
+        if (run) atomicAdd(&part[chunk], static_cast<unsigned long long>(run));
+        __syncthreads();
+        if (l < a.chunks) mine += static_cast<double>(part[l]) * (bin_edge(cut.bin) / UNIT);
     }
-    __syncthreads();
-    const double mine = l < a.chunks ? mass[l] : 0.0, upto = wave_scan(mine), total = __shfl(upto, 63), number = number_of(a, row) * total;
+    const double upto = wave_scan(mine), total = lane_double(upto, 63), number = u * total;
     const uint64_t past = __ballot(upto > number), some = __ballot(mine > 0.0);
     const int chunk = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
-    const double before = chunk ? __shfl(upto, chunk - 1) : 0.0;
-    constexpr int N = CHUNK / FT;
-    float v[N];
-#pragma unroll
-    for (int k = 0; k < N / 4; ++k) x.four(chunk * CHUNK + (k * FT + t) * 4, v + 4 * k);
-    draw<FT, N, false>(a, row, v, chunk * CHUNK, q, r, m.top, cut, number - before, total);
+    const double before = chunk ? lane_double(upto, chunk - 1) : 0.0;
+    __syncthreads();                                              // the list has been read
+    {
+        float v[4 * PARTS];
+        load_all<FT>(x, chunk * CHUNK, v);
+        see_all<FT>(x, chunk * CHUNK, v, r);
+        keep<FT, PARTS, T>(v, xs);
+    }
+    draw<FT, PARTS, false>(a, row, xs, chunk * CHUNK, q, r, top, cut, number - before, total);
 }
 
 // ---- launches --------------------------------------------------------------------------------
@@ -729,33 +1175,38 @@ int chunk_of(int rows, int vocab) {
 size_t workspace(int rows, int vocab) {
     if (vocab <= ROW_MOST || rows < 1) return 0;
     const int chunk = chunk_of(rows, vocab), chunks = (vocab + chunk - 1) / chunk;
-    return static_cast<size_t>(rows) * (static_cast<size_t>(chunks) * (BINS + 1) * 8 + CAP * 8 + 4);
+    return static_cast<size_t>(rows) * (static_cast<size_t>(chunks) * ((2 * BINS + 1) * 8 + chunk / 64) + (6 * BINS + CAP) * 8 + sizeof(Record));
 }
 
 template <class T>
 void launch(Args a, void *ws, hipStream_t s) {
     const dim3 rows(static_cast<unsigned>(a.rows));
-    if (a.vocab <= 1024) hipLaunchKernelGGL((k_row<T, 256, 4>), rows, dim3(256), 0, s, a);
-    else if (a.vocab <= 2048) hipLaunchKernelGGL((k_row<T, 256, 8>), rows, dim3(256), 0, s, a);
-    else if (a.vocab <= 4096) hipLaunchKernelGGL((k_row<T, 512, 8>), rows, dim3(512), 0, s, a);
-    else if (a.vocab <= 8192) hipLaunchKernelGGL((k_row<T, 1024, 8>), rows, dim3(1024), 0, s, a);
-    else if (a.vocab <= ROW_MOST) hipLaunchKernelGGL((k_row<T, 1024, 16>), rows, dim3(1024), 0, s, a);
+    if (a.vocab <= 1024) hipLaunchKernelGGL((k_row<T, 256, 1>), rows, dim3(256), 0, s, a);
+    else if (a.vocab <= 2048) hipLaunchKernelGGL((k_row<T, 256, 2>), rows, dim3(256), 0, s, a);
+    else if (a.vocab <= 4096) hipLaunchKernelGGL((k_row<T, 256, 4>), rows, dim3(256), 0, s, a);
+    else if (a.vocab <= 8192) hipLaunchKernelGGL((k_row<T, 512, 4>), rows, dim3(512), 0, s, a);
+    else if (a.vocab <= ROW_MOST) hipLaunchKernelGGL((k_row<T, 512, 8>), rows, dim3(512), 0, s, a);
     else {
         const int chunk = chunk_of(a.rows, a.vocab);
         a.chunks = (a.vocab + chunk - 1) / chunk;
         a.bins = static_cast<uint64_t *>(ws);
         a.best = a.bins + static_cast<size_t>(a.rows) * a.chunks * BINS;
-        a.list = a.best + static_cast<size_t>(a.rows) * a.chunks;
-        a.listed = reinterpret_cast<int32_t *>(a.list + static_cast<size_t>(a.rows) * CAP);
+        a.sums = a.best + static_cast<size_t>(a.rows) * a.chunks;
+        a.upto = reinterpret_cast<double *>(a.sums + static_cast<size_t>(a.rows) * 6 * BINS);
+        a.list = reinterpret_cast<uint64_t *>(a.upto + static_cast<size_t>(a.rows) * a.chunks * BINS);
+        a.record = reinterpret_cast<Record *>(a.list + static_cast<size_t>(a.rows) * CAP);
+        a.most = reinterpret_cast<float *>(a.record + a.rows);
         const dim3 grid(static_cast<unsigned>(a.rows) * a.chunks);
         if (chunk == 4096) {
             hipLaunchKernelGGL((k_bins<T, 256>), grid, dim3(256), 0, s, a);
+            hipLaunchKernelGGL(k_rows, rows, dim3(MT), 0, s, a);
             hipLaunchKernelGGL((k_list<T, 256>), grid, dim3(256), 0, s, a);
-            hipLaunchKernelGGL((k_pick<T, 4096>), rows, dim3(FT), 0, s, a);
+            hipLaunchKernelGGL((k_pick<T, 4096, 512>), rows, dim3(512), 0, s, a);
         } else {
             hipLaunchKernelGGL((k_bins<T, 1024>), grid, dim3(1024), 0, s, a);
+            hipLaunchKernelGGL(k_rows, rows, dim3(MT), 0, s, a);
             hipLaunchKernelGGL((k_list<T, 1024>), grid, dim3(1024), 0, s, a);
-            hipLaunchKernelGGL((k_pick<T, 16384>), rows, dim3(FT), 0, s, a);
+            hipLaunchKernelGGL((k_pick<T, 16384, 512>), rows, dim3(512), 0, s, a);
         }
     }
 }
