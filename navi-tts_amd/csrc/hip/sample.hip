@@ -34,7 +34,6 @@ constexpr int BINS = 256;
 constexpr int CAP = 8192;              // tokens of the bins in question that are kept in LDS; more are read from the row again
 constexpr int ROW_MOST = 16384;        // tokens of a row that a block has in registers
 constexpr int MAXC = 64;               // most chunks of a row
-constexpr int PER = 16;                // tokens of a thread of a chunk
 constexpr int COPIES = 4;
 constexpr unsigned long long ONE = 1ull << 48;   // a token in a sum of weights
 
@@ -55,7 +54,7 @@ struct Args {
 };
 
 // A token's place in the order as a number, the first the largest. 0 comes after all of them.
-__device__ __forceinline__ uint64_t key_of(float x, int i) { return static_cast<uint64_t>(float_key(x)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(i)); }
+__device__ __forceinline__ uint64_t key_of(float x, int i) { return static_cast<uint64_t>(float_key(x + 0.f)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(i)); }
 __device__ __forceinline__ float logit_of(uint64_t key) { return key_float(static_cast<unsigned>(key >> 32)); }
 __device__ __forceinline__ int index_of(uint64_t key) { return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key)); }
 
@@ -89,8 +88,8 @@ __device__ __forceinline__ Rule rule_of(const Args &a, int row) {
     return r;
 }
 
-// A row's logits: as they stand in memory, and as its rule sees them: -inf for what is not allowed, NaN and -inf; no -0; at most the
-// largest finite number.
+// A row's logits: as they stand in memory, and as its rule sees them: -inf for what is not allowed, NaN and -inf; at most the
+// largest finite number. (-0 is ordered as 0: key_of.)
 template <class T>
 struct Row {
     const T *x;
@@ -104,10 +103,7 @@ struct Row {
         vocab = a.vocab;
         vec = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0;
     }
-    static __device__ __forceinline__ float number(float v) {
-        v = v > FLT_MAX ? FLT_MAX : v;
-        return (v == v ? v : -INFINITY) + 0.f;
-    }
+    static __device__ __forceinline__ float number(float v) { return v == v ? __builtin_amdgcn_fmed3f(v, -INFINITY, FLT_MAX) : -INFINITY; }
     __device__ __forceinline__ float at(int i, const Rule &r) const {
         float v = static_cast<float>(gld(x + i));
         if (seen && r.penal && gld(seen + (i >> 5)) >> (i & 31) & 1u) v = r.seen(v);
@@ -187,8 +183,8 @@ __device__ __forceinline__ void keep(const float (&v)[4 * PARTS], float *xs) {
     for (int k = 0; k < PARTS; ++k) *reinterpret_cast<f32x4_t *>(xs + token_at<BT>(0, 4 * k)) = f32x4_t{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
 }
 
-// A weight over its bin's edge, 2^(f / 4) for 0 <= f < 1, in units of 2^-31 of the edge: a polynomial in f (Taylor's about the
-// middle, its seventh power 2^-37), rounded.
+// A weight over its bin's edge, 2^(f / 4) for 0 <= f < 1: Taylor's polynomial about the middle, its eighth power 2^-43. In units of 2^-31 and
+// rounded: one through Chebyshev's points, 2^-35 at most from it, its mean 2^-40.
 constexpr double UNIT = 2147483648.0;
 constexpr double LN = 0.25 * 0.693147180559945309417;
 __device__ __forceinline__ double quarter(double f) {
@@ -204,27 +200,26 @@ __device__ __forceinline__ double quarter(double f) {
     s = fma(s, g, C1 * M);
     return fma(s, g, M);
 }
-// The constants in scalar registers: written as such, the compiler moves each into the sum's register first, three instructions a step.
+// The constants in registers that the compiler takes as they come: written as such, it moves each into the sum's register first, three
+// instructions a step.
 struct Units {
-    double c[7];
+    double c[6];
     __device__ __forceinline__ Units() {
-        constexpr double M = 1.09050773266525765921 * UNIT;
-        constexpr double C1 = LN, C2 = C1 * LN / 2, C3 = C2 * LN / 3, C4 = C3 * LN / 4, C5 = C4 * LN / 5, C6 = C5 * LN / 6;
-        const double k[7] = {M + 0.5, C1 * M, C2 * M, C3 * M, C4 * M, C5 * M, C6 * M};
+        const double k[6] = {0.9999999999802172 * UNIT + 0.5, 0.1732867965638913 * UNIT,    0.015014140101979987 * UNIT,
+                             0.0008673221940371589 * UNIT,    3.743580564591298e-05 * UNIT, 1.4203366711186339e-06 * UNIT};
 #pragma unroll
-        for (int i = 0; i < 7; ++i) {
+        for (int i = 0; i < 6; ++i) {
             c[i] = k[i];
-            asm("" : "+s"(c[i]));
+            if (i < 5) asm("" : "+s"(c[i]));
+            else asm("" : "+v"(c[i]));
         }
     }
     __device__ __forceinline__ uint32_t of(double f) const {
-        const double g = f - 0.5;
-        double s = fma(c[6], g, c[5]);
-        s = fma(s, g, c[4]);
-        s = fma(s, g, c[3]);
-        s = fma(s, g, c[2]);
-        s = fma(s, g, c[1]);
-        return static_cast<uint32_t>(fma(s, g, c[0]));
+        double s = fma(c[5], f, c[4]);
+        s = fma(s, f, c[3]);
+        s = fma(s, f, c[2]);
+        s = fma(s, f, c[1]);
+        return static_cast<uint32_t>(fma(s, f, c[0]));
     }
 };
 __device__ __forceinline__ uint32_t units(double f) { return Units().of(f); }
@@ -276,6 +271,19 @@ __device__ __forceinline__ Keys between(uint32_t lo, uint32_t hi) { return Keys{
 __device__ __forceinline__ uint32_t least_of(const Rule &r, double best4) {
     return least_key((best4 + 4.0 * r.m) * r.inv, [&](float x) { return (static_cast<double>(x) * r.c4 - best4) * 0.25 >= r.m; });
 }
+
+// Adds a token to its bin, if it has one. The instructions are what bounds a pass over a row: 16 a token and its atomic. (The conversion
+// takes numbers past its range to its ends; so written, since C++ leaves them undefined.)
+struct Adder {
+    double c4, top;
+    Units un;
+    __device__ __forceinline__ void add(unsigned long long *w, float x) const {
+        const double q = static_cast<double>(x) * c4, b = floor(q), d = top - b;
+        int j;
+        asm("v_cvt_i32_f64 %0, %1" : "=v"(j) : "v"(d));
+        if (static_cast<unsigned>(j) < BINS) atomicAdd(w + j, ONE + un.of(q - b));
+    }
+};
 
 // ---- 64 bits over a wave: DPP moves of both halves (dev_common.h has the patterns) --------------
 
@@ -508,45 +516,50 @@ struct Fine {
 };
 __device__ __forceinline__ int fine_shift(uint32_t len) { return len > 256u ? 24 - __builtin_clz(len - 1u) : 0; }
 
-// The digit in which the count reaches `need`, or (need 0) the weights `mass`; these and `sum` then without the digits above. Lane l has the counts and
-// weights of digits 255 - 4 l .. 252 - 4 l; every wave finds it for itself.
-__device__ __forceinline__ int digit_of(const int (&c)[4], const uint64_t (&w)[4], int &need, double &mass, uint64_t &sum) {
+// The digit in which the count reaches `need`, or (need 0) the weights `mass`; these and `sum` then without the digits above, n: its count. Lane l has
+// the counts and weights of digits 255 - 4 l .. 252 - 4 l; every wave finds it for itself.
+__device__ __forceinline__ int digit_of(const int (&c)[4], const uint64_t (&w)[4], int &n, int &need, double &mass, uint64_t &sum) {
     const int l = threadIdx.x & 63, cs = c[0] + c[1] + c[2] + c[3];
     const uint64_t ws = w[0] + w[1] + w[2] + w[3];
     int cb = wave_incl_scan(cs) - cs;
     uint64_t wb = wave_scan(ws) - ws;
-    int d = -1, dc = 0, last = -1, lc = 0;
+    int d = -1, dc = 0, dn = 0, last = -1, lc = 0, ln = 0;
     uint64_t db = 0, lb = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const bool reached = need > 0 ? cb + c[i] >= need : static_cast<double>(wb + w[i]) >= mass;
         if (c[i] > 0) {
-            if (d < 0 && reached) { d = 255 - 4 * l - i; dc = cb; db = wb; }
-            last = 255 - 4 * l - i; lc = cb; lb = wb;
+            if (d < 0 && reached) { d = 255 - 4 * l - i; dc = cb; dn = c[i]; db = wb; }
+            last = 255 - 4 * l - i; lc = cb; ln = c[i]; lb = wb;
         }
         cb += c[i];
         wb += w[i];
     }
     const uint64_t hit = __ballot(d >= 0);
+    const uint64_t any = __ballot(last >= 0);
     int src;
     if (hit) {
         src = __builtin_ctzll(hit);
+    } else if (!any) {
+        n = 0;
+        return 0;
     } else {                                                      // the sum falls short of the mass by its rounding: the last one
-        src = 63 - __builtin_clzll(__ballot(last >= 0));
-        d = last; dc = lc; db = lb;
+        src = 63 - __builtin_clzll(any);
+        d = last; dc = lc; dn = ln; db = lb;
     }
     need -= need > 0 ? __builtin_amdgcn_readlane(dc, src) : 0;
     db = lane64(db, src);
     mass -= static_cast<double>(db);
     sum += db;
+    n = __builtin_amdgcn_readlane(dn, src);
     return __builtin_amdgcn_readlane(d, src);
 }
 
-// The same for the tokens of `in`; all threads. Up to 64 tokens every wave ranks for itself. More: the block narrows them by a digit of 8 bits, from
-// the highest in which their keys differ (f16 logits have few different values, and indexes few different bits), and looks
-// again. q.w, q.n and q.few are used.
+// The same as rank for the n tokens of `in`; all threads. Up to 64 are ranked. More: first by the fine sums, if there are any; then the block narrows
+// them by a digit of 8 bits, from the highest in which their keys differ (f16 logits have few different values, and indexes few
+// different bits). q.w, q.n and q.few are used.
 template <int BT, class S>
-__device__ __forceinline__ uint64_t select(const S &s, Lds<BT> &q, Keys in, const Fine &fine, int need, double mass, uint64_t &sum) {
+__device__ __forceinline__ uint64_t select(const S &s, Lds<BT> &q, Keys in, int n, const Fine &fine, int need, double mass, uint64_t &sum) {
     const int t = threadIdx.x, l = t & 63;
     sum = 0;
     if (fine.sums) {
@@ -557,73 +570,38 @@ __device__ __forceinline__ uint64_t select(const S &s, Lds<BT> &q, Keys in, cons
             w[i] = gld(fine.sums + 255 - 4 * l - i);
             c[i] = static_cast<int>(gld(fine.sums + BINS + 255 - 4 * l - i));
         }
-        const int d = digit_of(c, w, need, mass, sum);
+        const int d = digit_of(c, w, n, need, mass, sum);
         in = Keys{in.lo + (static_cast<uint64_t>(d) << (32 + fine.shift)), uint64_t(1) << (32 + fine.shift)};
     }
-    if (s.held && s.n <= WAVE) {
-        __syncthreads();                                          // the caller's readers of q are done
-        if (t < WAVE) {                                           // those of `in`, side by side
-            const uint64_t k = t < s.n ? static_cast<uint64_t>(s.key[t]) : 0;
-            const bool on = in.have(k);
-            const uint64_t m = __ballot(on);
-            if (on) {
-                const int at = __popcll(m & ((uint64_t(1) << t) - 1));
-                q.few[at] = k;
-                q.unit[at] = s.units_of(k);
-            }
-            if (t == 0) q.listed = __popcll(m);
-        }
-        __syncthreads();
-        return rank(q, q.listed, need, mass, sum);
-    }
 #pragma unroll 1
-    while (true) {
+    while (n > WAVE) {
         __syncthreads();                                          // what the round before, or the caller, has left here has been read
-        if (t == 0) q.listed = 0;
         for (int i = t; i < COPIES * BINS; i += BT) q.w[0][i] = 0;
         if (t < BINS) q.n[t] = 0;
         uint64_t hi = 0, lo = 0;                                  // lo: of the complements
-        int n = 0;
         s.template each<BT>([&](const typename S::Batch &k) {
 #pragma unroll
             for (const uint64_t x : k) {
                 const bool on = in.have(x);
                 hi = max(hi, on ? x : 0);
                 lo = max(lo, on ? ~x : 0);
-                n += on;
             }
         });
         hi = wave_max64(hi);
         lo = wave_max64(lo);
-        n = wave_incl_scan(n);
         if (l == 63) {
             q.red[0][t >> 6] = hi;
             q.red[1][t >> 6] = lo;
-            q.count[t >> 6] = n;
         }
         __syncthreads();
         hi = lo = 0;
-        n = 0;
 #pragma unroll
         for (int i = 0; i < Lds<BT>::NW; ++i) {
             hi = max(hi, static_cast<uint64_t>(q.red[0][i]));
             lo = max(lo, static_cast<uint64_t>(q.red[1][i]));
-            n += q.count[i];
         }
         lo = ~lo;
-        if (n <= WAVE) {
-            s.template each<BT>([&](const typename S::Batch &k) {
-#pragma unroll
-                for (const uint64_t x : k)
-                    if (in.have(x)) {
-                        const int at = atomicAdd(&q.listed, 1);
-                        q.few[at] = x;
-                        q.unit[at] = s.units_of(x);
-                    }
-            });
-            __syncthreads();
-            return rank(q, n, need, mass, sum);
-        }
+        if (hi <= lo) break;                                      // one token, or (where the counts cannot be right) none
         const int h = 64 - __builtin_clzll(hi ^ lo), width = min(h, 8), at = h - width;   // bits from h on are alike
         s.template each<BT>([&](const typename S::Batch &k) {
 #pragma unroll
@@ -647,8 +625,24 @@ __device__ __forceinline__ uint64_t select(const S &s, Lds<BT> &q, Keys in, cons
             if (s.held) w[i] &= ONE - 1;
         }
         const uint64_t above = h < 64 ? hi >> h << h : 0;
-        in = Keys{above | static_cast<uint64_t>(digit_of(c, w, need, mass, sum)) << at, uint64_t(1) << at};
+        in = Keys{above | static_cast<uint64_t>(digit_of(c, w, n, need, mass, sum)) << at, uint64_t(1) << at};
     }
+    __syncthreads();
+    if (t == 0) q.listed = 0;
+    __syncthreads();
+    s.template each<BT>([&](const typename S::Batch &k) {
+#pragma unroll
+        for (const uint64_t x : k)
+            if (in.have(x)) {
+                const int at = atomicAdd(&q.listed, 1);
+                if (at < WAVE) {                                  // as many as there are
+                    q.few[at] = x;
+                    q.unit[at] = s.units_of(x);
+                }
+            }
+    });
+    __syncthreads();
+    return rank(q, min(q.listed, WAVE), need, mass, sum);
 }
 
 // The last of the order that is kept: keys from `key` on, the last of them in `bin` (BINS: all are kept).
@@ -678,6 +672,7 @@ struct Ranges {
         if (m.p0 > m.p1) p0 = p1 = 0u;
     }
     __device__ __forceinline__ bool has(uint32_t k) const { return k - k0 < k1 - k0 || k - p0 < p1 - p0; }
+    __device__ __forceinline__ uint32_t least() const { return min(k0 < k1 ? k0 : ~0u, p0 < p1 ? p0 : ~0u); }
 };
 
 // What top_k and top_p keep, from the bins' sums and the tokens of the marked bins.
@@ -689,7 +684,7 @@ __device__ __forceinline__ void cut_tokens(Cut &cut, const S &s, Lds<BT> &q, con
     for (int by = 0; by < 2; ++by) {                              // top_k, then top_p of what it leaves: one copy of the code
         if (by == 0 ? marks.k.bin >= BINS : r.p >= 1.0) continue;
         Keys in = between(ranges.k0, ranges.k1);
-        int bin = marks.k.bin, need = r.k - marks.k.count;
+        int bin = marks.k.bin, n = marks.k.own, need = r.k - marks.k.count;
         double mass = 0.0;
         if (by == 1) {
             // between p0 and p1 whatever the rounding of the sums
@@ -697,13 +692,14 @@ __device__ __forceinline__ void cut_tokens(Cut &cut, const S &s, Lds<BT> &q, con
             Edge e = bins.of_mass(mass);
             if (e.bin < marks.p0 || e.bin > marks.p1) e = bins.of_mass(r.p * (marks.k.bin < BINS ? marks.k.upto : bins.all));
             bin = e.bin;
+            n = e.own;
             need = 0;
             mass = (mass - e.before) * (UNIT / bin_edge(bin));
             in = marks.p0 == marks.p1 ? between(ranges.p0, ranges.p1) : between(bin_start(bin, r, top), bin_start(bin - 1, r, top));
         }
         uint64_t sum;
         const bool parts = fine && (by == 0 ? marks.fine_k() : marks.fine_p());
-        cut.narrow(bin, select(s, q, in, Fine{parts ? fine + by * 2 * BINS : nullptr, fine_shift(static_cast<uint32_t>(in.len >> 32))}, need, mass, sum));
+        cut.narrow(bin, select(s, q, in, n, Fine{parts ? fine + by * 2 * BINS : nullptr, fine_shift(static_cast<uint32_t>(in.len >> 32))}, need, mass, sum));
         if (by == 0) all = marks.k.before + static_cast<double>(sum) * (bin_edge(bin) / UNIT);
     }
 }
@@ -819,15 +815,12 @@ __global__ void __launch_bounds__(BT) k_row(Args a) {
     Cut cut;
     if (r.m != -INFINITY) cut.narrow(0, static_cast<uint64_t>(least_of(r, best4)) << 32);
     if (r.k > 0 || r.p < 1.0) {
-        const Units un;
+        const Adder to{r.c4, top, Units()};
 #pragma unroll 2
         for (int k = 0; k < PARTS; ++k) {
             const f32x4_t v = *reinterpret_cast<const f32x4_t *>(xs + token_at<BT>(0, 4 * k));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const Place p = place_of(v[e], r.c4, top);
-                if (p.j < BINS) atomicAdd(&q.w[t & (COPIES - 1)][p.j], ONE + un.of(p.f));
-            }
+            for (int e = 0; e < 4; ++e) to.add(q.w[t & (COPIES - 1)], v[e]);
         }
         __syncthreads();
         int n[4];
@@ -847,6 +840,7 @@ __global__ void __launch_bounds__(BT) k_row(Args a) {
         for (int k = 0; k < PARTS; ++k) {
             const int i = token_at<BT>(0, 4 * k);
             const f32x4_t v = *reinterpret_cast<const f32x4_t *>(xs + i);
+            if (float_key(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]))) < ranges.least()) continue;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (ranges.has(float_key(v[e]))) {
@@ -871,7 +865,7 @@ struct Record {
 };
 
 // A chunk's bins below its own largest token's, and that token's key.
-template <class T, int BT>
+template <class T, int BT, int PER>
 __global__ void __launch_bounds__(BT) k_bins(Args a) {
     constexpr int EIGHT = 8;           // copies of the bins
     __shared__ unsigned long long w[EIGHT][BINS + 1];
@@ -894,13 +888,9 @@ __global__ void __launch_bounds__(BT) k_bins(Args a) {
     }
     if (r.greedy) return;
     if (best) {
-        const double top = floor(static_cast<double>(logit_of(best)) * r.c4);
-        const Units un;
+        const Adder to{r.c4, floor(static_cast<double>(logit_of(best)) * r.c4), Units()};
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const Place p = place_of(v[i], r.c4, top);
-            if (p.j < BINS) atomicAdd(&w[t & (EIGHT - 1)][p.j], ONE + un.of(p.f));
-        }
+        for (int i = 0; i < PER; ++i) to.add(w[t & (EIGHT - 1)], v[i]);
     }
     __syncthreads();
     for (int i = t; i < BINS; i += BT) {
@@ -1000,7 +990,7 @@ __global__ void __launch_bounds__(MT) k_rows(Args a) {
 }
 
 // The tokens of the bins in question, in any order.
-template <class T, int BT>
+template <class T, int BT, int PER>
 __global__ void __launch_bounds__(BT) k_list(Args a) {
     constexpr int NW = BT / WAVE;
     __shared__ int part[NW], s_at;
@@ -1023,24 +1013,24 @@ __global__ void __launch_bounds__(BT) k_list(Args a) {
     float v[PER];
     // parts of a wave whose largest logit is below all marked bins are not read again
 #pragma unroll
-    for (int k = 0; k < PER / 4; ++k) {
-        if (float_key(top_of[k]) >= least) {
-            x.load(token_at<BT>(i0, 4 * k), v + 4 * k);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * k + e] = -INFINITY;
-        }
-    }
+    for (int k = 0; k < PER / 4; ++k)
+        if (float_key(top_of[k]) >= least) x.load(token_at<BT>(i0, 4 * k), v + 4 * k);
     const int fine = gld(&rec->fine);
     const uint64_t best = gld(&rec->best);
     const Rule r = rule_of(a, row);
     for (int i = t; i < 2 * BINS; i += BT) w[0][i] = 0;
-    see_all<BT>(x, i0, v, r);
     uint32_t mine = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const uint32_t k = float_key(v[i]);
-        mine |= static_cast<uint32_t>(k - lo[0] < len[0] || k - lo[1] < len[1] || k - lo[2] < len[2]) << i;
+    for (int k = 0; k < PER / 4; ++k) {
+        if (float_key(top_of[k]) < least) continue;
+        float *f = v + 4 * k;
+        x.see(token_at<BT>(i0, 4 * k), f, r);
+        if (!__ballot(float_key(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]))) >= least)) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t y = float_key(f[e]);
+            mine |= static_cast<uint32_t>(y - lo[0] < len[0] || y - lo[1] < len[1] || y - lo[2] < len[2]) << (4 * k + e);
+        }
     }
     const int n = __popc(mine), upto = wave_incl_scan(n);
     if (l == 63) part[wv] = upto;
@@ -1198,14 +1188,14 @@ void launch(Args a, void *ws, hipStream_t s) {
         a.most = reinterpret_cast<float *>(a.record + a.rows);
         const dim3 grid(static_cast<unsigned>(a.rows) * a.chunks);
         if (chunk == 4096) {
-            hipLaunchKernelGGL((k_bins<T, 256>), grid, dim3(256), 0, s, a);
+            hipLaunchKernelGGL((k_bins<T, 256, 16>), grid, dim3(256), 0, s, a);
             hipLaunchKernelGGL(k_rows, rows, dim3(MT), 0, s, a);
-            hipLaunchKernelGGL((k_list<T, 256>), grid, dim3(256), 0, s, a);
+            hipLaunchKernelGGL((k_list<T, 256, 16>), grid, dim3(256), 0, s, a);
             hipLaunchKernelGGL((k_pick<T, 4096, 512>), rows, dim3(512), 0, s, a);
         } else {
-            hipLaunchKernelGGL((k_bins<T, 1024>), grid, dim3(1024), 0, s, a);
+            hipLaunchKernelGGL((k_bins<T, 512, 32>), grid, dim3(512), 0, s, a);
             hipLaunchKernelGGL(k_rows, rows, dim3(MT), 0, s, a);
-            hipLaunchKernelGGL((k_list<T, 1024>), grid, dim3(1024), 0, s, a);
+            hipLaunchKernelGGL((k_list<T, 512, 32>), grid, dim3(512), 0, s, a);
             hipLaunchKernelGGL((k_pick<T, 16384, 512>), rows, dim3(512), 0, s, a);
         }
     }

@@ -203,3 +203,18 @@ def test_no_rows_and_the_librarys_stream():
     c.go(abi.lib().navi_device_stream())
     abi.lib().navi_device_synchronize()
     assert c.token.tolist() == [w[0] for w in c.expect()]
+
+
+@pytest.mark.parametrize("vocab", [500, 2048, 20000])
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_every_kind_of_nan_is_left_out(vocab, kind):
+    """Signalling and quiet ones of both signs, among the likely tokens and instead of the likeliest."""
+    x, u = logits(len(RULES), vocab, 77, kind)
+    bits = {"f32": (np.int32, [0x7F800001, 0x7FC00000, 0x7FFFFFFF, -0x7FFFFF, -1, 0x7FBFFFFF]),
+            "f16": (np.int16, [0x7C01, 0x7E00, 0x7FFF, -0x3FF, -1, 0x7DFF]), "bf16": (np.int16, [0x7F81, 0x7FC0, 0x7FFF, -0x7F, -1, 0x7FBF])}[kind]
+    raw = x.view(torch.int32 if kind == "f32" else torch.int16)
+    for r in range(len(RULES)):
+        top = x[r].float().topk(3).indices
+        raw[r, top[::2]] = bits[1][r % 6]
+        raw[r, r::7] = bits[1][(r + 3) % 6]
+    Call(x, RULES, u).check()
