@@ -228,12 +228,16 @@ def run(s):
         return {"append": _append, "attention": _attention, "sample": _sample, "accept": _accept}[op](s)
 
 
+_LIBRARY = []
+
+
 def _abi():
-    at = str(Path(__file__).resolve().parent.parent / "navi-tts_amd")
-    if at not in sys.path:
-        sys.path.insert(0, at)
-    from navi_amd import abi
-    return abi
+    """The package, found once."""
+    if not _LIBRARY:
+        sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "navi-tts_amd"))
+        from navi_amd import abi
+        _LIBRARY.append(abi)
+    return _LIBRARY[0]
 
 
 def _stream():
