@@ -929,6 +929,7 @@ constexpr int MT = 1024;
 // The rows' bins and records.
 __global__ void __launch_bounds__(MT) k_rows(Args a) {
     __shared__ Lds<MT> q;
+    __shared__ int first[MAXC];
     const int row = blockIdx.x, t = threadIdx.x;
     const size_t at = static_cast<size_t>(row) * a.chunks;
     // all chunks' bins on their way at once (of a greedy row: nothing of use); a chunk without a token has none
@@ -940,7 +941,7 @@ __global__ void __launch_bounds__(MT) k_rows(Args a) {
         q.w[0][t] = 0;
         q.n[t] = 0;
     }
-    const uint64_t best = block_max(t < a.chunks ? gld(a.best + at + t) : uint64_t(0), q, 0);
+    const uint64_t mine = t < a.chunks ? gld(a.best + at + t) : uint64_t(0), best = block_max(mine, q, 0);
     Record *rec = a.record + row;
     if (t == 0) {
         gst(&rec->best, best);
@@ -950,14 +951,16 @@ __global__ void __launch_bounds__(MT) k_rows(Args a) {
     if (t == 0) gst(&rec->fine, 0);
     if (best == 0 || r.greedy) return;
     const double best4 = static_cast<double>(logit_of(best)) * r.c4, top = floor(best4);
+    // a chunk's first bin among the row's
+    if (t < MAXC) first[t] = mine ? bin_of(logit_of(mine), r.c4, top) : BINS;
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < MAXC * BINS / MT; ++i) {
-        if (i * (MT / BINS) >= a.chunks || !got[i]) continue;
-        const uint64_t b = gld(a.best + at + i * (MT / BINS) + t / BINS);
-        const double j = top - floor(static_cast<double>(logit_of(b)) * r.c4) + t % BINS;
-        if (j < BINS) {
-            atomicAdd(&q.n[static_cast<int>(j)], static_cast<unsigned>(got[i] >> 48));
-            atomicAdd(&q.w[0][static_cast<int>(j)], static_cast<unsigned long long>(got[i] & (ONE - 1)));
+        if (i * (MT / BINS) >= a.chunks) break;
+        const int j = first[i * (MT / BINS) + t / BINS] + t % BINS;
+        if (got[i] && j < BINS) {
+            atomicAdd(&q.n[j], static_cast<unsigned>(got[i] >> 48));
+            atomicAdd(&q.w[0][j], static_cast<unsigned long long>(got[i] & (ONE - 1)));
         }
     }
     __syncthreads();

@@ -725,12 +725,14 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
 template <class E, bool PAIR, class P, int D, int RW, bool CUT>
 __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args a) {
     constexpr bool F8 = sizeof(P) == 1;
-    typedef std::conditional_t<F8, u32x2_t, u32x4_t> Got;        // 8 elements of the pool; E in LDS
     constexpr int NT = 2, RWV = waves_of(PAIR, RW), KW = RWV / RW;
     typedef Rows<E, PAIR, D, NT> R;
     typedef typename R::v8 v8;
     constexpr int KS = R::KS, DT = R::DT, QP = R::QP, RB = D * 2, TB = KT * RB, DP = D + 4;
-    constexpr int LPR = RB / 16, RPI = WAVE / LPR, KPW = KT / RW, SI = KPW / RPI;   // lanes a row, rows a load, keys a wave, its loads
+    // keys a wave; elements of the pool that a lane loads: 16 bytes of them, or 8 where a wave would have less than a load; lanes a row, rows a load,
+    // its loads. In LDS a row is LCH 16-byte pieces of E
+    constexpr int KPW = KT / RW, EPL = F8 ? (KPW * D >= 16 * WAVE ? 16 : 8) : 8, LPR = D / EPL, RPI = WAVE / LPR, SI = KPW / RPI, LCH = RB / 16, CPL = LCH / LPR;
+    typedef std::conditional_t<F8 && EPL == 8, u32x2_t, u32x4_t> Got;
     static_assert(KW * RW == RWV && SI * RPI * RW == KT, "");
     constexpr int BUFS = 2 * KW * 2 * TB, JOIN = (KW - 1) * RW * 32 * DP * 4;
     __shared__ __align__(16) unsigned char sm[BUFS > JOIN ? BUFS : JOIN];
@@ -744,11 +746,11 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
     const int qrow0 = s.group * RW * 32 + rw * 32;
     const Pages pg{a.table + static_cast<size_t>(s.req) * a.blocks, min(s.at.len, s.t_end * KT), a};
 
-    // staging: this lane's 16 bytes of rows rw KPW + i RPI + l / LPR of the tile
+    // staging: this lane's EPL elements of rows rw KPW + i RPI + l / LPR of the tile
     const int c = l % LPR, r0 = rw * KPW + l / LPR;
     Got kr[SI], vr[SI];
     int slot[SI], page[SI];
-    const P *kb = static_cast<const P *>(a.k) + s.kvh * D + 8 * c, *vb = static_cast<const P *>(a.v) + s.kvh * D + 8 * c;
+    const P *kb = static_cast<const P *>(a.k) + s.kvh * D + EPL * c, *vb = static_cast<const P *>(a.v) + s.kvh * D + EPL * c;
     auto look_up = [&](int t) {
 #pragma unroll
         for (int i = 0; i < SI; ++i) page[i] = pg.page_of(t * KT + r0 + i * RPI);
@@ -768,10 +770,12 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
         for (int r = 0; r < RPI; ++r) x |= static_cast<uint32_t>((b >> (r * LPR) & ((uint64_t(1) << LPR) - 1)) != 0) << r;
         return x << (rw * KPW + i * RPI);
     };
-    auto as_e = [](const Got &g) {
+    auto as_e = [](const Got &g, int j) {                         // the load's j-th 16 bytes of E
         if constexpr (F8) {
-            const u32x4_t one[1] = {u32x4_t{g[0], g[1], 0u, 0u}};
-            return operand_of<E, true>(one, 0);
+            u32x4_t one[1];
+            if constexpr (EPL == 16) one[0] = g;
+            else one[0] = u32x4_t{g[0], g[1], 0u, 0u};
+            return operand_of<E, true>(one, j);
         } else {
             return g;
         }
@@ -790,7 +794,8 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
                 there |= bits_of(__ballot(slot[i] >= 0), i);
                 vr[i] = slot[i] < 0 ? Got(0u) : vr[i];
                 bool odd;
-                if constexpr (F8) odd = f8_any_nan(u32x4_t{vr[i][0], vr[i][1], 0u, 0u});
+                if constexpr (F8 && EPL == 8) odd = f8_any_nan(u32x4_t{vr[i][0], vr[i][1], 0u, 0u});
+                else if constexpr (F8) odd = f8_any_nan(vr[i]);
                 else odd = any_special<E>(vr[i]);
                 const uint32_t x = bits_of(__ballot(t * KT + r0 + i * RPI >= s.at.past && odd), i);
                 special |= x;
@@ -800,8 +805,12 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
 #pragma unroll
         for (int i = 0; i < SI; ++i) {
             const int r = r0 + i * RPI;
-            *reinterpret_cast<u32x4_t *>(kd + r * RB + ((c ^ (r & (LPR - 1))) << 4)) = as_e(kr[i]);
-            *reinterpret_cast<u32x4_t *>(v_at<D>(vd, r, c >> 1, c & 1)) = as_e(vr[i]);
+#pragma unroll
+            for (int j = 0; j < CPL; ++j) {
+                const int p = c * CPL + j;
+                *reinterpret_cast<u32x4_t *>(kd + r * RB + ((p ^ (r & (LCH - 1))) << 4)) = as_e(kr[i], j);
+                *reinterpret_cast<u32x4_t *>(v_at<D>(vd, r, p >> 1, p & 1)) = as_e(vr[i], j);
+            }
         }
         if (l == 0) {
             s_there[b][kw][rw] = there;
@@ -858,7 +867,7 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
                 const int r = kt * 16 + lr;
-                kf[kt] = bits<v8>(*reinterpret_cast<u32x4_t *>(kd + r * RB + (((4 * k + lg) ^ (r & (LPR - 1))) << 4)));
+                kf[kt] = bits<v8>(*reinterpret_cast<u32x4_t *>(kd + r * RB + (((4 * k + lg) ^ (r & (LCH - 1))) << 4)));
             }
 #pragma unroll
             for (int p = 0; p < QP; ++p)
