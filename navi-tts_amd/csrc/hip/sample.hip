@@ -1,21 +1,23 @@
 // A step's logits to its next codes on gfx950 (the C ABI's navi_sample_rows and navi_draft_accept): one token for every row under its
 // own rule, and the drafted rows that the sampled codes confirm.
 //
-// Sampling. A row's tokens stand in the order of their logits x (the lowest index first among equals). Their weights are
-// 2^(4 c (x - max) / 4) with c = log2 e / temperature; a rule keeps a prefix of the order, and the token is the first, in the order of the
-// indexes, at which the kept weights' running sum passes u of their total. So that the token is the definition's and not that of the
-// sums' rounding, weights are computed in 64 bits (2^-43) and summed as integers or in 64 bits.
+// Sampling. A row's tokens stand in the order of their logits x (the lowest index first among equals). Their weights are 2^(c (x - max)) with
+// c = log2 e / temperature; a rule keeps the beginning of the order, and the token is the first, in the order of the indexes, at which the
+// kept weights' running sum passes u of their total. So that the token is the definition's and not that of the sums' rounding, weights are
+// computed in 64 bits (2^-43) and summed as integers (in units of 2^-31 of a bin's edge) or in 64 bits.
 //
-//  * The order is cut into bins of a quarter of a power of two, bin floor(4 c x), 256 of them below the largest (2^-64: what is
-//    below has no weight). One pass counts the tokens and sums the weights of every bin, one LDS atomic a token: the weight in
-//    units of 2^-31 of its bin's edge below bit 48, the count above.
-//  * The sums over the bins say in which bin top-k and top-p end. Only that bin's tokens are looked at again: a radix
-//    select over (logit, index) as one 64-bit key, by count or by weight, gives the last key that is kept.
+//  * The order is cut into bins of a quarter of a power of two, floor(4 c x), 256 of them from the largest on (what is below 2^-63 has
+//    no weight). One pass counts the tokens and sums the weights of every bin, one LDS atomic a token: the weight below bit 48, the count above.
+//  * Sums over the bins, in a wave's registers, say in which bin top_k and top_p end. Only that bin's tokens are looked at again, by their
+//    64-bit keys (logit, then index): down to 64 by digits of the key, and these each against all.
 //  * Then the kept weights are summed in the order of the indexes, and the wave that holds the border names the token.
 //
-// Up to 16384 tokens a block has its row in registers and does all of this in one launch. Longer rows are cut into chunks: a launch makes
-// the chunks' bins, a second the rows', a third copies the tokens of the bins in question, a fourth does the rest, reading again only
-// the chunk that the number falls into.
+// Up to 16384 tokens a block has its row in LDS and does all of this in one launch: a chain of some twenty dependent steps, whose latencies bound it
+// (one row of 2048 tokens with top_k 10 us, 512 rows 14.5, 8192 rows 98, a CU's instructions by then). Longer rows are cut into chunks of
+// 4096 or 16384 tokens, in four launches: the chunks' bins (k_bins), the rows' (k_rows), the marked bins' tokens copied side by side (k_list),
+// and one block a row for the rest, which reads again only the chunk that the number falls into (k_pick). 256 rows of 151936 f32 tokens, each
+// with a rule of its own, take 91 us, of which k_bins 42 (156 MB at 3.7 TB/s; 20 instructions a token, all SIMDs issuing), k_rows 6,
+// k_list 17 and k_pick 27, as long as its slowest row: a nucleus that ends among thousands of tokens of one bin. One row 30 to 45 us.
 #include "host_util.h"
 #include "kv.h"
 #include "sampler.h"
@@ -31,8 +33,8 @@ namespace navi_amd {
 namespace sample {
 
 constexpr int BINS = 256;
-constexpr int CAP = 8192;              // tokens of the bins in question that are kept in LDS; more are read from the row again
-constexpr int ROW_MOST = 16384;        // tokens of a row that a block has in registers
+constexpr int CAP = 8192;              // tokens of the marked bins that are kept in LDS; where there are more, the row is read again
+constexpr int ROW_MOST = 16384;        // tokens of a row that a block has in LDS
 constexpr int MAXC = 64;               // most chunks of a row
 constexpr int COPIES = 4;
 constexpr unsigned long long ONE = 1ull << 48;   // a token in a sum of weights
@@ -45,7 +47,8 @@ struct Args {
     const uint32_t *allowed, *seen;
     int32_t *token;
     float *logprob;
-    // the workspace (ws_of): the chunks' bins and largest keys, the rows' bins, and the keys to look at again
+    // the workspace (launch): chunks' bins and largest keys; rows' sums and marked tokens; chunks' running sums of weights, and the largest logit of each
+    // part of a chunk
     uint64_t *bins, *best, *sums, *list;
     double *upto;
     float *most;
@@ -332,7 +335,7 @@ struct Lds {
     unsigned long long w[COPIES][BINS];    // sums of the bins' weights, counts above bit 48, by lane: fewer of an instruction meet; then of a digit's tokens
     unsigned n[BINS];                  // counts that may pass 16 bits
     unsigned long long red[2][NW];
-    int count[NW];
+    int at[NW];                        // of block_best
     float most[NW];
     double seg[64];
     unsigned long long few[WAVE];      // the tokens that are left to rank
@@ -437,7 +440,6 @@ struct Marks {
     // whether the parts' sums are made of top_k's bin, and of top_p's if that is one: where the tokens are too many to rank at once
     __device__ __forceinline__ bool fine_k() const { return k.bin < BINS && k.own > WAVE; }
     __device__ __forceinline__ bool fine_p() const { return p0 == p1 && own > WAVE; }
-    __device__ __forceinline__ bool has(int j) const { return j < BINS && (j == k.bin || (j >= p0 && j <= p1)); }
 };
 
 // Tokens to look at again: keys in LDS, or, where they are too many, the row.
@@ -704,6 +706,13 @@ __device__ __forceinline__ void cut_tokens(Cut &cut, const S &s, Lds<BT> &q, con
     }
 }
 
+// log x of 2^-64 < x < 2^64 in 64 bits (2^-41): a 32-bit logarithm l, and with x 2^-l = 1 + d, |d| < 2^-18, the series of log(1 + d).
+__device__ __forceinline__ double log_of(double x) {
+    const double l = static_cast<double>(__builtin_amdgcn_logf(static_cast<float>(x))), q = -4.0 * l, b = floor(q);
+    const double d = x * quarter(q - b) * bin_edge(-static_cast<int>(b)) - 1.0;
+    return l * (4.0 * LN) + d * (1.0 - d * (0.5 - d * (1.0 / 3.0)));
+}
+
 __device__ __forceinline__ void put(const Args &a, int row, int token, float logprob) {
     gst(a.token + static_cast<size_t>(row) * a.ld_token, token);
     if (a.logprob) gst(a.logprob + row, logprob);
@@ -756,7 +765,7 @@ __device__ __forceinline__ void draw(const Args &a, int row, const float *xs, in
     if (!some) return;                                            // nothing is kept here
     const int seg = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
     if (seg % NW != wv) return;
-    const double before = seg ? lane_double(upto, seg - 1) : 0.0, log_total = a.logprob ? log(total) : 0.0;
+    const double before = seg ? lane_double(upto, seg - 1) : 0.0, log_total = a.logprob ? log_of(total) : 0.0;
     const double own = four(seg / NW, x), sum = before + wave_scan(own);
     const uint64_t over = __ballot(own > 0.0 && sum > number), any = __ballot(own > 0.0);
     if (l != (over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any))) return;
@@ -805,7 +814,7 @@ __global__ void __launch_bounds__(BT) k_row(Args a) {
         see_all<BT>(x, 0, v, r);
         keep<BT, PARTS, T>(v, xs);
         float most[PARTS];
-        best = block_best<BT, PARTS>(v, 0, most, r.greedy, q.most, q.count);
+        best = block_best<BT, PARTS>(v, 0, most, r.greedy, q.most, q.at);
     }
     if (best == 0 || r.greedy) {
         if (t == 0) put(a, row, best ? index_of(best) : -1, best ? 0.f : -INFINITY);
@@ -1118,11 +1127,11 @@ __global__ void __launch_bounds__(FT) k_pick(Args a) {
     if (cut.bin < BINS) {
         // and of that one's tokens those that are kept, chunk by chunk of a wave's: a chunk's lie side by side in the list
         const Keys in = between(bin_start(cut.bin, r, top), bin_start(cut.bin - 1, r, top));
-        // tokens side by side to a thread, which adds up those of a chunk first
-        const int count = held ? n : a.vocab, share = (count + FT - 1) / FT, end = min(count, (t + 1) * share);
+        // a thread adds up its tokens of a chunk first: of the list's, which lie side by side, consecutive ones
+        const int share = (n + FT - 1) / FT, end = held ? min(n, (t + 1) * share) : a.vocab, step = held ? 1 : FT;
         uint64_t run = 0;
         int chunk = 0;
-        for (int i = t * share; i < end; ++i) {
+        for (int i = held ? t * share : t; i < end; i += step) {
             uint64_t k;
             if (held) {
                 k = list[i];
