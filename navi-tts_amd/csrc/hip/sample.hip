@@ -1066,7 +1066,7 @@ __global__ void __launch_bounds__(BT) k_list(Args a) {
         const float y = x.at(i, r);
         if (at < CAP) gst(a.list + static_cast<size_t>(row) * CAP + at, key_of(y, i));
         if (!fine) continue;
-        const uint32_t k = float_key(y);
+        const uint32_t k = float_key(y + 0.f);                    // -0 where its key is, at 0
         const unsigned long long one = ONE + units(place_of(y, r.c4, top).f);
         if ((fine & 1) && k - lo[0] < len[0]) atomicAdd(&w[0][(k - lo[0]) >> s0], one);
         if ((fine & 2) && k - lo[1] < len[1]) atomicAdd(&w[1][(k - lo[1]) >> s1], one);

@@ -76,6 +76,17 @@ def test_values_that_are_no_ordinary_numbers(vocab):
         Call(x, rules[shift:] + rules[:shift], torch.rand(12, generator=g).numpy()).check()
 
 
+@pytest.mark.parametrize("vocab", [2048, 20000])
+def test_zeros_of_both_signs_are_equal_where_bins_are_narrow(vocab):
+    """At temperatures near the least, a bin holds few float keys, and 0 and -0 are neighbours among them: more than can be ranked at once."""
+    x = torch.full((6, vocab), -1.0)
+    x[:, 3:900:2], x[:, 4:900:2] = -0.0, 0.0
+    u = np.array([0.0, 0.3, 0.9, 0.999, 0.5, 1.0], np.float32)
+    for t in (1e-43, 1e-44, 1e-41):
+        Call(x, [(t, k, 1, 0, 1) for k in (300, 65, 600, 880, 1, 897)], u).check()
+        Call(x, [(t, 0, p, 0, 1) for p in (0.3, 0.08, 0.6, 0.97, 1e-6, 0.5)], u).check()
+
+
 @pytest.mark.parametrize("vocab", [300, 2048, 33333])
 def test_numbers_at_and_past_the_ends(vocab):
     """0 is the first kept token, what is not below 1 the last quantile, NaN and below 0 as 0."""
