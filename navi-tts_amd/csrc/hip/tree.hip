@@ -24,6 +24,12 @@
 //    products are 880 TFLOP/s, and 20 us for the start, the parts' 17 MB and the join.
 //  * Softmax against a reference value that moves only when a score passes it by more than SLACK: the
 //    rescaling, and the maximum over lanes that it needs, are off the common path. exp2 with the scale folded in.
+//  * An e4m3 pool's codes become f16 or bf16, which hold them exactly, on their way to the matrix units: in registers up to 32 query rows (16
+//    codes a lane and load, so that a lane's two operands have columns 64 i + 16 (l / 16) .. and q is read in that order), as they are staged
+//    above. K's factor goes into the scores' and V's into the sum's inverse, so that the loops are those of the other pools. 32 requests with one
+//    row each over 1024 keys take 16.9 us (67.5 MB, 4.0 TB/s); 64 requests x 24 rows over 8192 keys 284 to 305 us from card to card (1.08 GB,
+//    3.5 to 3.8 TB/s): half the bytes of f16 under the same products, softmax and barriers (scores alone 208 us), which two waves a SIMD
+//    overlap only in part; fewer cycles have come with a lower clock. Loads of 8 codes a lane took 310 us where these take 292.
 //  * Requests are cut into even chunks over the blocks, however uneven their lengths (lay_out): 64 requests of lengths spread from
 //    1 to 8000 71 us, uncut 145. A second kernel joins the chunks' results (unnormalised sums, reference, sum) in their order.
 #include "dev_common.h"
