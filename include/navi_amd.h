@@ -373,7 +373,7 @@ navi_status navi_kv_commit(const navi_kv_pages *pages, const navi_kv_view *kv, c
                            const int32_t *d_accept, int32_t *d_n_past_out, int32_t *d_status, void *stream, char *err,
                            size_t errlen);
 /* ---- a step's logits to its next codes: no counterpart in the reference, whose sampler is part of the frame -----------------
- * Both enqueue on `stream` and return, as the four above; pointers named d_* are device memory of the library's device. */
+ * Both enqueue on `stream` and return, as the operators above; pointers named d_* are device memory of the library's device. */
 
 typedef struct {                       /* how a row's token is taken */
     float   temperature;               /* not above 0, or NaN: the largest logit */
