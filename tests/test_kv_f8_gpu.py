@@ -324,3 +324,37 @@ def test_append_attend_commit(dim):
     rows_of = list(range(past)) + [past + a for a in (0, 2, 4, 5)]
     q, got = step(1, [-1], x[:1].contiguous())
     assert (got[0].double() - want(q[0], rows_of + [0])).abs().max() <= 2.0 ** -8
+
+
+def test_pages_past_32_bits():
+    """The same step in pages at the start of a pool of 5 GB and at its end: K, V and the attention alike."""
+    g = torch.Generator().manual_seed(5)
+    heads, kv, dim, page, n_pages, rows = 16, 8, 128, 16, 330_000, 60
+    w = kv * dim
+    assert n_pages * page * w > 1 << 32
+    k, v = (torch.empty(n_pages * page, w, dtype=torch.uint8, device="cuda") for _ in range(2))
+    x = torch.randn(rows, (heads + 2 * kv) * dim, generator=g).bfloat16().cuda()
+    lay = abi.KvHeads(heads, kv, dim, abi.DT_F8E4M3, None, None)
+    got = []
+    for table in ([0, 1, 2, 3], [n_pages - 1, n_pages - 3, n_pages - 2, n_pages - 4]):
+        t = torch.tensor(table, dtype=torch.int32)
+        at = torch.arange(rows)
+        slot = (t[at // page] * page + at % page).int()
+        d = [a.int().cuda() for a in (t, torch.tensor([0]), torch.tensor([0, rows]), slot, at)]
+        mask = torch.tensor([(1 << (r + 1)) - 1 for r in range(rows)], dtype=torch.int64, device="cuda")
+        pages = abi.KvPages(1, page, n_pages, 4, rows, 64, *(a.data_ptr() for a in d), mask.data_ptr())
+        q = torch.zeros(rows, heads * dim, dtype=torch.bfloat16, device="cuda")
+        out = torch.full_like(q, 7.0)
+        abi.kv_append(pages, lay, x.data_ptr(), abi.DT_BF16, x.shape[1], k.data_ptr(), v.data_ptr(), w, q.data_ptr(), abi.DT_BF16, q.shape[1], stream=stream())
+        ws = torch.empty(abi.tree_workspace(pages, lay, rows), dtype=torch.uint8, device="cuda")
+        abi.tree_attention(pages, lay, q.data_ptr(), abi.DT_BF16, q.shape[1], k.data_ptr(), v.data_ptr(), w, dim ** -0.5, rows, out.data_ptr(), out.shape[1], ws.data_ptr(),
+                           ws.numel(), stream=stream())
+        path, acc, past, done = (torch.tensor(a, dtype=torch.int32, device="cuda") for a in ([[1, 4, 59]], [3], [9], [9]))
+        abi.kv_commit(pages, [k.data_ptr()], [v.data_ptr()], w // 2, path.data_ptr(), 3, acc.data_ptr(), past.data_ptr(), done.data_ptr(), stream=stream())
+        torch.cuda.synchronize()
+        assert past.tolist() == [3] and done.tolist() == [0]
+        got.append([out.cpu()] + [c[slot.long().cuda()].cpu() for c in (k, v)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    want = codes_of(x.cpu().float().view(rows, -1, dim)[:, heads:heads + kv].reshape(rows, w))
+    order = [1, 4, 59] + list(range(3, rows))
+    assert torch.equal(got[0][1], want[order])

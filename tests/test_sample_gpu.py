@@ -229,3 +229,21 @@ def test_every_kind_of_nan_is_left_out(vocab, kind):
         raw[r, top[::2]] = bits[1][r % 6]
         raw[r, r::7] = bits[1][(r + 3) % 6]
     Call(x, RULES, u).check()
+
+
+@pytest.mark.parametrize("vocab", [2048, 20000])
+def test_rows_past_32_bits(vocab):
+    """Three rows 2^31 - 1 elements apart, the last from the 2^32nd on."""
+    x, u = logits(3, vocab, 17, "bf16")
+    rules = [(0.9, 40, 0.95, 0, 1), (1.0, 0, 0.8, 0, 1), (1.1, 60, 1, 0.02, 1)]
+    c = Call(x, rules, u)
+    ld = (1 << 31) - 1
+    far = torch.empty(2 * ld + vocab, dtype=torch.bfloat16, device="cuda")
+    for r in range(3):
+        far[r * ld:r * ld + vocab] = x[r].cuda()
+    want = c.check()
+    c.d_x, c.ld = far, ld
+    c.token.fill_(-5)
+    c.go()
+    torch.cuda.synchronize()
+    assert c.token.tolist() == want
