@@ -442,35 +442,57 @@ struct Marks {
     __device__ __forceinline__ bool fine_p() const { return p0 == p1 && own > WAVE; }
 };
 
-// Tokens to look at again: keys in LDS, or, where they are too many, the row.
-template <class T, int BATCH>
+// Tokens to look at again: keys in LDS, or, where they are too many, all of the row's, SPAN at a time in LDS as the rule sees them (WHOLE: there already).
+// A thread reads back those that it has put there. Rows so flat are slow, since one block goes over all of the row several times: 151936 normal logits with
+// sigma 0.3, of which the largest bin has a quarter, 310 us, 256 such rows 432 (418 and 726 with the logits loaded one by one); all alike 533.
+template <class T, int BATCH, int SPAN, bool WHOLE>
 struct Tokens {
     typedef uint64_t Batch[BATCH];
     const unsigned long long *key;
+    float *xs;
     int n;
     bool held;
     const Row<T> &row;
     const Rule &r;
     double top;
+    // tokens i0 .. i0 + SPAN - 1 into xs
+    template <int BT>
+    __device__ __forceinline__ void bring(int i0) const {
+        if constexpr (!WHOLE) {
+            float v[SPAN / BT];
+            load_all<BT>(row, i0, v);
+            see_all<BT>(row, i0, v, r);
+            keep<BT, SPAN / BT / 4, T>(v, xs);
+        }
+    }
+    // the key of the thread's j-th of these, 0: none
+    template <int BT>
+    __device__ __forceinline__ uint64_t brought(int i0, int j) const {
+        const int i = token_at<BT>(0, j);
+        const float x = xs[i];
+        return x == -INFINITY ? 0 : key_of(x, i0 + i);
+    }
     // f(keys) of the thread's tokens, BATCH at a time (0: none), so that their loads and sums overlap
     template <int BT, class F>
     __device__ __forceinline__ void each(F f) const {
-        const int end = held ? n : row.vocab;
+        const int end = held ? n - (threadIdx.x & ~63) : row.vocab, step = held ? BATCH * BT : SPAN;
 #pragma unroll 1
-        for (int i0 = threadIdx.x & ~63; i0 < end; i0 += BATCH * BT) {
-            Batch k;
+        for (int i0 = 0; i0 < end; i0 += step) {
+            if (!held) bring<BT>(i0);
+#pragma unroll 1
+            for (int b = 0; b < (held ? BATCH : SPAN / BT); b += BATCH) {
+                Batch k;
 #pragma unroll
-            for (int j = 0; j < BATCH; ++j) {
-                const int i = i0 + j * BT + (threadIdx.x & 63);
-                k[j] = 0;
-                if (held) {
-                    if (i < end) k[j] = key[i];
-                } else if (i < end) {
-                    const float x = row.at(i, r);
-                    if (x != -INFINITY) k[j] = key_of(x, i);
+                for (int j = 0; j < BATCH; ++j) {
+                    if (held) {
+                        const int i = i0 + j * BT + threadIdx.x;
+                        k[j] = i < n ? key[i] : 0;
+                    } else {
+                        k[j] = brought<BT>(i0, b + j);
+                    }
                 }
+                f(k);
             }
-            f(k);
         }
     }
     __device__ __forceinline__ uint32_t units_of(uint64_t k) const { return units(place_of(logit_of(k), r.c4, top).f); }
@@ -859,7 +881,7 @@ __global__ void __launch_bounds__(BT) k_row(Args a) {
         }
         __syncthreads();
         const int listed = q.listed;
-        cut_tokens(cut, Tokens<T, 2>{list, listed, listed <= HELD, x, r, top}, q, r, bins, top, marks, ranges, nullptr);
+        cut_tokens(cut, Tokens<T, 2, MOST, true>{list, xs, listed, listed <= HELD, x, r, top}, q, r, bins, top, marks, ranges, nullptr);
     }
     draw<BT, PARTS, true>(a, row, xs, 0, q, r, top, cut, number, 0.0);
 }
@@ -1114,10 +1136,11 @@ __global__ void __launch_bounds__(FT) k_pick(Args a) {
         cut.narrow(bin_of(key_float(k), r.c4, top), static_cast<uint64_t>(k) << 32);
     }
     __syncthreads();
+    const Tokens<T, 8, 2 * CAP, false> tokens{list, xs, n, held, x, r, top};
     if (r.k > 0 || r.p < 1.0) {
         const Bins bins = bins_of(a, row);
         const Marks marks(bins, r);
-        cut_tokens(cut, Tokens<T, 8>{list, n, held, x, r, top}, q, r, bins, top, marks, Ranges(marks, r, top), a.sums + (static_cast<size_t>(row) * 3 + 1) * 2 * BINS);
+        cut_tokens(cut, tokens, q, r, bins, top, marks, Ranges(marks, r, top), a.sums + (static_cast<size_t>(row) * 3 + 1) * 2 * BINS);
     }
     // the chunks' weights in the bins before the last kept one
     const double first = top - floor(static_cast<double>(logit_of(own)) * r.c4);   // a chunk's first bin among the row's
@@ -1128,25 +1151,26 @@ __global__ void __launch_bounds__(FT) k_pick(Args a) {
         // and of that one's tokens those that are kept, chunk by chunk of a wave's: a chunk's lie side by side in the list
         const Keys in = between(bin_start(cut.bin, r, top), bin_start(cut.bin - 1, r, top));
         // a thread adds up its tokens of a chunk first: of the list's, which lie side by side, consecutive ones
-        const int share = (n + FT - 1) / FT, end = held ? min(n, (t + 1) * share) : a.vocab, step = held ? 1 : FT;
         uint64_t run = 0;
         int chunk = 0;
-        for (int i = held ? t * share : t; i < end; i += step) {
-            uint64_t k;
-            if (held) {
-                k = list[i];
-            } else {
-                const float y = x.at(i, r);
-                k = y == -INFINITY ? 0 : key_of(y, i);
-            }
-            if (!in.have(k) || k < cut.key) continue;
+        auto take = [&](uint64_t k) {
+            if (!in.have(k) || k < cut.key) return;
             const int c = index_of(k) / CHUNK;
             if (c != chunk) {
                 if (run) atomicAdd(&part[chunk], static_cast<unsigned long long>(run));
                 chunk = c;
                 run = 0;
             }
-            run += units(place_of(logit_of(k), r.c4, top).f);
+            run += tokens.units_of(k);
+        };
+        if (held) {
+            const int share = (n + FT - 1) / FT, end = min(n, (t + 1) * share);
+            for (int i = t * share; i < end; ++i) take(list[i]);
+        } else {
+            for (int i0 = 0; i0 < a.vocab; i0 += 2 * CAP) {
+                tokens.template bring<FT>(i0);
+                for (int j = 0; j < 2 * CAP / FT; ++j) take(tokens.template brought<FT>(i0, j));
+            }
         }
         if (run) atomicAdd(&part[chunk], static_cast<unsigned long long>(run));
         __syncthreads();
