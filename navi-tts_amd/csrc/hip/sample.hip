@@ -1178,7 +1178,8 @@ __global__ void __launch_bounds__(FT) k_pick(Args a) {
     }
     const double upto = wave_scan(mine), total = lane_double(upto, 63), number = u * total;
     const uint64_t past = __ballot(upto > number), some = __ballot(mine > 0.0);
-    const int chunk = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+    // none has a weight only if the logits have been written to since the bins were made: a chunk of the row even then
+    const int chunk = past ? __builtin_ctzll(past) : some ? 63 - __builtin_clzll(some) : index_of(best) / CHUNK;
     const double before = chunk ? lane_double(upto, chunk - 1) : 0.0;
     __syncthreads();                                              // the list has been read
     {
