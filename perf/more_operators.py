@@ -228,16 +228,12 @@ def run(s):
         return {"append": _append, "attention": _attention, "sample": _sample, "accept": _accept}[op](s)
 
 
-_LIBRARY = []
-
-
 def _abi():
-    """The package, found once."""
-    if not _LIBRARY:
-        sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "navi-tts_amd"))
-        from navi_amd import abi
-        _LIBRARY.append(abi)
-    return _LIBRARY[0]
+    at = str(Path(__file__).resolve().parent.parent / "navi-tts_amd")
+    if at not in sys.path:
+        sys.path.insert(0, at)
+    from navi_amd import abi
+    return abi
 
 
 def _stream():
