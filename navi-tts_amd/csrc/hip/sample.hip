@@ -783,8 +783,12 @@ __device__ __forceinline__ void draw(const Args &a, int row, const float *xs, in
         total = lane_double(upto, 63);
         number *= total;
     }
-    const uint64_t past = __ballot(upto > number), some = __ballot(mine > 0.0);
-    if (!some) return;                                            // nothing is kept here
+    // only where something is kept: the lanes' sums associate differently, so that one that adds nothing can be a rounding above the one before it
+    const uint64_t past = __ballot(mine > 0.0 && upto > number), some = __ballot(mine > 0.0);
+    if (!some) {                                                  // nothing is: the logits have been written to meanwhile
+        if (t == 0) put(a, row, -1, -INFINITY);
+        return;
+    }
     const int seg = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
     if (seg % NW != wv) return;
     const double before = seg ? lane_double(upto, seg - 1) : 0.0, log_total = a.logprob ? log_of(total) : 0.0;
@@ -1177,7 +1181,7 @@ __global__ void __launch_bounds__(FT) k_pick(Args a) {
         if (l < a.chunks) mine += static_cast<double>(part[l]) * (bin_edge(cut.bin) / UNIT);
     }
     const double upto = wave_scan(mine), total = lane_double(upto, 63), number = u * total;
-    const uint64_t past = __ballot(upto > number), some = __ballot(mine > 0.0);
+    const uint64_t past = __ballot(mine > 0.0 && upto > number), some = __ballot(mine > 0.0);   // as in draw
     // none has a weight only if the logits have been written to since the bins were made: a chunk of the row even then
     const int chunk = past ? __builtin_ctzll(past) : some ? 63 - __builtin_clzll(some) : index_of(best) / CHUNK;
     const double before = chunk ? lane_double(upto, chunk - 1) : 0.0;
