@@ -387,9 +387,10 @@ typedef struct {                       /* how a row's token is taken */
  * order of their logits, the lowest index first among equals; a row's rule keeps a part of that order, with probabilities
  * softmax(logit / temperature) over the tokens that top_k leaves for top_p, and over those that are left at the end for the draw: the token
  * is the first, in the order of the indexes, at which the sum of the kept ones passes d_u[row] (0 <= u < 1; what is outside counts as the end of
- * that range). Weights are computed and summed in 64 bits, so that a row's token does not depend on what is sampled beside it, but where d_u times the
- * kept ones' sum is a running sum to 2^-45 of it: above 16384 tokens the order of the additions goes with n_rows. Tokens below 2^-63 of the first one's
- * probability have none.
+ * that range). A weight is off by 2^-31 of itself at most (|logit| / temperature below 2^20), for the draw from up to 16384 tokens by 2^-37, and sums of
+ * them by 2^-45 of the whole, where all the kept ones are equal not at all: a number on a border between these gets the token that real numbers would. So a
+ * row's token does not depend on what is sampled beside it, but where d_u times the kept ones' sum is a running sum to 2^-45 of it: above 16384 tokens the
+ * order of the additions goes with n_rows. Tokens below 2^-63 of the first one's probability have none.
  * d_rules: device [n_rules], n_rules 1 (for all rows) or n_rows. d_allowed: bits [n_rows][ld_allowed words], token i bit i % 32 of word i / 32; a token
  * without its bit is left out, as are NaN and -infinity; +infinity counts as the largest finite number. d_seen: bits of the tokens that the repetition penalty
  * applies to. Either may be NULL; a stride of 0: one set for all rows. A row without a token gets -1, and log probability -infinity.

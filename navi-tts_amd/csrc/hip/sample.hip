@@ -3,8 +3,9 @@
 //
 // Sampling. A row's tokens stand in the order of their logits x (the lowest index first among equals). Their weights are 2^(c (x - max)) with
 // c = log2 e / temperature; a rule keeps the beginning of the order, and the token is the first, in the order of the indexes, at which the
-// kept weights' running sum passes u of their total. So that the token is the definition's and not that of the sums' rounding, weights are
-// computed in 64 bits (2^-43) and summed as integers (in units of 2^-31 of a bin's edge) or in 64 bits.
+// kept weights' running sum passes u of their total. So that the token is the definition's and not that of the sums' rounding, weights have few
+// enough bits that a block's sums of equal ones are exact in 64: integers in units of 2^-31 of a bin's edge (2^-32 off at most) for the cuts and for rows
+// in chunks, whose chunk and token are then found on one scale; 39 bits (computed to 2^-43) for the draw from a row that a block has whole.
 //
 //  * The order is cut into bins of a quarter of a power of two, floor(4 c x), 256 of them from the largest on (what is below 2^-63 has
 //    no weight). One pass counts the tokens and sums the weights of every bin, one LDS atomic a token: the weight below bit 48, the count above.
@@ -742,17 +743,21 @@ __device__ __forceinline__ void put(const Args &a, int row, int token, float log
 
 // The first token of the 4 BT PARTS in LDS (from i0 on) at which the kept weights' sum passes `number` (FROM_U: that part of the sum); none
 // passes it: the last kept one. `total`: the sum of all kept weights of the row, for the log probability (FROM_U: of those here).
+// Equal tokens, which 16-bit logits often have, are on a border between them for many a u: there the sums have to be those of real numbers. FROM_U: 39 bits
+// of a weight leave 14 for the 16384 tokens of a row. Else the weights are those of which `number` and `total` were made, the chunks' units: two
+// roundings of one weight, 2^-32 apart, would put the number on the wrong side.
 template <int BT, int PARTS, bool FROM_U>
 __device__ __forceinline__ void draw(const Args &a, int row, const float *xs, int i0, Lds<BT> &q, const Rule &r, double top, const Cut &cut, double number,
                                      double total) {
     constexpr int NW = BT / WAVE;
     static_assert(PARTS * NW <= 64, "a segment a lane");
     const int t = threadIdx.x, l = t & 63, wv = t >> 6;
+    const Units un;
     auto weight = [&](float x, int i) {                           // of token i, 0 where it is not kept
         double w = 0.0;
         if (key_of(x, i0 + i) >= cut.key) {
             const Place p = place_of(x, r.c4, top);
-            if (p.j < BINS) w = quarter(p.f) * bin_edge(p.j);
+            if (p.j < BINS) w = FROM_U ? as_double(as_bits(quarter(p.f) * bin_edge(p.j)) & ~uint64_t(0x3FFF)) : un.of(p.f) * (bin_edge(p.j) / UNIT);
         }
         return w;
     };

@@ -43,3 +43,33 @@ def test_a_chunk_without_a_kept_token_is_not_drawn_from(case):
     assert call.token.item() in (size * at[i - 1] + 300, size * at[i] + 100)
     w = weights(x[0].numpy(), call.rules[0])
     assert abs(call.logprob.item() - np.log(w[call.token.item()] / w.sum())) <= 8 * 2.0 ** -24 + 2.0 ** -28
+
+
+@pytest.mark.parametrize("kind", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("vocab", [2048, 16384, 20000, 151936])
+def test_a_number_on_a_border_between_equal_tokens(vocab, kind):
+    """2, 3, 4, 8 and 12 equal tokens, near each other and far apart, under u = j / 64: the first one at which the sum passes u, j n / 64 whole or not, is token
+    floor(j n / 64) of the n. All rows in one call, and a few a call: the same."""
+    rng = np.random.default_rng(vocab)
+    rows = 240
+    x = torch.full((rows, vocab), -float("inf"))
+    u, want, rules = [], [], []
+    for r in range(rows):
+        n, j = int(rng.choice([2, 3, 4, 8, 12])), int(rng.integers(1, 64))
+        if r % 3 < 2:
+            j = int(rng.integers(1, 4)) * 16 if n % 3 else 48                                # on a border, but for 3 tokens
+        width = vocab if r % 2 else 64
+        at = np.sort(rng.integers(0, vocab - width + 1) + rng.permutation(width)[:n])
+        x[r, at] = float(rng.integers(-400, 400)) / 16
+        u.append(j / 64)
+        want.append(int(at[j * n // 64]))
+        rules.append((float(rng.choice([0.7, 0.9, 1.0, 1.3])), int(rng.choice([0, n, 50])), float(rng.choice([1.0, 0.9999])), 0, 1))
+    x = x.to(kind)
+    call = Call(x, rules, u).go()
+    torch.cuda.synchronize()
+    assert call.token.tolist() == want
+    for r in range(0, rows, 6):
+        few = Call(x[r:r + 6], rules[r:r + 6], u[r:r + 6]).go()
+        torch.cuda.synchronize()
+        assert few.token.tolist() == want[r:r + 6]
+        assert torch.equal(few.logprob, call.logprob[r:r + 6])
