@@ -269,6 +269,11 @@ __device__ __forceinline__ uint32_t bin_start(int j, const Rule &r, double top) 
 struct Keys {
     uint64_t lo, len;
     __device__ __forceinline__ bool have(uint64_t k) const { return k - lo < len; }
+    // those of them from `from` on, n at most: a part, or a digit's keys, may reach past a bin's ends
+    __device__ __forceinline__ Keys part(uint64_t from, uint64_t n) const {
+        const uint64_t first = max(lo, from), last = min(lo + (len - 1), from + (n - 1));
+        return Keys{first, first <= last ? last - first + 1 : 0};
+    }
 };
 __device__ __forceinline__ Keys between(uint32_t lo, uint32_t hi) { return Keys{static_cast<uint64_t>(lo) << 32, static_cast<uint64_t>(hi - lo) << 32}; }
 // The least float key that min_p leaves (m > -inf).
@@ -596,7 +601,7 @@ __device__ __forceinline__ uint64_t select(const S &s, Lds<BT> &q, Keys in, int 
             c[i] = static_cast<int>(gld(fine.sums + BINS + 255 - 4 * l - i));
         }
         const int d = digit_of(c, w, n, need, mass, sum);
-        in = Keys{in.lo + (static_cast<uint64_t>(d) << (32 + fine.shift)), uint64_t(1) << (32 + fine.shift)};
+        in = in.part(in.lo + (static_cast<uint64_t>(d) << (32 + fine.shift)), uint64_t(1) << (32 + fine.shift));
     }
 #pragma unroll 1
     while (n > WAVE) {
@@ -650,7 +655,7 @@ __device__ __forceinline__ uint64_t select(const S &s, Lds<BT> &q, Keys in, int 
             if (s.held) w[i] &= ONE - 1;
         }
         const uint64_t above = h < 64 ? hi >> h << h : 0;
-        in = Keys{above | static_cast<uint64_t>(digit_of(c, w, n, need, mass, sum)) << at, uint64_t(1) << at};
+        in = in.part(above | static_cast<uint64_t>(digit_of(c, w, n, need, mass, sum)) << at, uint64_t(1) << at);
     }
     __syncthreads();
     if (t == 0) q.listed = 0;
