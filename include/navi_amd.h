@@ -401,7 +401,8 @@ navi_status navi_sample_rows(const void *d_logits, int32_t dtype, int32_t ld, in
                              int32_t n_rules, const float *d_u, const uint32_t *d_allowed, int32_t ld_allowed, const uint32_t *d_seen,
                              int32_t ld_seen, int32_t *d_token, int32_t ld_token, float *d_logprob, void *d_ws, size_t ws_bytes, void *stream,
                              char *err, size_t errlen);
-/* Workspace bytes of navi_sample_rows (host only; 0 where none is needed, or the arguments are not valid). */
+/* Workspace bytes that suffice for navi_sample_rows with up to n_rows rows of up to vocab tokens (host only; 0 where none are needed, or the arguments
+ * are not valid). */
 size_t navi_sample_workspace(int32_t n_rows, int32_t vocab);
 /* Which drafted rows the sampled codes confirm, for navi_kv_commit. Row r of a planned step was drafted to follow its parent (d_parent as
  * navi_kv_plan's; NULL: the row before) with the n_codes codes of d_drafted row r (stride ld_drafted); the model has given the codes of d_sampled

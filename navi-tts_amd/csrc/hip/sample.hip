@@ -1209,14 +1209,27 @@ __global__ void __launch_bounds__(FT) k_pick(Args a) {
 
 // Tokens of a chunk: 4096, 16 of 256 threads, so that few long rows still reach many CUs; 16384 where there are blocks for all of them
 // anyway, or more than 64 chunks otherwise.
+constexpr int SHORT_MOST = 1024;       // most chunks of 4096 tokens in a call
 int chunk_of(int rows, int vocab) {
     const int64_t blocks = static_cast<int64_t>(rows) * ((vocab + 4095) / 4096);
-    return blocks <= 1024 && vocab <= MAXC * 4096 ? 4096 : 16384;
+    return blocks <= SHORT_MOST && vocab <= MAXC * 4096 ? 4096 : 16384;
 }
-size_t workspace(int rows, int vocab) {
-    if (vocab <= ROW_MOST || rows < 1) return 0;
-    const int chunk = chunk_of(rows, vocab), chunks = (vocab + chunk - 1) / chunk;
+size_t bytes_of(int rows, int chunks, int chunk) {
     return static_cast<size_t>(rows) * (static_cast<size_t>(chunks) * ((2 * BINS + 1) * 8 + chunk / 64) + (6 * BINS + CAP) * 8 + sizeof(Record));
+}
+// What a call takes of its workspace.
+size_t need_of(int rows, int vocab) {
+    if (vocab <= ROW_MOST || rows < 1) return 0;
+    const int chunk = chunk_of(rows, vocab);
+    return bytes_of(rows, (vocab + chunk - 1) / chunk, chunk);
+}
+// What suffices for every call of up to so many rows and tokens: fewer or shorter rows may be in smaller chunks, and take more.
+size_t workspace(int rows, int vocab) {
+    size_t most = need_of(rows, vocab);
+    if (most > 0)
+        for (int chunks = ROW_MOST / 4096 + 1; chunks <= std::min(MAXC, (vocab + 4095) / 4096); ++chunks)
+            most = std::max(most, bytes_of(std::min(rows, SHORT_MOST / chunks), chunks, 4096));
+    return most;
 }
 
 template <class T>
@@ -1348,7 +1361,7 @@ navi_status navi_sample_rows(const void *d_logits, int32_t dtype, int32_t ld, in
         set_err(err, errlen, "sample_rows: %d rows of %d tokens are too many for one call", n_rows, vocab);
         return NAVI_ERR_INVALID;
     }
-    const size_t need = sample::workspace(n_rows, vocab);
+    const size_t need = sample::need_of(n_rows, vocab);
     if (need > 0 && (!d_ws || !kv::aligned16(d_ws) || ws_bytes < need)) {
         set_err(err, errlen, "sample_rows: the workspace is null, misaligned or smaller than %zu bytes (%zu)", need, ws_bytes);
         return NAVI_ERR_INVALID;
