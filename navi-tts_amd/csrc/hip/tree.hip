@@ -108,9 +108,11 @@ __device__ __forceinline__ bool any_special(u32x4_t x) {
     return b;
 }
 
-// What the scores of a kv head's keys are multiplied with, and what its sums of V are.
-__device__ __forceinline__ float score_factor(const Args &a, int kvh) { return a.ks ? a.scale * gld(a.ks + kvh) : a.scale; }
-__device__ __forceinline__ float value_factor(const Args &a, int kvh) { return a.vs ? gld(a.vs + kvh) : 1.f; }
+// What the scores of a kv head's keys are multiplied with, and what its sums of V are. P: the pool's elements; only e4m3 has factors.
+template <class P>
+__device__ __forceinline__ float score_factor(const Args &a, int kvh) { return sizeof(P) == 1 && a.ks ? a.scale * gld(a.ks + kvh) : a.scale; }
+template <class P>
+__device__ __forceinline__ float value_factor(const Args &a, int kvh) { return sizeof(P) == 1 && a.vs ? gld(a.vs + kvh) : 1.f; }
 
 // Four consecutive columns of an output row.
 template <class E, bool PAIR>
@@ -506,6 +508,7 @@ struct Rows {
     }
 
     // Row r of the group, columns col ..: stored, or kept as the chunk's part.
+    template <class P>
     static __device__ __forceinline__ void finish(const Args &a, const Share &s, int group_rows, int r, int col, f32x4_t o, float m, float total) {
         const int q = s.group * group_rows + r, j = div_by(a.heads_per, q);
         if (j >= s.at.rows) return;
@@ -517,7 +520,7 @@ struct Rows {
                 gst(a.pm + 2 * at + 1, total);
             }
         } else {
-            store_out<E, PAIR>(a, s.at.c0 + j, (s.kvh * a.g + q - j * a.g) * D + col, a.hkv * a.g * D, o * (m == NONE ? 0.f : value_factor(a, s.kvh) / total));
+            store_out<E, PAIR>(a, s.at.c0 + j, (s.kvh * a.g + q - j * a.g) * D + col, a.hkv * a.g * D, o * (m == NONE ? 0.f : value_factor<P>(a, s.kvh) / total));
         }
     }
 };
@@ -606,7 +609,7 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
     u32x4_t *s_q = reinterpret_cast<u32x4_t *>(sm + W * VB);
     if (wv < NT) {
         v8 q[QP * KS];
-        const float f = R::operands(a, score_factor(a, s.kvh), raw, q);
+        const float f = R::operands(a, score_factor<P>(a, s.kvh), raw, q);
 #pragma unroll
         for (int i = 0; i < QP * KS; ++i) s_q[((i / KS * NT + wv) * KS + i % KS) * WAVE + l] = bits<u32x4_t>(q[i]);
         if (lg == 0) s_fac[wv * 16 + lr] = f;
@@ -721,7 +724,7 @@ __global__ void __launch_bounds__(alone_of(CUT) * WAVE, NT == 1 && CUT ? 3 : 2) 
         }
 #pragma unroll
         for (int w = 0; w < W; ++w) total += s_ref[w][r] == NONE ? 0.f : s_sum[w][r] * __builtin_amdgcn_exp2f(s_ref[w][r] - m);
-        R::finish(a, s, NT * 16, r, c, o, m, total);
+        R::template finish<P>(a, s, NT * 16, r, c, o, m, total);
     }
 }
 
@@ -837,7 +840,7 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
         v8 x[QP * KS];
         typename R::Raw raw;
         R::template fetch<false>(a, s, qrow0 + nt * 16 + lr, raw);
-        rows.fac[nt] = R::operands(a, score_factor(a, s.kvh), raw, x);
+        rows.fac[nt] = R::operands(a, score_factor<P>(a, s.kvh), raw, x);
 #pragma unroll
         for (int i = 0; i < QP * KS; ++i)
             if (i < KS) q[nt][i] = x[i];
@@ -930,13 +933,13 @@ __global__ void __launch_bounds__(waves_of(PAIR, RW) * WAVE, 2) k_tree_rows(Args
             f32x4_t o = rows.acc[nt][d];
 #pragma unroll
             for (int w = 1; w < KW; ++w) o += *reinterpret_cast<f32x4_t *>(js + (((w - 1) * RW + rw) * 32 + nt * 16 + lr) * DP + d * 16 + 4 * lg);
-            R::finish(a, s, RW * 32, rw * 32 + nt * 16 + lr, d * 16 + 4 * lg, o, m[nt], total[nt]);
+            R::template finish<P>(a, s, RW * 32, rw * 32 + nt * 16 + lr, d * 16 + 4 * lg, o, m[nt], total[nt]);
         }
 }
 
 // Joins the parts of the requests that were cut, in their order: a wave takes a query row, D / 8 lanes its
 // columns and the others further parts. Block (request x kv head x group, rows).
-template <class E, bool PAIR, int D>
+template <class E, bool PAIR, class P, int D>
 __global__ void __launch_bounds__(BT) k_tree_join(Args a, int group_rows) {
     constexpr int CL = D / 8, PL = WAVE / CL;
     const int l = threadIdx.x & 63, c = l % CL, pl = l / CL;
@@ -979,7 +982,7 @@ __global__ void __launch_bounds__(BT) k_tree_join(Args a, int group_rows) {
         }
         if (pl == 0) {
             const int mrow = qrow0 + r, j = div_by(a.heads_per, mrow), head = kvh * a.g + mrow - j * a.g;
-            const float inv = top == NONE ? 0.f : value_factor(a, kvh) / sum;
+            const float inv = top == NONE ? 0.f : value_factor<P>(a, kvh) / sum;
             store_out<E, PAIR>(a, wh.c0 + j, head * D + 8 * c, a.hkv * a.g * D, o[0] * inv);
             store_out<E, PAIR>(a, wh.c0 + j, head * D + 8 * c + 4, a.hkv * a.g * D, o[1] * inv);
         }
@@ -1055,7 +1058,7 @@ void launch_as(const Args &a, const Cut &c, hipStream_t s) {
     if (c.workers == 0) return launch_cut<E, PAIR, P, D, false>(a, c, s);
     launch_cut<E, PAIR, P, D, true>(a, c, s);
     const unsigned units = static_cast<unsigned>(a.n) * a.groups * a.hkv;
-    hipLaunchKernelGGL((k_tree_join<E, PAIR, D>), dim3(units, std::max(1u, std::min(static_cast<unsigned>(c.rows / NW), 1024u / units))), dim3(BT), 0, s,
+    hipLaunchKernelGGL((k_tree_join<E, PAIR, P, D>), dim3(units, std::max(1u, std::min(static_cast<unsigned>(c.rows / NW), 1024u / units))), dim3(BT), 0, s,
                        a, c.rows);
 }
 
