@@ -281,7 +281,7 @@ __device__ __forceinline__ uint32_t least_of(const Rule &r, double best4) {
     return least_key((best4 + 4.0 * r.m) * r.inv, [&](float x) { return (static_cast<double>(x) * r.c4 - best4) * 0.25 >= r.m; });
 }
 
-// Adds a token to its bin, if it has one. The instructions are what bounds a pass over a row: 16 a token and its atomic. (The conversion
+// Adds a token to its bin, if it has one. The instructions are what bounds a pass over a row: 15 vector ones a token, four scalar ones and its atomic. (The conversion
 // takes numbers past its range to its ends; so written, since C++ leaves them undefined.)
 struct Adder {
     double c4, top;
@@ -450,7 +450,7 @@ struct Marks {
 
 // Tokens to look at again: keys in LDS, or, where they are too many, all of the row's, SPAN at a time in LDS as the rule sees them (WHOLE: there already).
 // A thread reads back those that it has put there. Rows so flat are slow, since one block goes over all of the row several times: 151936 normal logits with
-// sigma 0.3, of which the largest bin has a quarter, 310 us, 256 such rows 432 (418 and 726 with the logits loaded one by one); all alike 533.
+// sigma 0.3, of which the largest bin has a quarter, 310 us, 256 such rows 430 to 540 (418 and 726 with the logits loaded one by one); all alike 530.
 template <class T, int BATCH, int SPAN, bool WHOLE>
 struct Tokens {
     typedef uint64_t Batch[BATCH];
