@@ -818,8 +818,8 @@ __device__ __forceinline__ void draw(const Args &a, int row, const float *xs, in
             run += w;
         }
     }
-    // the logarithm of a weight is what it was made from
-    put(a, row, pick, static_cast<float>((static_cast<double>(y) * r.c4 - top) * LN - log_total));
+    // the logarithm of a weight is what it was made from; the sum's rounding can put a lone token's above 0
+    put(a, row, pick, fminf(static_cast<float>((static_cast<double>(y) * r.c4 - top) * LN - log_total), 0.f));
 }
 
 __device__ __forceinline__ double number_of(const Args &a, int row) {
