@@ -356,7 +356,8 @@ navi_status navi_kv_append(const navi_kv_pages *pages, const navi_kv_heads *head
 navi_status navi_tree_attention(const navi_kv_pages *pages, const navi_kv_heads *heads, const void *d_q, int32_t q_dtype, int32_t ldq,
                                 const void *d_k, const void *d_v, int32_t ld_kv, float scale, int32_t max_keys, void *d_out,
                                 int32_t ldo, void *d_ws, size_t ws_bytes, void *stream, char *err, size_t errlen);
-/* Workspace bytes of navi_tree_attention (host only; 0 when the work is not split, or the arguments are not valid). */
+/* Workspace bytes of navi_tree_attention with these arguments (host only; 0 when the work is not split, or the arguments are not valid). Not the most
+ * that smaller calls take: fewer requests, rows or keys can be split further. */
 size_t navi_tree_workspace(const navi_kv_pages *pages, const navi_kv_heads *heads, int32_t max_keys);
 /* The accepted rows of each request moved into place in every layer of `kv` (n_layer, max_pos >= the pool's rows, kv_dim the
  * row stride, a multiple of 8; whole strides are moved, so that the layers' K and V must not overlap as n_pages * page_size rows of kv_dim: K
